@@ -99,8 +99,18 @@ class Runtime:
         return v.value
 
 
+class Kv8(ctypes.Structure):
+    """nya_hip_kv8 (include/fyodor_hip_serving.h)."""
+    _fields_ = [("keys", _up), ("values", _up), ("key_scales", _up), ("value_scales", _up), ("pages", _sz),
+                ("page_tokens", _sz), ("kv_heads", _sz), ("width", _sz)]
+
+
+ROPE_INTERLEAVED, ROPE_HALVES = 0, 1
+ROPE_SCALINGS = {"none": 0, "linear": 1, "bands": 2, "ramp": 3}
+
+
 class Kernels:
-    """libfyodor_hip.so (include/fyodor_hip.h)."""
+    """libfyodor_hip.so (include/fyodor_hip.h, include/fyodor_hip_serving.h)."""
 
     def __init__(self, path: Path = KERNEL_LIBRARY):
         if not Path(path).exists():
@@ -119,6 +129,19 @@ class Kernels:
         L.nya_hip_read_shaped.argtypes = [_up, _sz, _up, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _up]
         L.nya_hip_kernel_name.restype = ctypes.c_char_p
         L.nya_hip_kernel_name.argtypes = [_u, _sz, _sz, _sz]
+        cache = ctypes.POINTER(Kv8)
+        L.nya_hip_page_step.argtypes = [_up, _up, _sz, _sz, _up, _sz, _up, _up, _sz, _up, _up, _up, _up, _sz, _up]
+        L.nya_hip_rope_frequencies.argtypes = [_vp, _sz, ctypes.c_double, _vp, _u, ctypes.c_double, ctypes.c_double,
+                                               ctypes.c_double, ctypes.c_double, ctypes.POINTER(ctypes.c_float)]
+        L.nya_hip_rope_angles.argtypes = [_up, _sz, _up, _sz, ctypes.c_float, _up, _up]
+        L.nya_hip_rope.argtypes = [_up, _sz, _up, _sz, _sz, _up, _sz, _up, _sz, _sz, _sz, _sz, _up, _sz, _u, _up]
+        L.nya_hip_kv8_bytes.argtypes = [cache, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]
+        L.nya_hip_kv8_store.argtypes = [cache, _up, _sz, _up, _sz, _up, _sz, _up, _sz, _u, _up, _sz, _up, _sz, _sz,
+                                        _up]
+        L.nya_hip_kv8_load.argtypes = [cache, _up, _sz, _up, _sz, _up, _sz, _up]
+        L.nya_hip_kv8_attention_bytes.argtypes = [cache, _sz, _sz, _sz, _sz, _sz, _sz, ctypes.POINTER(_sz)]
+        L.nya_hip_kv8_attention.argtypes = [cache, _up, _sz, _up, _sz, _sz, _up, _up, _up, _sz, _sz, _sz, _sz, _sz,
+                                            _sz, ctypes.c_float, _up, _sz, _up]
 
     def device_weights(self, w: np.ndarray, type_id: int, rows: int, cols: int) -> np.ndarray:
         """GGUF bytes -> the device layout (host side)."""
@@ -174,6 +197,97 @@ class Kernels:
     def kernel_name(self, type_id: int, rows: int, cols: int, batch: int) -> str:
         name = self.lib.nya_hip_kernel_name(type_id, rows, cols, batch)
         return name.decode() if name else ""
+
+    # ---- serving (include/fyodor_hip_serving.h) ----------------------------
+
+    def page_step(self, lengths: int, counts: int, requests: int, page_tokens: int, table: int, table_stride: int,
+                  held: int, free_pages: int, pages: int, free_count: int, starts: int, positions: int, slots: int,
+                  max_tokens: int, stream: int) -> None:
+        """Pages, rows, positions and cache slots of a step from its requests' lengths."""
+        status = self.lib.nya_hip_page_step(lengths, counts, requests, page_tokens, table, table_stride, held,
+                                            free_pages, pages, free_count, starts, positions, slots, max_tokens, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_page_step returned {status}")
+
+    def rope_frequencies(self, rotated: int, base: float, factors: np.ndarray | None = None, scaling: str = "none",
+                         factor: float = 1.0, original: float = 0.0, low: float = 0.0,
+                         high: float = 0.0) -> tuple[np.ndarray, float]:
+        """(rotated / 2 fp32 frequencies, the magnitude of (cos, sin)), on the host."""
+        out, magnitude = np.empty(max(rotated // 2, 1), np.float32), ctypes.c_float()
+        if factors is not None:
+            factors = np.ascontiguousarray(factors, np.float32)
+            if factors.size != rotated // 2:
+                raise ValueError("factors must hold rotated / 2 floats")
+        if self.lib.nya_hip_rope_frequencies(out.ctypes.data, rotated, base,
+                                             None if factors is None else factors.ctypes.data, ROPE_SCALINGS[scaling],
+                                             factor, original, low, high, ctypes.byref(magnitude)):
+            raise ValueError("nya_hip_rope_frequencies declined")
+        return out, magnitude.value
+
+    def rope_angles(self, positions: int, count: int, frequencies: int, rotated: int, magnitude: float, angles: int,
+                    stream: int) -> None:
+        """(cos, sin) of every position and frequency: what all layers of a step read."""
+        status = self.lib.nya_hip_rope_angles(positions, count, frequencies, rotated, magnitude, angles, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_rope_angles returned {status}")
+
+    def rope(self, q: int, q_stride: int, q_out: int, q_out_stride: int, heads: int, k: int, k_stride: int, k_out: int,
+             k_out_stride: int, kv_heads: int, width: int, count: int, angles: int, rotated: int, layout: int,
+             stream: int) -> None:
+        """The rotary step of q and k rows (k 0: q only)."""
+        status = self.lib.nya_hip_rope(q, q_stride, q_out, q_out_stride, heads, k, k_stride, k_out, k_out_stride,
+                                       kv_heads, width, count, angles, rotated, layout, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_rope returned {status}")
+
+    def kv8(self, keys: int, values: int, key_scales: int, value_scales: int, pages: int, page_tokens: int,
+            kv_heads: int, width: int) -> Kv8:
+        """The 8-bit paged cache at these device addresses."""
+        return Kv8(keys, values, key_scales, value_scales, pages, page_tokens, kv_heads, width)
+
+    def kv8_bytes(self, pages: int, page_tokens: int, kv_heads: int, width: int) -> tuple[int, int]:
+        """Bytes of each code array and of each scale array."""
+        codes, scales = _sz(), _sz()
+        cache = Kv8(0, 0, 0, 0, pages, page_tokens, kv_heads, width)
+        if self.lib.nya_hip_kv8_bytes(ctypes.byref(cache), ctypes.byref(codes), ctypes.byref(scales)):
+            raise ValueError("cache geometry unsupported")
+        return codes.value, scales.value
+
+    def kv8_store(self, cache: Kv8, slots: int, count: int, k: int, k_stride: int, v: int, v_stride: int, angles: int,
+                  rotated: int, layout: int, q: int, q_stride: int, q_out: int, q_out_stride: int, heads: int,
+                  stream: int) -> None:
+        """Rows of k (rotated, with angles) and v into the cache, q rotated into q_out (q 0: none)."""
+        status = self.lib.nya_hip_kv8_store(ctypes.byref(cache), slots, count, k, k_stride, v, v_stride, angles,
+                                            rotated, layout, q, q_stride, q_out, q_out_stride, heads, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_kv8_store returned {status}")
+
+    def kv8_load(self, cache: Kv8, slots: int, count: int, k: int, k_stride: int, v: int, v_stride: int,
+                 stream: int) -> None:
+        """Cache rows back as fp32."""
+        status = self.lib.nya_hip_kv8_load(ctypes.byref(cache), slots, count, k, k_stride, v, v_stride, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_kv8_load returned {status}")
+
+    def kv8_attention_bytes(self, cache: Kv8, count: int, requests: int, max_tokens: int, max_length: int, heads: int,
+                            window: int) -> int:
+        """The workspace with which kv8_attention splits the work as it wants to."""
+        b = _sz()
+        if self.lib.nya_hip_kv8_attention_bytes(ctypes.byref(cache), count, requests, max_tokens, max_length, heads,
+                                                window, ctypes.byref(b)):
+            raise ValueError("request unsupported")
+        return b.value
+
+    def kv8_attention(self, cache: Kv8, q: int, q_stride: int, out: int, out_stride: int, count: int, starts: int,
+                      lengths: int, table: int, table_stride: int, requests: int, max_tokens: int, max_length: int,
+                      heads: int, window: int, scale: float, workspace: int, workspace_bytes: int,
+                      stream: int) -> None:
+        """Causal attention of a step's rows over their requests' pages."""
+        status = self.lib.nya_hip_kv8_attention(ctypes.byref(cache), q, q_stride, out, out_stride, count, starts,
+                                                lengths, table, table_stride, requests, max_tokens, max_length, heads,
+                                                window, scale, workspace, workspace_bytes, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_kv8_attention returned {status}")
 
 
 class Graph:
