@@ -10,10 +10,12 @@ namespace {
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kStep = 64;   // positions per step of a wavefront
-constexpr int kRows = 16;   // query rows per tile
+constexpr int kRows = 16;   // query rows per tile of a few
 constexpr int kWaves = 4;
+constexpr int kWideRows = 32 * kWaves;   // query rows per tile of many
 
 // The positions that a tile of query rows sees and how they are split: steps
 // [begin, end) of 64 positions in `active` shares of `chunk`.
@@ -69,37 +71,53 @@ __device__ __forceinline__ half8 codes_f16(uint32_t lo, uint32_t hi)
     return u.v;
 }
 
-// x as two fp16 pieces, hi + lo = x to 2^-22.
+// x as two fp16 pieces, hi + lo = x to 2^-22; the remainder x - hi is exact.
 __device__ __forceinline__ void split_f16(const float *x, half8 &hi, half8 &lo)
 {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     union { half8 v; half2 p[4]; } h, l;
+    float minus = -1.f;
+    asm("" : "+s"(minus));   // keeps the product: one v_fma_mix_f32 instead of a conversion and a subtraction
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const f32x2 v = {x[2 * i], x[2 * i + 1]};
         h.p[i] = __builtin_convertvector(v, half2);
-        const f32x2 r = {v.x - (float)h.p[i].x, v.y - (float)h.p[i].y};
+        const f32x2 r = {__builtin_fmaf((float)h.p[i].x, minus, v.x), __builtin_fmaf((float)h.p[i].y, minus, v.y)};
         l.p[i] = __builtin_convertvector(r, half2);
     }
     hi = h.v;
     lo = l.v;
 }
 
-// The largest over lanes l, l ^ 16, l ^ 32, l ^ 48.
+// max / sum over lanes l and l ^ 32 (and l ^ 16), in all of them.
+__device__ __forceinline__ float halves_max(float v)
+{
+    const int b = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v)
+{
+    const int b = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]);
+}
 __device__ __forceinline__ float column_max(float v)
 {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const int b = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return halves_max(fmaxf(__builtin_bit_cast(float, (int)r[0]), __builtin_bit_cast(float, (int)r[1])));
 }
 __device__ __forceinline__ float column_sum(float v)
 {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    const int b = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return halves_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
 }
 
 template <int W>
 __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Attention a, int splits, int least,
-    float *__restrict__ partials)
+    int most_rows, float *__restrict__ partials)
 {
     constexpr int C = W / 64, D = W / 16;
     const Kv8 &c = a.cache;
@@ -111,7 +129,7 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     x /= c.kv_heads;
     const int sp = x % splits, tile = x / splits;
     const Request rq = request_of(a, r);
-    if (kRows * tile >= rq.rows) return;
+    if (kRows * tile >= rq.rows || rq.rows > most_rows) return;
     const Range g = range_of(a, rq, tile, kRows, splits, least);
     if (sp >= g.active) return;
 
@@ -287,17 +305,282 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     }
 }
 
+// Many rows of one request: 32 per wavefront, 128 per workgroup, whose
+// wavefronts share every step's keys and values, converted to fp16 in LDS once.
+template <int W>
+__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_wide(Kv8Attention a, int splits, int most_rows,
+    float *__restrict__ partials)
+{
+    constexpr int M = W / 16;       // MFMA steps of a score
+    constexpr int D = W / 32;       // output tiles
+    constexpr int N = W / 64;       // 16-byte pieces of K, and of V, per thread and step
+    constexpr int kBytes = 2 * kStep * W;
+    __shared__ __align__(16) uint8_t smem[2][2][kBytes];   // [buffer][K, V]
+    __shared__ float2 scales[2][4];
+    const Kv8 &c = a.cache;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, h = lane >> 5;
+    const int group = a.heads / c.kv_heads, r = blockIdx.y;
+    int x = blockIdx.x;
+    const int kvh = x % c.kv_heads;
+    x /= c.kv_heads;
+    const int sp = x % splits;
+    const Request rq = request_of(a, r);
+    // Later tokens see more: their tiles first.
+    const int tile = (rq.rows + kWideRows - 1) / kWideRows - 1 - x / splits;
+    if (tile < 0 || rq.rows <= most_rows) return;
+    const Range g = range_of(a, rq, tile, kWideRows, splits, 1);
+    if (sp >= g.active) return;
+
+    const int row = kWideRows * tile + 32 * wave + col, row_in = min(row, rq.rows - 1), token = row_in / group;
+    const int head = kvh * group + row_in % group;
+    const int64_t p = rq.first + token;
+    const int last = row < rq.rows ? (int)(p < g.highest ? p : g.highest) : -1;
+    const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
+    // What the wavefront's rows see: any of [low, high], all of [all_from, high_all].
+    int low = last < 0 ? INT32_MAX : first, high = last, all_from = first, all_to = last;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        low = min(low, __shfl_xor(low, o, 64));
+        high = max(high, __shfl_xor(high, o, 64));
+        all_from = max(all_from, __shfl_xor(all_from, o, 64));
+        all_to = min(all_to, __shfl_xor(all_to, o, 64));
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    high = __builtin_amdgcn_readfirstlane(high);
+    all_from = __builtin_amdgcn_readfirstlane(all_from);
+    all_to = __builtin_amdgcn_readfirstlane(all_to);
+
+    half8 qh[M], ql[M];
+    float qscale;
+    {
+        const float *q = a.q + (rq.begin + token) * a.q_stride + (int64_t)head * W + 8 * h;
+        const bool aligned = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 4 == 0;
+        float v[8 * M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            if (aligned) {
+                *(float4 *)(v + 8 * i) = *(const float4 *)(q + 16 * i);
+                *(float4 *)(v + 8 * i + 4) = *(const float4 *)(q + 16 * i + 4);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * i + e] = q[16 * i + e];
+            }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8 * M; ++i) top = fmaxf(top, fabsf(v[i]));
+        const int e = 14 - __builtin_amdgcn_frexp_expf(halves_max(top));
+#pragma unroll
+        for (int i = 0; i < 8 * M; ++i) v[i] = ldexpf(v[i], e);
+#pragma unroll
+        for (int i = 0; i < M; ++i) split_f16(v + 8 * i, qh[i], ql[i]);
+        qscale = ldexpf(a.scale * 1.44269504f, -e);
+    }
+
+    const int *table = a.table + (size_t)r * a.table_stride;
+    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
+    const int begin = g.begin + sp * g.chunk, stop = min(begin + g.chunk, g.end);
+    auto page_of = [&](int at) {
+        const int j = at >> shift;
+        int page = -1;
+        if (at <= g.highest && j < a.table_stride) page = table[j];
+        return (unsigned)page < (unsigned)c.pages ? page : -1;
+    };
+    auto place_of = [&](int page) { return (size_t)max(page, 0) * c.kv_heads + kvh; };
+    const size_t plane = (size_t)c.page_tokens * W;
+    // A step's codes on their way to LDS: thread piece i of K is dims
+    // 16 (wave + 4 i).. of position `lane`, of V dim (tid + 256 i) % W of granule
+    // (tid + 256 i) / W.
+    uint4 kreg[N], vreg[N];
+    float2 sreg;
+    auto fetch = [&](int step) {
+        const int at = kStep * step, kat = at + lane;
+        const int8_t *kb = c.keys + place_of(page_of(at + (lane & 48))) * plane + (wave * c.page_tokens + (kat & within)) * 16;
+#pragma unroll
+        for (int i = 0; i < N; ++i) kreg[i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = tid + 256 * i, vat = at + 16 * (piece / W);
+            const int8_t *vb = c.values + place_of(page_of(vat)) * plane + ((vat & within) * W + 16 * (piece % W));
+            vreg[i] = *(const uint4 *)vb;
+        }
+        if (tid < 4) {
+            const int page = page_of(at + 16 * tid);
+            sreg = make_float2(0.f, -1.f);   // a value scale below 0: nothing there
+            if (page >= 0) sreg = make_float2(c.key_scales[place_of(page)], fabsf(c.value_scales[place_of(page)]));
+        }
+    };
+    auto stage = [&](int buffer) {
+        uint8_t *ks = smem[buffer][0], *vs = smem[buffer][1];
+        const int t = lane & 31, rho = 8 * ((t & 15) >> 2) + 4 * (t >> 4) + (t & 3);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            uint8_t *to = ks + (((lane >> 5) * M + wave + 4 * i) * 64 + rho) * 16;
+            *(half8 *)to = codes_f16(kreg[i].x, kreg[i].y);
+            *(half8 *)(to + 512) = codes_f16(kreg[i].z, kreg[i].w);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = tid + 256 * i, granule = piece / W, d = piece % W;
+            uint8_t *to = vs + ((((granule >> 1) * D + (d >> 5)) * 2) * 64 + 32 * (granule & 1) + (d & 31)) * 16;
+            *(half8 *)to = codes_f16(vreg[i].x, vreg[i].y);
+            *(half8 *)(to + 1024) = codes_f16(vreg[i].z, vreg[i].w);
+        }
+        if (tid < 4) scales[buffer][tid] = sreg;
+    };
+
+    f32x16 O[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) O[d] = (f32x16){};
+    float m = -INFINITY, l = 0.f;
+    if (begin < stop) {
+        fetch(begin);
+        stage(0);
+        if (begin + 1 < stop) fetch(begin + 1);
+    }
+    __syncthreads();
+    for (int step = begin; step < stop; ++step) {
+        const int buffer = (step - begin) & 1, at = kStep * step;
+        const bool active = at <= high && at + kStep - 1 >= low;
+        f32x16 S[2];
+        if (active) {
+            const uint8_t *ks = smem[buffer][0] + 16 * lane;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) S[t] = (f32x16){};
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const half8 k = *(const half8 *)(ks + (t * M + i) * 1024);
+                    S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], S[t], 0, 0, 0);
+                    S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i], S[t], 0, 0, 0);
+                }
+        }
+        if (step + 1 < stop) {
+            stage(buffer ^ 1);
+            if (step + 2 < stop) fetch(step + 2);
+        }
+        if (active) {
+            const bool whole = all_from <= at && all_to >= at + kStep - 1;
+            float scale[2], mant[2], top = -INFINITY;
+            int e[2];
+            bool there[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float2 s = scales[buffer][2 * t + h];
+                there[t] = !(s.y < 0.f);
+                scale[t] = __builtin_isfinite(s.x) ? s.x * qscale : NAN;
+                e[t] = __builtin_amdgcn_frexp_expf(s.y);
+                mant[t] = __builtin_isfinite(s.y) ? __builtin_amdgcn_frexp_mantf(s.y) : NAN;
+            }
+            const bool masked = !whole || __builtin_amdgcn_ballot_w64(!there[0] || !there[1]);
+            uint32_t seen[2] = {0xFFFFu, 0xFFFFu};
+            if (masked) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int from = max(first - (at + 32 * t + 16 * h), 0), to = min(last - (at + 32 * t + 16 * h), 15);
+                    seen[t] = there[t] && from <= to ? (0xFFFFu >> (15 - to)) & (0xFFFFu << from) : 0;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float best = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float s = S[t][i] * scale[t];
+                    best = fmaxf(best, !masked || (seen[t] >> i & 1) ? s : -INFINITY);
+                }
+                top = fmaxf(top, best + e[t]);
+            }
+            if (__builtin_amdgcn_ballot_w64(top > m)) {
+                const float next = fmaxf(m, ceilf(halves_max(top)));
+                const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+                m = next;
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < D; ++d) O[d] *= alpha;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            half8 ph[2][2], pl[2][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float w[16], sum[2] = {0.f, 0.f};
+                const float add = e[t] - base + 15.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i], scale[t], add)), weight = v * mant[t];
+                    if (masked && !(seen[t] >> i & 1)) v = weight = 0.f;
+                    sum[i & 1] += v;
+                    w[i] = weight;
+                }
+                l += ldexpf(sum[0] + sum[1], -e[t]);
+                split_f16(w, ph[t][0], pl[t][0]);
+                split_f16(w + 8, ph[t][1], pl[t][1]);
+            }
+            const uint8_t *vs = smem[buffer][1] + 16 * lane;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int d = 0; d < D; ++d) {
+                        const half8 v = *(const half8 *)(vs + ((t * D + d) * 2 + u) * 1024);
+                        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t][u], O[d], 0, 0, 0);
+                        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[t][u], O[d], 0, 0, 0);
+                    }
+        }
+        __syncthreads();
+    }
+    l = halves_sum(l);
+    if (row >= rq.rows) return;
+    if (g.active > 1) {
+        const size_t prow = ((size_t)r * a.max_tokens * group + row) * c.kv_heads + kvh;
+        float *to = partials + (prow * splits + sp) * W + 4 * h;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(float4 *)(to + 32 * d + 8 * i) = make_float4(O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]);
+        if (h == 0) {
+            float *pm = partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * (prow * splits + sp);
+            pm[0] = m;
+            pm[1] = l;
+        }
+        return;
+    }
+    float *out = a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W + 4 * h;
+    const float inverse = l == 0.f ? 0.f : 1.f / l;
+    const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 o = make_float4(O[d][4 * i] * inverse, O[d][4 * i + 1] * inverse, O[d][4 * i + 2] * inverse,
+                                         O[d][4 * i + 3] * inverse);
+            if (aligned) {
+                *(float4 *)(out + 32 * d + 8 * i) = o;
+            } else {
+                out[32 * d + 8 * i] = o.x;
+                out[32 * d + 8 * i + 1] = o.y;
+                out[32 * d + 8 * i + 2] = o.z;
+                out[32 * d + 8 * i + 3] = o.w;
+            }
+        }
+}
+
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over a row's shares.
 // Workgroup (row of a KV head and request).
 template <int W>
 __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, int splits, int least,
-    const float *__restrict__ partials)
+    int most_rows, const float *__restrict__ partials)
 {
     const Kv8 &c = a.cache;
     const int group = a.heads / c.kv_heads, r = blockIdx.y, kvh = blockIdx.x % c.kv_heads, row = blockIdx.x / c.kv_heads;
     const Request rq = request_of(a, r);
     if (row >= rq.rows) return;
-    const Range g = range_of(a, rq, row / kRows, kRows, splits, least);
+    const int rows = rq.rows > most_rows ? kWideRows : kRows;
+    const Range g = range_of(a, rq, row / rows, rows, splits, rows == kRows ? least : 1);
     if (g.active <= 1) return;
     const size_t prow = ((size_t)r * a.max_tokens * group + row) * c.kv_heads + kvh;
     const float *pm = partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * prow * splits;
@@ -325,23 +608,28 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, int splits, int 
 }
 
 // How the work is split: `splits` workgroups at most share a tile's
-// positions, at least `least` steps each.
+// positions, in tiles of a few rows at least `least` steps each; requests of
+// more than most_rows rows (of one KV head) run in wide tiles.
 struct Plan {
-    int splits, least;
+    int splits, least, most_rows;
 };
 
-Plan plan_of(int requests, int max_tokens, int max_length, int heads, int kv_heads, int window)
+Plan plan_of(int requests, int max_tokens, int max_length, int heads, int kv_heads, int width, int window)
 {
-    const int64_t tiles = ((int64_t)max_tokens * (heads / kv_heads) + kRows - 1) / kRows;
-    const int64_t groups = tiles * kv_heads * requests;
+    const int64_t rows = (int64_t)max_tokens * (heads / kv_heads);
+    Plan p = {1, kWaves, INT32_MAX};
+    if (width <= 256 && rows > 32) p.most_rows = requests == 1 ? 0 : 32;
+    const int tile = rows > p.most_rows ? kWideRows : kRows;
+    const int64_t groups = (rows + tile - 1) / tile * kv_heads * requests;
     int64_t range = max_length;
     if (window && (int64_t)window + max_tokens < range) range = (int64_t)window + max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    int64_t splits = (1024 + groups - 1) / groups;
+    const int64_t wanted = tile == kRows ? 1024 : 512, least = tile == kRows ? kWaves : 4;
+    int64_t splits = wanted / groups;
     if (splits > 64) splits = 64;
-    if (splits > (steps + kWaves - 1) / kWaves) splits = (steps + kWaves - 1) / kWaves;
-    if (splits < 1) splits = 1;
-    return {(int)splits, kWaves};
+    if (splits > steps / least) splits = steps / least;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    return p;
 }
 
 size_t row_bytes(int requests, int max_tokens, int heads, int width)
@@ -352,13 +640,22 @@ size_t row_bytes(int requests, int max_tokens, int heads, int width)
 template <int W>
 hipError_t launch_rows(const Kv8Attention &a, Plan p, float *partials, hipStream_t s)
 {
-    const int group = a.heads / a.cache.kv_heads;
-    const int64_t tiles = ((int64_t)a.max_tokens * group + kRows - 1) / kRows;
-    hipLaunchKernelGGL((kv8_rows<W>), dim3((unsigned)(tiles * p.splits * a.cache.kv_heads), (unsigned)a.requests),
-                       dim3(64 * kWaves), 0, s, a, p.splits, p.least, partials);
+    const int64_t rows = (int64_t)a.max_tokens * (a.heads / a.cache.kv_heads);
+    const int64_t each = (int64_t)p.splits * a.cache.kv_heads;
+    if (p.most_rows) {
+        const int64_t most = rows < p.most_rows ? rows : p.most_rows;
+        hipLaunchKernelGGL((kv8_rows<W>), dim3((unsigned)((most + kRows - 1) / kRows * each), (unsigned)a.requests),
+                           dim3(64 * kWaves), 0, s, a, p.splits, p.least, p.most_rows, partials);
+    }
+    if constexpr (W <= 256) {
+        if (rows > p.most_rows)
+            hipLaunchKernelGGL((kv8_wide<W>), dim3((unsigned)((rows + kWideRows - 1) / kWideRows * each),
+                                                   (unsigned)a.requests),
+                               dim3(64 * kWaves), 0, s, a, p.splits, p.most_rows, partials);
+    }
     if (p.splits > 1)
         hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)(a.max_tokens * a.heads), (unsigned)a.requests), dim3(256), 0,
-                           s, a, p.splits, p.least, partials);
+                           s, a, p.splits, p.least, p.most_rows, partials);
     return hipGetLastError();
 }
 
@@ -367,13 +664,13 @@ hipError_t launch_rows(const Kv8Attention &a, Plan p, float *partials, hipStream
 size_t kv8_attention_workspace(int requests, int max_tokens, int max_length, int heads, int kv_heads, int width,
     int window)
 {
-    const Plan p = plan_of(requests, max_tokens, max_length, heads, kv_heads, window);
+    const Plan p = plan_of(requests, max_tokens, max_length, heads, kv_heads, width, window);
     return p.splits > 1 ? p.splits * row_bytes(requests, max_tokens, heads, width) : 0;
 }
 
 hipError_t launch_kv8_attention(const Kv8Attention &a, void *workspace, size_t workspace_bytes, hipStream_t s)
 {
-    Plan p = plan_of(a.requests, a.max_tokens, a.max_length, a.heads, a.cache.kv_heads, a.window);
+    Plan p = plan_of(a.requests, a.max_tokens, a.max_length, a.heads, a.cache.kv_heads, a.cache.width, a.window);
     const size_t each = row_bytes(a.requests, a.max_tokens, a.heads, a.cache.width);
     if (workspace_bytes / each < (size_t)p.splits) p.splits = (int)(workspace_bytes / each);
     if (p.splits < 1) p.splits = 1;
