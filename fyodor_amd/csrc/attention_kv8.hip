@@ -305,30 +305,76 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     }
 }
 
-// Many rows of one request: 32 per wavefront, 128 per workgroup, whose
-// wavefronts share every step's keys and values, converted to fp16 in LDS once.
-template <int W>
-__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_wide(Kv8Attention a, int splits, int most_rows,
-    float *__restrict__ partials)
+// LDS writes and reads of the workgroup up to here; global loads stay in flight.
+__device__ __forceinline__ void lds_barrier()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The request and the tile of number `index` over the requests that run in
+// wide tiles, in order (request < 0: past the last). Later tokens see more:
+// a request's last tile comes first.
+struct TileOf {
+    int request, tile;
+};
+
+__device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, int index)
+{
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.requests; base += 64) {
+        const int r = base + lane, rows = r < a.requests ? request_of(a, r).rows : 0;
+        const int tiles = rows > most_rows ? (rows + kWideRows - 1) / kWideRows : 0;
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(sum > index);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            return {base + at, __builtin_amdgcn_readlane(sum, at) - 1 - index};
+        }
+        index -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return {-1, 0};
+}
+
+// Many rows of one request: 32 per wavefront, 128 per group of four
+// wavefronts, which share every step's keys and values, converted to fp16 in
+// LDS once. KS groups take every KS-th step of the same rows and meet at the
+// end. Two groups run half a step apart: while one is in its MFMAs (last
+// step's outputs, this step's scores) the other does its softmax and stages
+// its next codes, so that the matrix cores of a SIMD always have one of its two
+// wavefronts.
+template <int W, int KS>
+__global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
+void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ partials)
 {
     constexpr int M = W / 16;       // MFMA steps of a score
     constexpr int D = W / 32;       // output tiles
     constexpr int N = W / 64;       // 16-byte pieces of K, and of V, per thread and step
     constexpr int kBytes = 2 * kStep * W;
-    __shared__ __align__(16) uint8_t smem[2][2][kBytes];   // [buffer][K, V]
-    __shared__ float2 scales[2][4];
+    __shared__ __align__(16) uint8_t smem[KS][2][kBytes];   // [group][K, V]
+    __shared__ float2 scales[KS][2][4];
+    __shared__ float2 smem_ml[4][32];
     const Kv8 &c = a.cache;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
+    const int ks = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), tid = threadIdx.x & 255;
     const int col = lane & 31, h = lane >> 5;
-    const int group = a.heads / c.kv_heads, r = blockIdx.y;
+    const int group = a.heads / c.kv_heads;
     int x = blockIdx.x;
     const int kvh = x % c.kv_heads;
     x /= c.kv_heads;
     const int sp = x % splits;
+    const TileOf at_tile = tile_of(a, most_rows, x / splits);
+    const int r = at_tile.request, tile = at_tile.tile;
+    if (r < 0) return;
     const Request rq = request_of(a, r);
-    // Later tokens see more: their tiles first.
-    const int tile = (rq.rows + kWideRows - 1) / kWideRows - 1 - x / splits;
-    if (tile < 0 || rq.rows <= most_rows) return;
     const Range g = range_of(a, rq, tile, kWideRows, splits, 1);
     if (sp >= g.active) return;
 
@@ -337,19 +383,86 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_wide(Kv8Att
     const int64_t p = rq.first + token;
     const int last = row < rq.rows ? (int)(p < g.highest ? p : g.highest) : -1;
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
-    // What the wavefront's rows see: any of [low, high], all of [all_from, high_all].
-    int low = last < 0 ? INT32_MAX : first, high = last, all_from = first, all_to = last;
+    // Positions that all of the wavefront's rows see.
+    int all_from = first, all_to = last;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        low = min(low, __shfl_xor(low, o, 64));
-        high = max(high, __shfl_xor(high, o, 64));
         all_from = max(all_from, __shfl_xor(all_from, o, 64));
         all_to = min(all_to, __shfl_xor(all_to, o, 64));
     }
-    low = __builtin_amdgcn_readfirstlane(low);
-    high = __builtin_amdgcn_readfirstlane(high);
     all_from = __builtin_amdgcn_readfirstlane(all_from);
     all_to = __builtin_amdgcn_readfirstlane(all_to);
+
+    const int *table = a.table + (size_t)r * a.table_stride;
+    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
+    // This group's steps: begin, begin + KS, ...
+    const int begin = g.begin + sp * g.chunk + ks, stop = min(g.begin + (sp + 1) * g.chunk, g.end);
+    const int rounds = (stop - (begin - ks) + KS - 1) / KS;   // the same for every group
+    // Table entries are read a round before the codes they lead to, and
+    // everything unconditionally (positions past the last one lead to page 0):
+    // loads under a condition would be waited for where it ends.
+    const int until = min(g.highest, kStep * stop - 1);   // this workgroup's last position
+    auto entry_of = [&](int at) {
+        const int entry = table[min(at >> shift, a.table_stride - 1)];
+        return at <= until ? entry : -1;
+    };
+    auto place_of = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + kvh; };
+    const size_t plane = (size_t)c.page_tokens * W;
+    int kpage, vpage[N], spage;
+    auto look_k = [&](int step) {
+        kpage = entry_of(kStep * step + (lane & 48));
+        spage = entry_of(kStep * step + 16 * (tid & 3));
+    };
+    auto look_v = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) vpage[i] = entry_of(kStep * step + 16 * ((tid + 256 * i) / W));
+    };
+    // Codes on their way to LDS: this thread's piece i of K is dims
+    // 16 (wave + 4 i).. of position `lane` of the step, of V dim
+    // (tid + 256 i) % W of granule (tid + 256 i) / W.
+    uint4 kreg[N], vreg[N];
+    float2 sreg;
+    bool sthere;
+    auto fetch_k = [&](int step) {
+        const int8_t *kb = c.keys + place_of(kpage) * plane + (wave * c.page_tokens + ((kStep * step + lane) & within)) * 16;
+#pragma unroll
+        for (int i = 0; i < N; ++i) kreg[i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i);
+        sreg = make_float2(c.key_scales[place_of(spage)], c.value_scales[place_of(spage)]);
+        sthere = (unsigned)spage < (unsigned)c.pages;
+    };
+    auto fetch_v = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = tid + 256 * i, vat = kStep * step + 16 * (piece / W);
+            const int8_t *vb = c.values + place_of(vpage[i]) * plane + ((vat & within) * W + 16 * (piece % W));
+            vreg[i] = *(const uint4 *)vb;
+        }
+    };
+    uint8_t *const ksm = smem[ks][0], *const vsm = smem[ks][1];
+    auto stage_k = [&](int buffer) {
+        const int t = lane & 31, rho = 8 * ((t & 15) >> 2) + 4 * (t >> 4) + (t & 3);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            uint8_t *to = ksm + (((lane >> 5) * M + wave + 4 * i) * 64 + rho) * 16;
+            *(half8 *)to = codes_f16(kreg[i].x, kreg[i].y);
+            *(half8 *)(to + 512) = codes_f16(kreg[i].z, kreg[i].w);
+        }
+        // A value scale below 0: nothing there.
+        if (tid < 4) scales[ks][buffer][tid] = make_float2(sreg.x, sthere ? fabsf(sreg.y) : -1.f);
+    };
+    auto stage_v = [&]() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = tid + 256 * i, granule = piece / W, d = piece % W;
+            uint8_t *to = vsm + ((((granule >> 1) * D + (d >> 5)) * 2) * 64 + 32 * (granule & 1) + (d & 31)) * 16;
+            *(half8 *)to = codes_f16(vreg[i].x, vreg[i].y);
+            *(half8 *)(to + 1024) = codes_f16(vreg[i].z, vreg[i].w);
+        }
+    };
+    look_k(begin);
+    fetch_k(begin);
+    look_v(begin);
+    look_k(begin + KS);
 
     half8 qh[M], ql[M];
     float qscale;
@@ -372,167 +485,169 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_wide(Kv8Att
         for (int i = 0; i < 8 * M; ++i) top = fmaxf(top, fabsf(v[i]));
         const int e = 14 - __builtin_amdgcn_frexp_expf(halves_max(top));
 #pragma unroll
-        for (int i = 0; i < 8 * M; ++i) v[i] = ldexpf(v[i], e);
+        for (int i = 0; i < 8 * M; ++i) v[i] = ldexpf(a.scale < 0.f ? -v[i] : v[i], e);
 #pragma unroll
         for (int i = 0; i < M; ++i) split_f16(v + 8 * i, qh[i], ql[i]);
-        qscale = ldexpf(a.scale * 1.44269504f, -e);
+        qscale = ldexpf(fabsf(a.scale) * 1.44269504f, -e);
     }
-
-    const int *table = a.table + (size_t)r * a.table_stride;
-    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
-    const int begin = g.begin + sp * g.chunk, stop = min(begin + g.chunk, g.end);
-    auto page_of = [&](int at) {
-        const int j = at >> shift;
-        int page = -1;
-        if (at <= g.highest && j < a.table_stride) page = table[j];
-        return (unsigned)page < (unsigned)c.pages ? page : -1;
-    };
-    auto place_of = [&](int page) { return (size_t)max(page, 0) * c.kv_heads + kvh; };
-    const size_t plane = (size_t)c.page_tokens * W;
-    // A step's codes on their way to LDS: thread piece i of K is dims
-    // 16 (wave + 4 i).. of position `lane`, of V dim (tid + 256 i) % W of granule
-    // (tid + 256 i) / W.
-    uint4 kreg[N], vreg[N];
-    float2 sreg;
-    auto fetch = [&](int step) {
-        const int at = kStep * step, kat = at + lane;
-        const int8_t *kb = c.keys + place_of(page_of(at + (lane & 48))) * plane + (wave * c.page_tokens + (kat & within)) * 16;
-#pragma unroll
-        for (int i = 0; i < N; ++i) kreg[i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int piece = tid + 256 * i, vat = at + 16 * (piece / W);
-            const int8_t *vb = c.values + place_of(page_of(vat)) * plane + ((vat & within) * W + 16 * (piece % W));
-            vreg[i] = *(const uint4 *)vb;
-        }
-        if (tid < 4) {
-            const int page = page_of(at + 16 * tid);
-            sreg = make_float2(0.f, -1.f);   // a value scale below 0: nothing there
-            if (page >= 0) sreg = make_float2(c.key_scales[place_of(page)], fabsf(c.value_scales[place_of(page)]));
-        }
-    };
-    auto stage = [&](int buffer) {
-        uint8_t *ks = smem[buffer][0], *vs = smem[buffer][1];
-        const int t = lane & 31, rho = 8 * ((t & 15) >> 2) + 4 * (t >> 4) + (t & 3);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            uint8_t *to = ks + (((lane >> 5) * M + wave + 4 * i) * 64 + rho) * 16;
-            *(half8 *)to = codes_f16(kreg[i].x, kreg[i].y);
-            *(half8 *)(to + 512) = codes_f16(kreg[i].z, kreg[i].w);
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int piece = tid + 256 * i, granule = piece / W, d = piece % W;
-            uint8_t *to = vs + ((((granule >> 1) * D + (d >> 5)) * 2) * 64 + 32 * (granule & 1) + (d & 31)) * 16;
-            *(half8 *)to = codes_f16(vreg[i].x, vreg[i].y);
-            *(half8 *)(to + 1024) = codes_f16(vreg[i].z, vreg[i].w);
-        }
-        if (tid < 4) scales[buffer][tid] = sreg;
-    };
-
-    f32x16 O[D];
+    f32x16 O[D], S[2];
 #pragma unroll
     for (int d = 0; d < D; ++d) O[d] = (f32x16){};
+    half8 ph[2][2], pl[2][2];
     float m = -INFINITY, l = 0.f;
-    if (begin < stop) {
-        fetch(begin);
-        stage(0);
-        if (begin + 1 < stop) fetch(begin + 1);
-    }
-    __syncthreads();
-    for (int step = begin; step < stop; ++step) {
-        const int buffer = (step - begin) & 1, at = kStep * step;
-        const bool active = at <= high && at + kStep - 1 >= low;
-        f32x16 S[2];
-        if (active) {
-            const uint8_t *ks = smem[buffer][0] + 16 * lane;
+    auto outputs = [&]() {
+        const uint8_t *vs = vsm + 16 * lane;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) S[t] = (f32x16){};
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < M; ++i)
+            for (int u = 0; u < 2; ++u) {
+                half8 v[D];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const half8 k = *(const half8 *)(ks + (t * M + i) * 1024);
-                    S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], S[t], 0, 0, 0);
-                    S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i], S[t], 0, 0, 0);
-                }
+                for (int d = 0; d < D; ++d) v[d] = *(const half8 *)(vs + ((t * D + d) * 2 + u) * 1024);
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph[t][u], O[d], 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[t][u], O[d], 0, 0, 0);
+            }
+    };
+    auto scores = [&]() {
+        const uint8_t *kp = ksm + 16 * lane;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) S[t] = (f32x16){};
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            const half8 k0 = *(const half8 *)(kp + j * 1024), k1 = *(const half8 *)(kp + (M + j) * 1024);
+            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[j], S[0], 0, 0, 0);
+            S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[j], S[1], 0, 0, 0);
+            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[j], S[0], 0, 0, 0);
+            S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[j], S[1], 0, 0, 0);
         }
-        if (step + 1 < stop) {
-            stage(buffer ^ 1);
-            if (step + 2 < stop) fetch(step + 2);
+    };
+    // Between the MFMAs: softmax of the scores, the last codes into LDS.
+    auto between = [&](int step, int buffer) {
+        stage_v();
+        stage_k(buffer ^ 1);
+        const int at = kStep * step;
+        const bool whole = all_from <= at && all_to >= at + kStep - 1;
+        float scale[2], mant[2];
+        int e[2];
+        bool there[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const float2 s = scales[ks][buffer][2 * t + h];
+            there[t] = !(s.y < 0.f);
+            const bool fine = __builtin_isfinite(s.x) && __builtin_isfinite(s.y);
+            // Above 0, so that it keeps minus infinity. A page that reads as
+            // NaN makes the rows that see it NaN by their sum alone.
+            scale[t] = fine ? fmaxf(fabsf(s.x) * qscale, 0x1p-126f) : 1.f;
+            e[t] = fine ? __builtin_amdgcn_frexp_expf(s.y) : 0;
+            mant[t] = fine ? __builtin_amdgcn_frexp_mantf(s.y) : 1.f;
+            const int pos = at + 32 * t + 16 * h;
+            if (there[t] && !fine && first <= pos + 15 && last >= pos) l = NAN;
         }
-        if (active) {
-            const bool whole = all_from <= at && all_to >= at + kStep - 1;
-            float scale[2], mant[2], top = -INFINITY;
-            int e[2];
-            bool there[2];
+        if (!whole || __builtin_amdgcn_ballot_w64(!there[0] || !there[1])) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float2 s = scales[buffer][2 * t + h];
-                there[t] = !(s.y < 0.f);
-                scale[t] = __builtin_isfinite(s.x) ? s.x * qscale : NAN;
-                e[t] = __builtin_amdgcn_frexp_expf(s.y);
-                mant[t] = __builtin_isfinite(s.y) ? __builtin_amdgcn_frexp_mantf(s.y) : NAN;
+                const int from = max(first - (at + 32 * t + 16 * h), 0), to = min(last - (at + 32 * t + 16 * h), 15);
+                const uint32_t seen = there[t] && from <= to ? (0xFFFFu >> (15 - to)) & (0xFFFFu << from) : 0;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) S[t][n] = seen >> n & 1 ? S[t][n] : -INFINITY;
             }
-            const bool masked = !whole || __builtin_amdgcn_ballot_w64(!there[0] || !there[1]);
-            uint32_t seen[2] = {0xFFFFu, 0xFFFFu};
-            if (masked) {
+        }
+        float top = -INFINITY;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int from = max(first - (at + 32 * t + 16 * h), 0), to = min(last - (at + 32 * t + 16 * h), 15);
-                    seen[t] = there[t] && from <= to ? (0xFFFFu >> (15 - to)) & (0xFFFFu << from) : 0;
-                }
-            }
+        for (int t = 0; t < 2; ++t) {
+            float best = S[t][0];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                float best = -INFINITY;
+            for (int n = 1; n < 16; ++n) best = fmaxf(best, S[t][n]);
+            top = fmaxf(top, best * scale[t] + e[t]);
+        }
+        if (__builtin_amdgcn_ballot_w64(top > m)) {
+            const float next = fmaxf(m, ceilf(halves_max(top)));
+            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= alpha;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float s = S[t][i] * scale[t];
-                    best = fmaxf(best, !masked || (seen[t] >> i & 1) ? s : -INFINITY);
-                }
-                top = fmaxf(top, best + e[t]);
-            }
-            if (__builtin_amdgcn_ballot_w64(top > m)) {
-                const float next = fmaxf(m, ceilf(halves_max(top)));
-                const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
-                m = next;
-                l *= alpha;
+            for (int d = 0; d < D; ++d) O[d] *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                for (int d = 0; d < D; ++d) O[d] *= alpha;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            half8 ph[2][2], pl[2][2];
+        for (int t = 0; t < 2; ++t) {
+            float sum[2] = {0.f, 0.f};
+            const float add = e[t] - base + 15.f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                float w[16], sum[2] = {0.f, 0.f};
-                const float add = e[t] - base + 15.f;
+            for (int n = 0; n < 16; n += 8) {
+                float w[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][i], scale[t], add)), weight = v * mant[t];
-                    if (masked && !(seen[t] >> i & 1)) v = weight = 0.f;
+                for (int i = 0; i < 8; ++i) {
+                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][n + i], scale[t], add));
                     sum[i & 1] += v;
-                    w[i] = weight;
+                    w[i] = v * mant[t];
                 }
-                l += ldexpf(sum[0] + sum[1], -e[t]);
-                split_f16(w, ph[t][0], pl[t][0]);
-                split_f16(w + 8, ph[t][1], pl[t][1]);
+                split_f16(w, ph[t][n / 8], pl[t][n / 8]);
             }
-            const uint8_t *vs = smem[buffer][1] + 16 * lane;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int d = 0; d < D; ++d) {
-                        const half8 v = *(const half8 *)(vs + ((t * D + d) * 2 + u) * 1024);
-                        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t][u], O[d], 0, 0, 0);
-                        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[t][u], O[d], 0, 0, 0);
-                    }
+            l += ldexpf(sum[0] + sum[1], -e[t]);
         }
+    };
+    // The next codes set out before the MFMAs and are there after them. A
+    // round past the group's last step is one of positions that are not there.
+    auto ahead = [&](int step) {
+        fetch_k(step + KS);
+        fetch_v(step);
+        look_v(step + KS);
+        look_k(step + 2 * KS);
+    };
+    if (rounds > 0) {
+        stage_k(0);
+        lds_barrier();
+        if (KS == 2 && ks) lds_barrier();   // half a step behind
+        ahead(begin);
+        __builtin_amdgcn_s_setprio(1);
+        scores();
+        __builtin_amdgcn_s_setprio(0);
+        lds_barrier();
+        between(begin, 0);
+        lds_barrier();
+        for (int i = 1; i < rounds; ++i) {
+            ahead(begin + KS * i);
+            __builtin_amdgcn_s_setprio(1);
+            outputs();
+            scores();
+            __builtin_amdgcn_s_setprio(0);
+            lds_barrier();   // this group's tiles are read
+            between(begin + KS * i, i & 1);
+            lds_barrier();   // the next ones are there
+        }
+        outputs();
+        if (KS == 2 && !ks) lds_barrier();
         __syncthreads();
     }
     l = halves_sum(l);
+    if constexpr (KS == 2) {
+        // The second group's rows through LDS, as they lie in its registers.
+        float *po = (float *)&smem[0][0][0] + wave * (16 * D * 64) + lane;
+        static_assert(sizeof(smem) >= 4 * 16 * D * 64 * sizeof(float), "the second group's outputs fit");
+        if (ks) {
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) po[(16 * d + i) * 64] = O[d][i];
+            if (h == 0) smem_ml[wave][col] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (ks) return;
+        const float2 other = smem_ml[wave][col];
+        const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(other.x - base);
+        m = top;
+        l = l * f0 + other.y * f1;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[d][i] = O[d][i] * f0 + po[(16 * d + i) * 64] * f1;
+    }
     if (row >= rq.rows) return;
     if (g.active > 1) {
         const size_t prow = ((size_t)r * a.max_tokens * group + row) * c.kv_heads + kvh;
@@ -614,17 +729,26 @@ struct Plan {
     int splits, least, most_rows;
 };
 
-Plan plan_of(int requests, int max_tokens, int max_length, int heads, int kv_heads, int width, int window)
+// Wide tiles that a step can have: every request's last one may be short.
+int64_t wide_tiles(int requests, int max_tokens, int count, int group)
+{
+    const int64_t each = ((int64_t)max_tokens * group + kWideRows - 1) / kWideRows * requests;
+    const int64_t all = (int64_t)count * group / kWideRows + requests;
+    return each < all ? each : all;
+}
+
+Plan plan_of(int requests, int max_tokens, int count, int max_length, int heads, int kv_heads, int width, int window)
 {
     const int64_t rows = (int64_t)max_tokens * (heads / kv_heads);
     Plan p = {1, kWaves, INT32_MAX};
     if (width <= 256 && rows > 32) p.most_rows = requests == 1 ? 0 : 32;
     const int tile = rows > p.most_rows ? kWideRows : kRows;
-    const int64_t groups = (rows + tile - 1) / tile * kv_heads * requests;
+    const int64_t groups = (tile == kRows ? (rows + kRows - 1) / kRows * requests
+                                          : wide_tiles(requests, max_tokens, count, heads / kv_heads)) * kv_heads;
     int64_t range = max_length;
     if (window && (int64_t)window + max_tokens < range) range = (int64_t)window + max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    const int64_t wanted = tile == kRows ? 1024 : 512, least = tile == kRows ? kWaves : 4;
+    const int64_t wanted = tile == kRows ? 1024 : 256, least = tile == kRows ? kWaves : 4;
     int64_t splits = wanted / groups;
     if (splits > 64) splits = 64;
     if (splits > steps / least) splits = steps / least;
@@ -648,10 +772,12 @@ hipError_t launch_rows(const Kv8Attention &a, Plan p, float *partials, hipStream
                            dim3(64 * kWaves), 0, s, a, p.splits, p.least, p.most_rows, partials);
     }
     if constexpr (W <= 256) {
-        if (rows > p.most_rows)
-            hipLaunchKernelGGL((kv8_wide<W>), dim3((unsigned)((rows + kWideRows - 1) / kWideRows * each),
-                                                   (unsigned)a.requests),
-                               dim3(64 * kWaves), 0, s, a, p.splits, p.most_rows, partials);
+        if (rows > p.most_rows) {
+            constexpr int KS = W <= 128 ? 2 : 1;
+            hipLaunchKernelGGL((kv8_wide<W, KS>), dim3((unsigned)(wide_tiles(a.requests, a.max_tokens, a.count,
+                                                                             a.heads / a.cache.kv_heads) * each)),
+                               dim3(256 * KS), 0, s, a, p.splits, p.most_rows, partials);
+        }
     }
     if (p.splits > 1)
         hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)(a.max_tokens * a.heads), (unsigned)a.requests), dim3(256), 0,
@@ -661,16 +787,16 @@ hipError_t launch_rows(const Kv8Attention &a, Plan p, float *partials, hipStream
 
 }  // namespace
 
-size_t kv8_attention_workspace(int requests, int max_tokens, int max_length, int heads, int kv_heads, int width,
-    int window)
+size_t kv8_attention_workspace(int requests, int max_tokens, int count, int max_length, int heads, int kv_heads,
+    int width, int window)
 {
-    const Plan p = plan_of(requests, max_tokens, max_length, heads, kv_heads, width, window);
+    const Plan p = plan_of(requests, max_tokens, count, max_length, heads, kv_heads, width, window);
     return p.splits > 1 ? p.splits * row_bytes(requests, max_tokens, heads, width) : 0;
 }
 
 hipError_t launch_kv8_attention(const Kv8Attention &a, void *workspace, size_t workspace_bytes, hipStream_t s)
 {
-    Plan p = plan_of(a.requests, a.max_tokens, a.max_length, a.heads, a.cache.kv_heads, a.cache.width, a.window);
+    Plan p = plan_of(a.requests, a.max_tokens, a.count, a.max_length, a.heads, a.cache.kv_heads, a.cache.width, a.window);
     const size_t each = row_bytes(a.requests, a.max_tokens, a.heads, a.cache.width);
     if (workspace_bytes / each < (size_t)p.splits) p.splits = (int)(workspace_bytes / each);
     if (p.splits < 1) p.splits = 1;
