@@ -58,7 +58,7 @@ bool page_ok(size_t n) { return n == 16 || n == 32 || n == 64 || n == 128; }
 bool geometry_ok(const nya_hip_kv8 *c)
 {
     return c && some(c->pages) && page_ok(c->page_tokens) && (c->width == 64 || c->width == 128 || c->width == 256 || c->width == 512) &&
-           heads_ok(c->kv_heads, c->width) &&
+           c->kv_heads <= 16384 && heads_ok(c->kv_heads, c->width) &&
            c->pages <= (size_t)INT_MAX / c->page_tokens && c->pages <= (size_t)INT_MAX / c->kv_heads;
 }
 

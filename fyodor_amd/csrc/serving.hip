@@ -195,26 +195,113 @@ __device__ __forceinline__ float rotated_at(const float *x, int d, const float2 
     return (float)(second ? a * s + b * c : a * c - b * s);
 }
 
-// Thread (row, head, pair or kept element).
-__global__ __launch_bounds__(256) void rope_rows(Rows q, Rows k, int width, const float2 *__restrict__ angles,
-    int rotated, bool halves)
+// (a, b) by the angle of (c, s).
+__device__ __forceinline__ void rotate_pair(float &a, float &b, double c, double s)
 {
-    const int row = blockIdx.x, half = rotated / 2, per_head = width - half;
-    const int i = blockIdx.y * 256 + threadIdx.x, head = i / per_head, e = i % per_head;
-    if (head >= q.heads + k.heads) return;
-    const Rows &t = head < q.heads ? q : k;
-    const int h = head < q.heads ? head : head - q.heads;
-    const float *x = t.x + row * t.stride + (int64_t)h * width;
-    float *out = t.out + row * t.out_stride + (int64_t)h * width;
-    if (e >= half) {
-        out[half + e] = x[half + e];
+    const double x = a, y = b;
+    a = (float)(x * c - y * s);
+    b = (float)(x * s + y * c);
+}
+
+// Heads head, head + step, ... of one row: their elements 4 quad .. + 3 (as
+// HALVES the pairs' other halves with them), 16 bytes at a time. What does not
+// turn is copied, or stays where it is in place.
+__device__ __forceinline__ void rotate_quads(const float *x, float *out, int head, int step, int heads,
+    int width, int quad, const float2 *__restrict__ angles, int rotated, bool halves)
+{
+    const int d = 4 * quad, half = rotated / 2;
+    const bool turns = halves ? d < half : d < rotated;
+    if (!turns && ((halves && d < rotated) || x == out)) return;
+    x += d;
+    out += d;
+    if (!turns) {
+#pragma unroll 4
+        for (int h = head; h < heads; h += step)
+            *(float4 *)(out + (size_t)h * width) = *(const float4 *)(x + (size_t)h * width);
+    } else if (halves) {
+        const float4 *a4 = (const float4 *)(angles + d);
+        const float4 p = a4[0], q = a4[1];
+        const double c0 = p.x, s0 = p.y, c1 = p.z, s1 = p.w, c2 = q.x, s2 = q.y, c3 = q.z, s3 = q.w;
+#pragma unroll 2
+        for (int h = head; h < heads; h += step) {
+            float4 u = *(const float4 *)(x + (size_t)h * width), v = *(const float4 *)(x + (size_t)h * width + half);
+            rotate_pair(u.x, v.x, c0, s0);
+            rotate_pair(u.y, v.y, c1, s1);
+            rotate_pair(u.z, v.z, c2, s2);
+            rotate_pair(u.w, v.w, c3, s3);
+            *(float4 *)(out + (size_t)h * width) = u;
+            *(float4 *)(out + (size_t)h * width + half) = v;
+        }
+    } else {
+        const float4 p = *(const float4 *)(angles + d / 2);
+        const double c0 = p.x, s0 = p.y, c1 = p.z, s1 = p.w;
+#pragma unroll 4
+        for (int h = head; h < heads; h += step) {
+            float4 u = *(const float4 *)(x + (size_t)h * width);
+            rotate_pair(u.x, u.y, c0, s0);
+            rotate_pair(u.z, u.w, c1, s1);
+            *(float4 *)(out + (size_t)h * width) = u;
+        }
+    }
+}
+
+// Heads [first, last) of one row by the workgroup's 256 threads: 16 bytes a
+// thread where everything allows it, else a pair or a kept element.
+__device__ __forceinline__ void rotate_heads(const Rows &t, int row, int first, int last, int width,
+    const float2 *__restrict__ angles, int rotated, bool halves, bool quads)
+{
+    const float *x = t.x + row * t.stride;
+    float *out = t.out + row * t.out_stride;
+    angles += (size_t)row * (rotated / 2);
+    const int tid = threadIdx.x;
+    if (quads) {
+        const int n = width / 4, step = 256 / n, head = tid / n;
+        if (head < step) rotate_quads(x, out, first + head, step, last, width, tid - head * n, angles, rotated, halves);
         return;
     }
-    const int d0 = halves ? e : 2 * e, d1 = halves ? e + half : 2 * e + 1;
-    const float2 *a = angles + (size_t)row * half;
-    const float u = rotated_at(x, d0, a, rotated, halves), v = rotated_at(x, d1, a, rotated, halves);
-    out[d0] = u;
-    out[d1] = v;
+    const int half = rotated / 2, n = width - half;
+    for (int i = tid; i < (last - first) * n; i += 256) {
+        const int h = first + i / n, e = i % n;
+        const float *xh = x + (size_t)h * width;
+        float *oh = out + (size_t)h * width;
+        if (e >= half) {
+            oh[half + e] = xh[half + e];
+            continue;
+        }
+        const int d0 = halves ? e : 2 * e, d1 = halves ? e + half : 2 * e + 1;
+        const float u = rotated_at(xh, d0, angles, rotated, halves), v = rotated_at(xh, d1, angles, rotated, halves);
+        oh[d0] = u;
+        oh[d1] = v;
+    }
+}
+
+// Workgroup (row, part of its heads).
+__global__ __launch_bounds__(256) void rope_rows(Rows q, Rows k, int width, const float2 *__restrict__ angles,
+    int rotated, bool halves, int q_parts, int each, bool quads)
+{
+    const int part = blockIdx.y;
+    if (part < q_parts)
+        rotate_heads(q, blockIdx.x, part * each, min(part * each + each, q.heads), width, angles, rotated, halves, quads);
+    else
+        rotate_heads(k, blockIdx.x, (part - q_parts) * each, min((part - q_parts) * each + each, k.heads), width, angles,
+                     rotated, halves, quads);
+}
+
+bool quads_ok(const Rows &t, int width, int rotated, bool halves, const float2 *angles)
+{
+    return !t.heads || (width % 4 == 0 && width <= 1024 && rotated % (halves ? 8 : 4) == 0 && t.stride % 4 == 0 &&
+                        t.out_stride % 4 == 0 && (((uintptr_t)t.x | (uintptr_t)t.out | (uintptr_t)angles) & 15) == 0);
+}
+
+// Heads of a row per workgroup: few where there are few rows, so that there
+// are workgroups for the chip; more where a thread can then use its angles for
+// several heads.
+int heads_each(int count, int heads, int width)
+{
+    const int at_once = width <= 1024 ? 1024 / width : 1;
+    int each = at_once;
+    while (each < heads && (int64_t)count * ((heads + each - 1) / each) > 4096) each += at_once;
+    return each;
 }
 
 // ---- the 8-bit cache ------------------------------------------------------
@@ -237,90 +324,249 @@ __device__ __forceinline__ int8_t code_of(float x, float scale, float inverse)
     return (int8_t)(int)fminf(fmaxf(n, -127.f), 127.f);
 }
 
-// Workgroup (row, KV head): the run of rows that begins at this one, if one
-// does; (row, kv_heads + part): a part of this row's q.
-__global__ __launch_bounds__(256) void kv8_store(Kv8 c, const int *__restrict__ slots, int count,
-    const float *__restrict__ k, int64_t k_stride, const float *__restrict__ v, int64_t v_stride,
-    const float2 *__restrict__ angles, int rotated, bool halves, Rows q)
+// The largest magnitude by its bits: NaN above infinity above the rest.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+
+struct Store {
+    Kv8 c;
+    const int *slots;
+    int count;
+    const float *k, *v;
+    int64_t k_stride, v_stride;
+    const float2 *angles;
+    int rotated;
+    bool halves, quads_k, quads_q;
+    Rows q;
+    int each;   // q heads per workgroup
+};
+
+// 16 elements of a key from element 16 chunk, rotated.
+__device__ __forceinline__ void key_chunk(const Store &s, int row, int head, int chunk, float (&x)[16])
 {
-    __shared__ uint32_t top[2][4];
-    const int row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, width = c.width, page_tokens = c.page_tokens;
-    if (head >= c.kv_heads) {
-        const int half = rotated / 2, per_head = width - half;
-        const int i = (head - c.kv_heads) * 256 + tid, h = i / per_head, e = i % per_head;
-        if (h >= q.heads) return;
-        const float *x = q.x + row * q.stride + (int64_t)h * width;
-        float *out = q.out + row * q.out_stride + (int64_t)h * width;
-        if (e >= half) {
-            out[half + e] = x[half + e];
-            return;
-        }
-        const int d0 = halves ? e : 2 * e, d1 = halves ? e + half : 2 * e + 1;
-        const float2 *a = angles + (size_t)row * half;
-        const float u = rotated_at(x, d0, a, rotated, halves), w = rotated_at(x, d1, a, rotated, halves);
-        out[d0] = u;
-        out[d1] = w;
+    const int d = 16 * chunk, half = s.rotated / 2;
+    const float *k = s.k + row * s.k_stride + (int64_t)head * s.c.width;
+    const float2 *angles = s.angles + (size_t)row * half;
+    if (!s.quads_k) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = rotated_at(k, d + i, angles, s.rotated, s.halves);
         return;
     }
-    const int slot = slots[row], at = slot % page_tokens;
-    if (slot < 0 || slot >= c.pages * page_tokens) return;
-    if (at && row && slots[row - 1] == slot - 1) return;
-    int n = 1;
-    while (row + n < count && at + n < page_tokens && slots[row + n] == slot + n) ++n;
-    const size_t place = (size_t)(slot / page_tokens) * c.kv_heads + head;
-    int8_t *codes[2] = {c.keys + place * page_tokens * width, c.values + place * page_tokens * width};
-    float *scales[2] = {c.key_scales + place, c.value_scales + place};
-    auto key = [&](int t, int d) {
-        return rotated_at(k + (row + t) * k_stride + (int64_t)head * width, d,
-                          angles + (size_t)(row + t) * (rotated / 2), rotated, halves);
-    };
-    auto value = [&](int t, int d) { return v[(row + t) * v_stride + (int64_t)head * width + d]; };
-    // The largest magnitude by its bits: NaN above infinity above the rest.
-    uint32_t big[2] = {0, 0};
-    for (int i = tid; i < n * width; i += 256) {
-        big[0] = max(big[0], __builtin_bit_cast(uint32_t, key(i / width, i % width)) & 0x7FFFFFFFu);
-        big[1] = max(big[1], __builtin_bit_cast(uint32_t, value(i / width, i % width)) & 0x7FFFFFFFu);
-    }
-    const float old[2] = {*scales[0], *scales[1]};
-    for (int kind = 0; kind < 2; ++kind) {
-        for (int o = 32; o; o >>= 1) big[kind] = max(big[kind], (uint32_t)__shfl_xor((int)big[kind], o, 64));
-        if ((tid & 63) == 0) top[kind][tid >> 6] = big[kind];
-    }
-    __syncthreads();
-    for (int kind = 0; kind < 2; ++kind) {
-        const uint32_t b = max(max(top[kind][0], top[kind][1]), max(top[kind][2], top[kind][3]));
-        const float amax = __builtin_bit_cast(float, b);
-        float scale = amax / 127.f;
-        if (scale < kScaleFloor) scale = kScaleFloor;
-        if (at) {
-            if (scale <= old[kind] || old[kind] != old[kind]) {
-                scale = old[kind];
-            } else {
-                for (int i = tid; i < page_tokens * width; i += 256)
-                    codes[kind][i] = (int8_t)(int)fmin(fmax(rint((double)codes[kind][i] * old[kind] / scale), -127.0), 127.0);
-                __syncthreads();
-            }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(float4 *)(x + 4 * i) = *(const float4 *)(k + d + 4 * i);
+    if (d >= s.rotated) return;
+    if (!s.halves) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 a = *(const float4 *)(angles + d / 2 + 2 * i);
+            rotate_pair(x[4 * i], x[4 * i + 1], a.x, a.y);
+            rotate_pair(x[4 * i + 2], x[4 * i + 3], a.z, a.w);
         }
-        const float inverse = 1.f / scale;
-        for (int i = tid; i < n * width; i += 256) {
-            const int t = i / width, d = i % width;
-            if (kind == 0) codes[0][key_at(at + t, d, page_tokens)] = code_of(key(t, d), scale, inverse);
-            else codes[1][value_at(at + t, d, width)] = code_of(value(t, d), scale, inverse);
+        return;
+    }
+    const bool second = d >= half;
+    const int j = second ? d - half : d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float4 o = *(const float4 *)(k + (second ? j : d + half) + 4 * i);
+        const float4 a0 = *(const float4 *)(angles + j + 4 * i), a1 = *(const float4 *)(angles + j + 4 * i + 2);
+        const float ov[4] = {o.x, o.y, o.z, o.w}, cv[4] = {a0.x, a0.z, a1.x, a1.z}, sv[4] = {a0.y, a0.w, a1.y, a1.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float u = second ? ov[e] : x[4 * i + e], w = second ? x[4 * i + e] : ov[e];
+            rotate_pair(u, w, cv[e], sv[e]);
+            x[4 * i + e] = second ? w : u;
         }
-        if (tid == 0) *scales[kind] = scale;
     }
 }
 
-__global__ __launch_bounds__(256) void kv8_load(Kv8 c, const int *__restrict__ slots, float *__restrict__ k,
-    int64_t k_stride, float *__restrict__ v, int64_t v_stride)
+// Element d of the run's values of granule g (positions 16 g.. of the page);
+// those outside the run are 0.
+__device__ __forceinline__ void value_granule(const Store &s, int row, int at, int n, int head, int g, int d,
+    float (&x)[16])
 {
-    const int row = blockIdx.x, i = blockIdx.y * 256 + threadIdx.x, head = i / c.width, d = i % c.width;
-    const int slot = slots[row];
-    if (head >= c.kv_heads || slot < 0 || slot >= c.pages * c.page_tokens) return;
-    const int t = slot % c.page_tokens;
-    const size_t place = (size_t)(slot / c.page_tokens) * c.kv_heads + head, codes = place * c.page_tokens * c.width;
-    k[row * k_stride + i] = (float)c.keys[codes + key_at(t, d, c.page_tokens)] * c.key_scales[place];
-    v[row * v_stride + i] = (float)c.values[codes + value_at(t, d, c.width)] * c.value_scales[place];
+    const float *v = s.v + (int64_t)head * s.c.width + d;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int t = 16 * g + i - at;
+        x[i] = t >= 0 && t < n ? v[(row + t) * s.v_stride] : 0.f;
+    }
+}
+
+__device__ __forceinline__ uint4 codes_of(const float (&x)[16], float scale, float inverse)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[i] |= (uint32_t)(uint8_t)code_of(x[4 * i + e], scale, inverse) << (8 * e);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Workgroup (row, 2 head + kind): the run of rows that begins at this one, if
+// one does, of the head's keys or values; (row, 2 kv_heads + part): a part of
+// this row's q. A thread forms 16 codes that lie together: of one position's key,
+// or of 16 positions of one element of the values. Bound by its chain of waits
+// (slots, rows and the old scale, codes) for a few rows, by the rows' bytes for many.
+__global__ __launch_bounds__(256) void kv8_store(Store s)
+{
+    __shared__ uint32_t top[4];
+    const Kv8 &c = s.c;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, width = c.width, page_tokens = c.page_tokens;
+    if ((int)blockIdx.y >= 2 * c.kv_heads) {
+        const int first = (blockIdx.y - 2 * c.kv_heads) * s.each;
+        rotate_heads(s.q, row, first, min(first + s.each, s.q.heads), width, s.angles, s.rotated, s.halves, s.quads_q);
+        return;
+    }
+    const int head = blockIdx.y >> 1, kind = blockIdx.y & 1;
+    const int slot = s.slots[row], before = row ? s.slots[row - 1] : -1;
+    if (slot < 0 || slot >= c.pages * page_tokens) return;
+    const int page = slot / page_tokens, at = slot % page_tokens;
+    if (at && row && before == slot - 1) return;
+    // The run's length: up to the first row that does not follow on, or the page's end.
+    int n = min(page_tokens - at, s.count - row);
+    {
+        const uint64_t off0 = __builtin_amdgcn_ballot_w64(lane >= n || s.slots[row + min(lane, n - 1)] != slot + lane);
+        if (off0) {
+            n = __builtin_ctzll(off0);
+        } else if (n > 64) {
+            const uint64_t off1 =
+                __builtin_amdgcn_ballot_w64(lane + 64 >= n || s.slots[row + min(lane + 64, n - 1)] != slot + lane + 64);
+            if (off1) n = 64 + __builtin_ctzll(off1);
+        }
+    }
+    const size_t place = (size_t)page * c.kv_heads + head;
+    uint4 *codes = (uint4 *)((kind ? c.values : c.keys) + place * page_tokens * width);
+    float *scale_at = (kind ? c.value_scales : c.key_scales) + place;
+    const float old = at ? *scale_at : 0.f;
+    // Pieces: (position, 16 elements) of the keys, 16 positions together; or
+    // (granule, element) of the values.
+    const int chunks = width / 16, g0 = at / 16;
+    const int pieces = kind ? ((at + n - 1) / 16 - g0 + 1) * width : (n + 15) / 16 * 16 * chunks;
+    auto piece_at = [&](int i, float (&x)[16]) {
+        if (kind) {
+            value_granule(s, row, at, n, head, g0 + i / width, i % width, x);
+        } else {
+            const int t = i / (16 * chunks) * 16 + i % 16, chunk = i / 16 % chunks;
+            if (t < n) {
+                key_chunk(s, row + t, head, chunk, x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = 0.f;
+            }
+        }
+    };
+    uint32_t big = 0;
+    float kept[2][16];   // this thread's first pieces; more are read again
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+        if (tid + 256 * p < pieces) {
+            piece_at(tid + 256 * p, kept[p]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) big = max(big, magnitude(kept[p][e]));
+        }
+    for (int i = tid + 512; i < pieces; i += 256) {
+        float x[16];
+        piece_at(i, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) big = max(big, magnitude(x[e]));
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o, 64));
+    if (lane == 0) top[tid >> 6] = big;
+    __syncthreads();
+    big = max(max(top[0], top[1]), max(top[2], top[3]));
+    float scale = __builtin_bit_cast(float, big) / 127.f;
+    if (scale < kScaleFloor) scale = kScaleFloor;
+    if (at) {
+        if (scale <= old || old != old) {
+            scale = old;
+        } else {
+            // The page's codes to the new step.
+            int8_t *all = (int8_t *)codes;
+            for (int i = tid; i < page_tokens * width; i += 256)
+                all[i] = (int8_t)(int)fmin(fmax(rint((double)all[i] * old / scale), -127.0), 127.0);
+            __syncthreads();
+        }
+    }
+    const float inverse = 1.f / scale;
+    auto put = [&](int i, const float (&x)[16]) {
+        const uint4 w = codes_of(x, scale, inverse);
+        if (kind) {
+            const int g = g0 + i / width, d = i % width;
+            // Positions of the granule outside the run keep their codes.
+            const int from = at - 16 * g, to = at + n - 16 * g;
+            uint4 *there = codes + g * width + d;
+            if (from <= 0 && to >= 16) {
+                *there = w;
+            } else {
+                int8_t *bytes = (int8_t *)there;
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (e >= from && e < to) bytes[e] = (int8_t)(word_of(w, e >> 2) >> (8 * (e & 3)));
+            }
+        } else {
+            const int t = i / (16 * chunks) * 16 + i % 16, chunk = i / 16 % chunks;
+            if (t < n) codes[chunk * page_tokens + at + t] = w;
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+        if (tid + 256 * p < pieces) put(tid + 256 * p, kept[p]);
+    for (int i = tid + 512; i < pieces; i += 256) {
+        float x[16];
+        piece_at(i, x);
+        put(i, x);
+    }
+    if (tid == 0) *scale_at = scale;
+}
+
+// Workgroup (rows, 1024 columns of heads x width): a thread 4 columns of each
+// row. The 4 x 16 codes of a granule's values stay for the rows that follow in it.
+__global__ __launch_bounds__(256) void kv8_load(Kv8 c, const int *__restrict__ slots, int count, int rows,
+    float *__restrict__ k, int64_t k_stride, float *__restrict__ v, int64_t v_stride, bool quads)
+{
+    const int i = 4 * (blockIdx.y * 256 + threadIdx.x), head = i / c.width, d = i % c.width;
+    if (head >= c.kv_heads) return;
+    const int end = min((int)(blockIdx.x + 1) * rows, count);
+    int held = -1;
+    uint4 w[4];
+    float ks = 0.f, vs = 0.f;
+    for (int row = blockIdx.x * rows; row < end; ++row) {
+        const int slot = slots[row];
+        if (slot < 0 || slot >= c.pages * c.page_tokens) continue;
+        const int t = slot % c.page_tokens;
+        const size_t place = (size_t)(slot / c.page_tokens) * c.kv_heads + head, codes = place * c.page_tokens * c.width;
+        if (slot / 16 != held) {
+            held = slot / 16;
+            const uint4 *there = (const uint4 *)(c.values + codes + value_at(t & ~15, d, c.width));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = there[e];
+            ks = c.key_scales[place];
+            vs = c.value_scales[place];
+        }
+        const uint32_t kw = *(const uint32_t *)(c.keys + codes + key_at(t, d, c.page_tokens));
+        float x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t q = (t & 8) ? ((t & 4) ? w[e].w : w[e].z) : ((t & 4) ? w[e].y : w[e].x);
+            x[e] = (float)(int8_t)(kw >> (8 * e)) * ks;
+            y[e] = (float)(int8_t)(q >> (8 * (t & 3))) * vs;
+        }
+        float *to_k = k + row * k_stride + i, *to_v = v + row * v_stride + i;
+        if (quads) {
+            *(float4 *)to_k = make_float4(x[0], x[1], x[2], x[3]);
+            *(float4 *)to_v = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                to_k[e] = x[e];
+                to_v[e] = y[e];
+            }
+        }
+    }
 }
 
 }  // namespace
@@ -344,26 +590,34 @@ hipError_t launch_rope_angles(const int *positions, int count, const float *freq
 hipError_t launch_rope(const Rows &q, const Rows &k, int width, int count, const float2 *angles, int rotated,
     bool halves, hipStream_t s)
 {
-    const int64_t n = (int64_t)(q.heads + k.heads) * (width - rotated / 2);
-    hipLaunchKernelGGL(rope_rows, dim3((unsigned)count, (unsigned)((n + 255) / 256)), dim3(256), 0, s, q, k, width,
-                       angles, rotated, halves);
+    const bool quads = quads_ok(q, width, rotated, halves, angles) && quads_ok(k, width, rotated, halves, angles);
+    const int each = heads_each(count, q.heads + k.heads, width);
+    const int q_parts = (q.heads + each - 1) / each, k_parts = (k.heads + each - 1) / each;
+    hipLaunchKernelGGL(rope_rows, dim3((unsigned)count, (unsigned)(q_parts + k_parts)), dim3(256), 0, s, q, k, width,
+                       angles, rotated, halves, q_parts, each, quads);
     return hipGetLastError();
 }
 
 hipError_t launch_kv8_store(const Kv8 &cache, const int *slots, int count, const float *k, int64_t k_stride,
     const float *v, int64_t v_stride, const float2 *angles, int rotated, bool halves, const Rows &q, hipStream_t s)
 {
-    const int64_t n = (int64_t)q.heads * (cache.width - rotated / 2);
-    hipLaunchKernelGGL(kv8_store, dim3((unsigned)count, (unsigned)(cache.kv_heads + (n + 255) / 256)), dim3(256), 0, s,
-                       cache, slots, count, k, k_stride, v, v_stride, angles, rotated, halves, q);
+    const uintptr_t all = (uintptr_t)k | (uintptr_t)angles;
+    const bool quads_k = (all & 15) == 0 && k_stride % 4 == 0 && rotated % (halves ? 32 : 16) == 0;
+    const bool quads_q = quads_ok(q, cache.width, rotated, halves, angles);
+    const int each = heads_each(count, q.heads, cache.width), parts = (q.heads + each - 1) / each;
+    const Store args = {cache, slots, count, k, v, k_stride, v_stride, angles, rotated, halves, quads_k, quads_q, q, each};
+    hipLaunchKernelGGL(kv8_store, dim3((unsigned)count, (unsigned)(2 * cache.kv_heads + parts)), dim3(256), 0, s, args);
     return hipGetLastError();
 }
 
 hipError_t launch_kv8_load(const Kv8 &cache, const int *slots, int count, float *k, int64_t k_stride, float *v,
     int64_t v_stride, hipStream_t s)
 {
-    hipLaunchKernelGGL(kv8_load, dim3((unsigned)count, (unsigned)(((int64_t)cache.kv_heads * cache.width + 255) / 256)),
-                       dim3(256), 0, s, cache, slots, k, k_stride, v, v_stride);
+    const bool quads = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
+    const int64_t parts = ((int64_t)cache.kv_heads * cache.width + 1023) / 1024;
+    const int rows = count * parts >= 8192 ? 16 : 4;
+    hipLaunchKernelGGL(kv8_load, dim3((unsigned)((count + rows - 1) / rows), (unsigned)parts), dim3(256), 0, s, cache,
+                       slots, count, rows, k, k_stride, v, v_stride, quads);
     return hipGetLastError();
 }
 

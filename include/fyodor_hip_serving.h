@@ -127,7 +127,7 @@ typedef struct nya_hip_kv8 {
 
 /* Bytes of one of the code arrays and of one of the scale arrays; 1 for
  * geometries that the cache does not have (widths and page sizes as above,
- * pages * page_tokens and pages * kv_heads <= INT_MAX). The addresses in `cache` are not looked at. */
+ * kv_heads <= 16384, pages * page_tokens and pages * kv_heads <= INT_MAX). The addresses in `cache` are not looked at. */
 NYA_HIP_EXPORT int nya_hip_kv8_bytes(const nya_hip_kv8 *cache, size_t *codes, size_t *scales);
 
 /* `count` rows of k and v (kv_heads heads of width, strides in floats) into
