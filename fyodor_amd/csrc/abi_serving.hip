@@ -68,6 +68,9 @@ bool cache_ok(const nya_hip_kv8 *c)
            vec(c->value_scales);
 }
 
+// (Row, KV head) pairs of a store or load: launches stay within 2^32 threads.
+bool pairs_fit(const nya_hip_kv8 *c, size_t count) { return rows_fit(count) && count <= ((size_t)1 << 25) / c->kv_heads; }
+
 Kv8 cache_of(const nya_hip_kv8 *c)
 {
     return {(int8_t *)c->keys, (int8_t *)c->values, (float *)c->key_scales, (float *)c->value_scales, (int)c->pages,
@@ -163,7 +166,7 @@ NYA_HIP_EXPORT int nya_hip_kv8_store(const nya_hip_kv8 *cache, uintptr_t slots, 
     size_t k_stride, uintptr_t v, size_t v_stride, uintptr_t angles, size_t rotated, unsigned layout, uintptr_t q,
     size_t q_stride, uintptr_t q_out, size_t q_out_stride, size_t heads, uintptr_t stream)
 {
-    if (!cache_ok(cache) || !vec(slots) || !rows_fit(count) || !vec(k) || !vec(v)) return 1;
+    if (!cache_ok(cache) || !vec(slots) || !pairs_fit(cache, count) || !vec(k) || !vec(v)) return 1;
     const size_t n = cache->kv_heads * cache->width;
     if (k_stride < n || v_stride < n || k_stride > (size_t)INT_MAX || v_stride > (size_t)INT_MAX) return 1;
     if (angles && !rotation_ok(angles, rotated, cache->width, layout)) return 1;
@@ -181,7 +184,7 @@ NYA_HIP_EXPORT int nya_hip_kv8_store(const nya_hip_kv8 *cache, uintptr_t slots, 
 NYA_HIP_EXPORT int nya_hip_kv8_load(const nya_hip_kv8 *cache, uintptr_t slots, size_t count, uintptr_t k,
     size_t k_stride, uintptr_t v, size_t v_stride, uintptr_t stream)
 {
-    if (!cache_ok(cache) || !vec(slots) || !rows_fit(count) || !vec(k) || !vec(v)) return 1;
+    if (!cache_ok(cache) || !vec(slots) || !pairs_fit(cache, count) || !vec(k) || !vec(v)) return 1;
     const size_t n = cache->kv_heads * cache->width;
     if (k_stride < n || v_stride < n || k_stride > (size_t)INT_MAX || v_stride > (size_t)INT_MAX ||
         !apart(k, k_stride, n, v, v_stride, n, count))
@@ -196,7 +199,7 @@ static bool attention_ok(const nya_hip_kv8 *cache, size_t count, size_t requests
 {
     return geometry_ok(cache) && rows_fit(count) && requests && requests <= 65535 && max_tokens && max_tokens <= count &&
            some(max_length) && heads_ok(heads, cache->width) && heads % cache->kv_heads == 0 &&
-           max_tokens <= ((size_t)1 << 26) / heads && window <= (size_t)INT_MAX;
+           count <= ((size_t)1 << 28) / heads && requests <= ((size_t)1 << 21) / cache->kv_heads && window <= (size_t)INT_MAX;
 }
 
 NYA_HIP_EXPORT int nya_hip_kv8_attention_bytes(const nya_hip_kv8 *cache, size_t count, size_t requests,

@@ -279,11 +279,11 @@ __device__ __forceinline__ void rotate_heads(const Rows &t, int row, int first, 
 __global__ __launch_bounds__(256) void rope_rows(Rows q, Rows k, int width, const float2 *__restrict__ angles,
     int rotated, bool halves, int q_parts, int each, bool quads)
 {
-    const int part = blockIdx.y;
+    const int row = blockIdx.x, part = blockIdx.y;
     if (part < q_parts)
-        rotate_heads(q, blockIdx.x, part * each, min(part * each + each, q.heads), width, angles, rotated, halves, quads);
+        rotate_heads(q, row, part * each, min(part * each + each, q.heads), width, angles, rotated, halves, quads);
     else
-        rotate_heads(k, blockIdx.x, (part - q_parts) * each, min((part - q_parts) * each + each, k.heads), width, angles,
+        rotate_heads(k, row, (part - q_parts) * each, min((part - q_parts) * each + each, k.heads), width, angles,
                      rotated, halves, quads);
 }
 
@@ -337,20 +337,19 @@ struct Store {
     int rotated;
     bool halves, quads_k, quads_q;
     Rows q;
-    int each;   // q heads per workgroup
+    int each;    // q heads per workgroup
+    int parts;   // workgroups per row of q
+    int rows;    // rows of a workgroup that stores
+    int stores;  // workgroups that store
 };
 
-// 16 elements of a key from element 16 chunk, rotated.
+// 16 elements of a key from element 16 chunk, rotated; rows and angles in 16 bytes.
+template <int W>
 __device__ __forceinline__ void key_chunk(const Store &s, int row, int head, int chunk, float (&x)[16])
 {
     const int d = 16 * chunk, half = s.rotated / 2;
-    const float *k = s.k + row * s.k_stride + (int64_t)head * s.c.width;
+    const float *k = s.k + row * s.k_stride + head * W;
     const float2 *angles = s.angles + (size_t)row * half;
-    if (!s.quads_k) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = rotated_at(k, d + i, angles, s.rotated, s.halves);
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) *(float4 *)(x + 4 * i) = *(const float4 *)(k + d + 4 * i);
     if (d >= s.rotated) return;
@@ -380,15 +379,21 @@ __device__ __forceinline__ void key_chunk(const Store &s, int row, int head, int
 }
 
 // Element d of the run's values of granule g (positions 16 g.. of the page);
-// those outside the run are 0.
+// those outside the run are 0. g is the same in a wavefront: rows by scalar addresses.
+template <int W>
 __device__ __forceinline__ void value_granule(const Store &s, int row, int at, int n, int head, int g, int d,
     float (&x)[16])
 {
-    const float *v = s.v + (int64_t)head * s.c.width + d;
+    g = __builtin_amdgcn_readfirstlane(g);
+    const float *v = s.v + row * s.v_stride + head * W;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = (v + min(max(16 * g + i - at, 0), n - 1) * s.v_stride)[d];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
+        // All loads set out first: moved under the condition each would be waited for by itself.
+        asm volatile("" : "+v"(x[i]));
         const int t = 16 * g + i - at;
-        x[i] = t >= 0 && t < n ? v[(row + t) * s.v_stride] : 0.f;
+        x[i] = t >= 0 && t < n ? x[i] : 0.f;
     }
 }
 
@@ -405,53 +410,56 @@ __device__ __forceinline__ uint4 codes_of(const float (&x)[16], float scale, flo
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Workgroup (row, 2 head + kind): the run of rows that begins at this one, if
-// one does, of the head's keys or values; (row, 2 kv_heads + part): a part of
-// this row's q. A thread forms 16 codes that lie together: of one position's key,
-// or of 16 positions of one element of the values. Bound by its chain of waits
-// (slots, rows and the old scale, codes) for a few rows, by the rows' bytes for many.
-__global__ __launch_bounds__(256) void kv8_store(Store s)
+// The run of rows that begins at `row`: its head's keys (kind 0) or values. In
+// a long run a thread forms 16 codes that lie together: of one position's key, or
+// of 16 positions of one element of the values; in a short one (decoding) single
+// codes. Bound by its chain of waits (slots, rows and the old scale, codes) for a
+// few rows, by the rows' bytes for many.
+template <int W>
+__device__ __forceinline__ void store_run(const Store &args, int row, int head, int kind, uint32_t *top)
 {
-    __shared__ uint32_t top[4];
+    constexpr int kChunks = W / 16, kShort = 4;   // elements per thread of a short run
+    Store s = args;
+    // Opaque: what follows from them is formed for each run instead of living
+    // in registers over the loop of runs.
+    asm volatile("" : "+s"(s.k_stride), "+s"(s.v_stride), "+s"(s.c.page_tokens), "+s"(s.rotated), "+s"(head));
     const Kv8 &c = s.c;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, width = c.width, page_tokens = c.page_tokens;
-    if ((int)blockIdx.y >= 2 * c.kv_heads) {
-        const int first = (blockIdx.y - 2 * c.kv_heads) * s.each;
-        rotate_heads(s.q, row, first, min(first + s.each, s.q.heads), width, s.angles, s.rotated, s.halves, s.quads_q);
-        return;
-    }
-    const int head = blockIdx.y >> 1, kind = blockIdx.y & 1;
-    const int slot = s.slots[row], before = row ? s.slots[row - 1] : -1;
-    if (slot < 0 || slot >= c.pages * page_tokens) return;
-    const int page = slot / page_tokens, at = slot % page_tokens;
-    if (at && row && before == slot - 1) return;
+    const int tid = threadIdx.x, lane = tid & 63, page_tokens = c.page_tokens;
+    const int slot = s.slots[row], shift = 31 - __builtin_clz(page_tokens), page = slot >> shift,
+              at = slot & (page_tokens - 1);
+    const int next0 = s.slots[min(row + lane, s.count - 1)], next1 = s.slots[min(row + lane + 64, s.count - 1)];
     // The run's length: up to the first row that does not follow on, or the page's end.
     int n = min(page_tokens - at, s.count - row);
     {
-        const uint64_t off0 = __builtin_amdgcn_ballot_w64(lane >= n || s.slots[row + min(lane, n - 1)] != slot + lane);
-        if (off0) {
-            n = __builtin_ctzll(off0);
-        } else if (n > 64) {
-            const uint64_t off1 =
-                __builtin_amdgcn_ballot_w64(lane + 64 >= n || s.slots[row + min(lane + 64, n - 1)] != slot + lane + 64);
-            if (off1) n = 64 + __builtin_ctzll(off1);
-        }
+        const uint64_t off0 = __builtin_amdgcn_ballot_w64(lane >= n || next0 != slot + lane);
+        const uint64_t off1 = __builtin_amdgcn_ballot_w64(lane + 64 >= n || next1 != slot + lane + 64);
+        if (off0) n = __builtin_ctzll(off0);
+        else if (off1) n = 64 + __builtin_ctzll(off1);
     }
     const size_t place = (size_t)page * c.kv_heads + head;
-    uint4 *codes = (uint4 *)((kind ? c.values : c.keys) + place * page_tokens * width);
+    uint4 *codes = (uint4 *)((kind ? c.values : c.keys) + place * page_tokens * W);
+    int8_t *bytes = (int8_t *)codes;
     float *scale_at = (kind ? c.value_scales : c.key_scales) + place;
     const float old = at ? *scale_at : 0.f;
+    // Single codes, too, of keys whose rows or angles do not come in 16 bytes.
+    const bool brief = n * W <= 256 * kShort || (!kind && !s.quads_k);
+    auto element = [&](int i) {
+        const int r = row + i / W, d = i % W;
+        return kind ? s.v[r * s.v_stride + head * W + d]
+                    : rotated_at(s.k + r * s.k_stride + head * W, d, s.angles + (size_t)r * (s.rotated / 2), s.rotated,
+                                 s.halves);
+    };
     // Pieces: (position, 16 elements) of the keys, 16 positions together; or
     // (granule, element) of the values.
-    const int chunks = width / 16, g0 = at / 16;
-    const int pieces = kind ? ((at + n - 1) / 16 - g0 + 1) * width : (n + 15) / 16 * 16 * chunks;
+    const int g0 = at / 16;
+    const int pieces = kind ? ((at + n - 1) / 16 - g0 + 1) * W : (n + 15) / 16 * 16 * kChunks;
     auto piece_at = [&](int i, float (&x)[16]) {
         if (kind) {
-            value_granule(s, row, at, n, head, g0 + i / width, i % width, x);
+            value_granule<W>(s, row, at, n, head, g0 + i / W, i % W, x);
         } else {
-            const int t = i / (16 * chunks) * 16 + i % 16, chunk = i / 16 % chunks;
+            const int t = i / (16 * kChunks) * 16 + i % 16, chunk = i / 16 % kChunks;
             if (t < n) {
-                key_chunk(s, row + t, head, chunk, x);
+                key_chunk<W>(s, row + t, head, chunk, x);
             } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[e] = 0.f;
@@ -459,68 +467,120 @@ __global__ __launch_bounds__(256) void kv8_store(Store s)
         }
     };
     uint32_t big = 0;
-    float kept[2][16];   // this thread's first pieces; more are read again
+    float few[kShort], kept[2][16];   // this thread's elements, or first pieces (more are read again)
+    if (brief) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p)
-        if (tid + 256 * p < pieces) {
-            piece_at(tid + 256 * p, kept[p]);
+        for (int p = 0; p < kShort; ++p)
+            if (tid + 256 * p < n * W) {
+                few[p] = element(tid + 256 * p);
+                big = max(big, magnitude(few[p]));
+            }
+#pragma unroll 1
+        for (int i = tid + 256 * kShort; i < n * W; i += 256) big = max(big, magnitude(element(i)));
+    } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) big = max(big, magnitude(kept[p][e]));
+        for (int p = 0; p < 2; ++p)
+            if (tid + 256 * p < pieces) {
+                piece_at(tid + 256 * p, kept[p]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) big = max(big, magnitude(kept[p][e]));
+            }
+#pragma unroll 1
+        for (int i = tid + 512; i < pieces; i += 256) {
+            float x[16];
+            piece_at(i, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) big = max(big, magnitude(x[e]));
         }
-    for (int i = tid + 512; i < pieces; i += 256) {
-        float x[16];
-        piece_at(i, x);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) big = max(big, magnitude(x[e]));
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o, 64));
     if (lane == 0) top[tid >> 6] = big;
     __syncthreads();
     big = max(max(top[0], top[1]), max(top[2], top[3]));
-    float scale = __builtin_bit_cast(float, big) / 127.f;
+    float scale = __builtin_bit_cast(float, big) * (1.f / 127.f);
     if (scale < kScaleFloor) scale = kScaleFloor;
     if (at) {
         if (scale <= old || old != old) {
             scale = old;
         } else {
             // The page's codes to the new step.
-            int8_t *all = (int8_t *)codes;
-            for (int i = tid; i < page_tokens * width; i += 256)
-                all[i] = (int8_t)(int)fmin(fmax(rint((double)all[i] * old / scale), -127.0), 127.0);
+#pragma unroll 1
+            for (int i = tid; i < page_tokens * W; i += 256)
+                bytes[i] = (int8_t)(int)fmin(fmax(rint((double)bytes[i] * old / scale), -127.0), 127.0);
             __syncthreads();
         }
     }
     const float inverse = 1.f / scale;
+    if (tid == 0) *scale_at = scale;
+    if (brief) {
+#pragma unroll
+        for (int p = 0; p < kShort; ++p) {
+            const int i = tid + 256 * p, t = at + i / W, d = i % W;
+            if (i < n * W) bytes[kind ? value_at(t, d, W) : key_at(t, d, page_tokens)] = code_of(few[p], scale, inverse);
+        }
+#pragma unroll 1
+        for (int i = tid + 256 * kShort; i < n * W; i += 256)
+            bytes[key_at(at + i / W, i % W, page_tokens)] = code_of(element(i), scale, inverse);
+        return;
+    }
     auto put = [&](int i, const float (&x)[16]) {
         const uint4 w = codes_of(x, scale, inverse);
         if (kind) {
-            const int g = g0 + i / width, d = i % width;
             // Positions of the granule outside the run keep their codes.
-            const int from = at - 16 * g, to = at + n - 16 * g;
-            uint4 *there = codes + g * width + d;
+            const int g = g0 + i / W, from = at - 16 * g, to = at + n - 16 * g;
+            uint4 *there = codes + g * W + i % W;
             if (from <= 0 && to >= 16) {
                 *there = w;
             } else {
-                int8_t *bytes = (int8_t *)there;
+                int8_t *b = (int8_t *)there;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (e >= from && e < to) bytes[e] = (int8_t)(word_of(w, e >> 2) >> (8 * (e & 3)));
+                    if (e >= from && e < to) b[e] = (int8_t)(word_of(w, e >> 2) >> (8 * (e & 3)));
             }
         } else {
-            const int t = i / (16 * chunks) * 16 + i % 16, chunk = i / 16 % chunks;
+            const int t = i / (16 * kChunks) * 16 + i % 16, chunk = i / 16 % kChunks;
             if (t < n) codes[chunk * page_tokens + at + t] = w;
         }
     };
 #pragma unroll
     for (int p = 0; p < 2; ++p)
         if (tid + 256 * p < pieces) put(tid + 256 * p, kept[p]);
+#pragma unroll 1
     for (int i = tid + 512; i < pieces; i += 256) {
         float x[16];
         piece_at(i, x);
         put(i, x);
     }
-    if (tid == 0) *scale_at = scale;
+}
+
+// Workgroup (group of rows, 2 head + kind): the runs that begin in its rows;
+// from number `stores` on, (row, part): a part of a row's q. A group's
+// workgroups stand together: with the rows' first head before all second ones, strides
+// that are multiples of 4 KB sent everything in flight to the same few channels
+// (4096 rows, 8 heads of 128, no q: 331 us, so 46). Most rows of a prompt begin
+// no run, and a workgroup that finds none costs 0.35 ns of the chip: rows go in
+// groups where there are many (those 46 us -> 27; the bytes alone take 8).
+template <int W>
+__global__ __launch_bounds__(256, 3) void kv8_store(Store s)
+{
+    __shared__ uint32_t top[4];
+    const int pairs = 2 * s.c.kv_heads;
+    if ((int)blockIdx.x >= s.stores) {
+        const int i = blockIdx.x - s.stores, first = i % s.parts * s.each;
+        rotate_heads(s.q, i / s.parts, first, min(first + s.each, s.q.heads), W, s.angles, s.rotated, s.halves,
+                     s.quads_q);
+        return;
+    }
+    const int first_row = blockIdx.x / pairs * s.rows, part = blockIdx.x % pairs;
+    const int lane = threadIdx.x & 63, rows = min(s.rows, s.count - first_row);
+    const int row = first_row + min(lane, rows - 1), slot = s.slots[row], before = row ? s.slots[row - 1] : -2;
+    uint64_t mask = __builtin_amdgcn_ballot_w64(lane < rows && (unsigned)slot < (unsigned)(s.c.pages * s.c.page_tokens) &&
+                                                (before != slot - 1 || (slot & (s.c.page_tokens - 1)) == 0));
+    for (; mask; mask &= mask - 1) {
+        store_run<W>(s, first_row + __builtin_ctzll(mask), part >> 1, part & 1, top);
+        __syncthreads();   // `top` is read
+    }
 }
 
 // Workgroup (rows, 1024 columns of heads x width): a thread 4 columns of each
@@ -604,9 +664,19 @@ hipError_t launch_kv8_store(const Kv8 &cache, const int *slots, int count, const
     const uintptr_t all = (uintptr_t)k | (uintptr_t)angles;
     const bool quads_k = (all & 15) == 0 && k_stride % 4 == 0 && rotated % (halves ? 32 : 16) == 0;
     const bool quads_q = quads_ok(q, cache.width, rotated, halves, angles);
-    const int each = heads_each(count, q.heads, cache.width), parts = (q.heads + each - 1) / each;
-    const Store args = {cache, slots, count, k, v, k_stride, v_stride, angles, rotated, halves, quads_k, quads_q, q, each};
-    hipLaunchKernelGGL(kv8_store, dim3((unsigned)count, (unsigned)(2 * cache.kv_heads + parts)), dim3(256), 0, s, args);
+    const int each = q.heads ? heads_each(count, q.heads, cache.width) : 1, parts = (q.heads + each - 1) / each;
+    const int64_t work = (int64_t)count * cache.kv_heads;
+    const int rows = work <= 2048 ? 1 : work <= 8192 ? 4 : 8;
+    const int64_t stores = (int64_t)((count + rows - 1) / rows) * 2 * cache.kv_heads;
+    const Store args = {cache, slots, count, k, v, k_stride, v_stride, angles, rotated, halves, quads_k, quads_q, q, each,
+                        parts, rows, (int)stores};
+    const dim3 grid((unsigned)(stores + (int64_t)count * parts));
+    switch (cache.width) {
+    case 64: hipLaunchKernelGGL(kv8_store<64>, grid, dim3(256), 0, s, args); break;
+    case 128: hipLaunchKernelGGL(kv8_store<128>, grid, dim3(256), 0, s, args); break;
+    case 256: hipLaunchKernelGGL(kv8_store<256>, grid, dim3(256), 0, s, args); break;
+    default: hipLaunchKernelGGL(kv8_store<512>, grid, dim3(256), 0, s, args); break;
+    }
     return hipGetLastError();
 }
 

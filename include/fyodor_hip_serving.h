@@ -17,7 +17,9 @@
  * a HIP failure. Vectors are fp32 device arrays, 4-byte aligned; 16-byte
  * aligned rows whose strides are multiples of 4 load and store faster.
  * Integers on the device (lengths, counts, tables, slots, positions) are
- * int32. A step has at most 2^22 rows (tokens), a row at most 2^22 floats.
+ * int32. A step has at most 2^22 rows (tokens), a row at most 2^22 floats;
+ * count * kv_heads <= 2^25 where rows are stored or loaded, count * heads <=
+ * 2^28 and requests * kv_heads <= 2^21 in attention.
  * The integers are data of the step that no call can check beforehand:
  * an entry outside its range is taken as "nothing there", never followed.
  *
@@ -138,7 +140,7 @@ NYA_HIP_EXPORT int nya_hip_kv8_bytes(const nya_hip_kv8 *cache, size_t *codes, si
  * both.
  *
  * Rows of one page stand together, in the order of their positions, and no
- * slot twice. Such a run takes wanted = max|x| / 127 (in fp32, at least
+ * slot twice. Such a run takes wanted = max|x| * (1 / 127) (in fp32, at least
  * 2^-100) of its rows in a head. A run from the page's first slot sets the
  * scale to that; a later one raises it to that if it is lower, and the
  * page's codes are rounded again to the new step, code = round(code * old /

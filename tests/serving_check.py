@@ -150,7 +150,7 @@ class Cache:
             x = rows[:, h]
             old = self.scales[page, h]
             with np.errstate(all="ignore"):
-                wanted = np.float32(np.max(np.abs(x))) / np.float32(127)
+                wanted = np.float32(np.max(np.abs(x))) * (np.float32(1) / np.float32(127))
                 if wanted < SCALE_FLOOR:
                     wanted = np.float32(SCALE_FLOOR)
                 scale = wanted
