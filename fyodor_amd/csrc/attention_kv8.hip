@@ -15,6 +15,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kStep = 64;   // positions per step of a wavefront
 constexpr int kRows = 16;   // query rows per tile of a few
 constexpr int kWaves = 4;
+constexpr int kMostSplits = 64;   // a lane each where they are joined
 constexpr int kWideRows = 32 * kWaves;   // query rows per tile of many
 
 // The positions that a tile of query rows sees and how they are split: steps
@@ -42,8 +43,8 @@ __device__ __forceinline__ Range range_of(const Kv8Attention &a, const Request &
     int least)
 {
     const int group = a.heads / a.cache.kv_heads;
-    // Positions of a whole step past the last one still fit 31 bits.
-    const int64_t most = min((int64_t)a.table_stride * a.cache.page_tokens - 1, (int64_t)INT32_MAX - 2 * kStep);
+    // Positions of the steps looked up past the last one still fit 31 bits.
+    const int64_t most = min((int64_t)a.table_stride * a.cache.page_tokens - 1, (int64_t)INT32_MAX - 64 * kStep);
     const int64_t low = q.first + rows * tile / group, high = q.first + (min(rows * tile + rows, q.rows) - 1) / group;
     Range g;
     g.highest = (int)(high < 0 ? -1 : high < most ? high : most);
@@ -115,31 +116,84 @@ __device__ __forceinline__ float column_sum(float v)
     return halves_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
 }
 
+// Requests of a few rows: 16 rows per workgroup, whose wavefronts take every
+// fourth step of its share of the positions and meet in LDS at the end. Keys
+// and values go from memory straight into the operands' lanes: K and V of a
+// step are requested as soon as the last step's are used up, pages a step
+// before that.
 template <int W>
-__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Attention a, int splits, int least,
-    int most_rows, float *__restrict__ partials)
+__device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, int sp, int tile, int splits, int least,
+    int most_rows, float *__restrict__ partials, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
 {
     constexpr int C = W / 64, D = W / 16;
+    constexpr bool kAhead = W <= 256;   // room for a step's K and V in registers
     const Kv8 &c = a.cache;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, part = lane >> 4;
-    const int group = a.heads / c.kv_heads, r = blockIdx.y;
-    int x = blockIdx.x;
-    const int kvh = x % c.kv_heads;
-    x /= c.kv_heads;
-    const int sp = x % splits, tile = x / splits;
+    const int group = a.heads / c.kv_heads;
     const Request rq = request_of(a, r);
     if (kRows * tile >= rq.rows || rq.rows > most_rows) return;
     const Range g = range_of(a, rq, tile, kRows, splits, least);
     if (sp >= g.active) return;
 
-    const int row = kRows * tile + col, row_in = min(row, rq.rows - 1), token = row_in / group;
-    const int head = kvh * group + row_in % group;
+    // Rows past the request's last repeat it and are not written.
+    const int row = min(kRows * tile + col, rq.rows - 1), token = row / group, head = kvh * group + row % group;
     const int64_t p = rq.first + token;
-    const int last = row < rq.rows ? (int)(p < g.highest ? p : g.highest) : -1;
+    const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
+    // Positions that all rows see: up to the first row's last, from the last row's first.
+    const int64_t p0 = rq.first + kRows * tile / group, p1 = rq.first + min(kRows * tile + kRows - 1, rq.rows - 1) / group;
+    const int all_to = (int)(p0 < g.highest ? p0 : g.highest);
+    const int all_from = (int)(a.window && p1 >= a.window ? (p1 - a.window < g.highest ? p1 - a.window + 1 : g.highest + 1) : 0);
 
-    // The row's q in two pieces, scaled by a power of two.
+    const int *table = a.table + (size_t)r * a.table_stride;
+    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
+    const int begin = g.begin + sp * g.chunk + wave, stop = min(g.begin + (sp + 1) * g.chunk, g.end);
+    // Lane l reads keys of the granule of 16 positions (l % 16) / 4 of a step and
+    // holds scores and values of granule l / 16. Everything is read
+    // unconditionally (positions past the last one lead to page 0).
+    auto entry_of = [&](int at) {
+        const int entry = table[min(at >> shift, a.table_stride - 1)];
+        return at <= g.highest ? entry : -1;
+    };
+    auto place_of = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + kvh; };
+    const size_t plane = (size_t)c.page_tokens * W;
+    int kpage, vpage;
+    auto look = [&](int step) {
+        kpage = entry_of(kStep * step + 16 * (col >> 2));
+        vpage = entry_of(kStep * step + 16 * part);
+    };
+    auto keys_at = [&](int step) {
+        const int at = kStep * step + 16 * (col >> 2);
+        return c.keys + place_of(kpage) * plane + (part * c.page_tokens + (at & within) + (col & 3)) * 16;
+    };
+    auto values_at = [&](int step) {
+        const int at = kStep * step + 16 * part;
+        return c.values + place_of(vpage) * plane + ((at & within) * W + 16 * col);
+    };
+    uint4 kr[4][C], vr[D];
+    float ks, vs;
+    bool there;
+    auto fetch_k = [&](int step) {
+        const int8_t *kb = keys_at(step);
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) kr[t][i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i + 64 * t);
+    };
+    auto fetch_v = [&](int step) {
+        const int8_t *vb = values_at(step);
+        ks = c.key_scales[place_of(vpage)];
+        vs = c.value_scales[place_of(vpage)];
+        there = (unsigned)vpage < (unsigned)c.pages;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) vr[d] = *(const uint4 *)(vb + 256 * d);
+        }
+    };
+    look(begin);
+
+    // The row's q in two pieces, scaled by a power of two; the scale's sign goes with it.
     half8 qh[2 * C], ql[2 * C];
     float qscale;
     {
@@ -156,113 +210,124 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[16 * i + e] = q[64 * i + e];
         }
+        if constexpr (kAhead) {
+            fetch_k(begin);
+            fetch_v(begin);
+            look(begin + kWaves);
+        }
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < 16 * C; ++i) top = fmaxf(top, fabsf(v[i]));
         const int e = 14 - __builtin_amdgcn_frexp_expf(column_max(top));
 #pragma unroll
-        for (int i = 0; i < 16 * C; ++i) v[i] = ldexpf(v[i], e);
+        for (int i = 0; i < 16 * C; ++i) v[i] = ldexpf(a.scale < 0.f ? -v[i] : v[i], e);
 #pragma unroll
         for (int i = 0; i < 2 * C; ++i) split_f16(v + 8 * i, qh[i], ql[i]);
         // exp(s) = exp2(s log2 e), q back to its size.
-        qscale = ldexpf(a.scale * 1.44269504f, -e);
+        qscale = ldexpf(fabsf(a.scale) * 1.44269504f, -e);
     }
-
-    const int *table = a.table + (size_t)r * a.table_stride;
-    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
-    // Lane l reads keys of the granule of 16 positions (l % 16) / 4 of a step and
-    // holds scores and values of granule l / 16.
-    auto page_of = [&](int at) {
-        const int j = at >> shift;
-        int page = -1;
-        if (at <= g.highest && j < a.table_stride) page = table[j];
-        return (unsigned)page < (unsigned)c.pages ? page : -1;
-    };
-    auto place_of = [&](int page) { return (size_t)max(page, 0) * c.kv_heads + kvh; };
-    const size_t plane = (size_t)c.page_tokens * W;
 
     f32x4 O[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) O[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    const int stop = min(g.begin + (sp + 1) * g.chunk, g.end);
-    for (int step = g.begin + sp * g.chunk + wave; step < stop; step += kWaves) {
-        const int kat = kStep * step + 16 * (col >> 2), vat = kStep * step + 16 * part;
-        const int kpage = page_of(kat), vpage = page_of(vat);
-        const int8_t *kb = c.keys + place_of(kpage) * plane + (part * c.page_tokens + (kat & within) + (col & 3)) * 16;
-        const int8_t *vb = c.values + place_of(vpage) * plane + ((vat & within) * W + 16 * col);
-        uint4 kr[4][C], vr[D];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < C; ++i) kr[t][i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i + 64 * t);
-#pragma unroll
-        for (int d = 0; d < D; ++d) vr[d] = *(const uint4 *)(vb + 256 * d);
-        float ks = 0.f, vs = 0.f;
-        if (vpage >= 0) {
-            ks = c.key_scales[place_of(vpage)];
-            vs = c.value_scales[place_of(vpage)];
+    for (int step = begin; step < stop; step += kWaves) {
+        const int8_t *vb = nullptr;
+        if constexpr (!kAhead) {
+            fetch_k(step);
+            fetch_v(step);
+            vb = values_at(step);
+            look(step + kWaves);
         }
         f32x4 S[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            S[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) S[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                const half8 k0 = codes_f16(kr[t][i].x, kr[t][i].y), k1 = codes_f16(kr[t][i].z, kr[t][i].w);
-                S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * i], S[t], 0, 0, 0);
-                S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[2 * i], S[t], 0, 0, 0);
-                S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * i + 1], S[t], 0, 0, 0);
-                S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[2 * i + 1], S[t], 0, 0, 0);
-            }
+        for (int i = 0; i < C; ++i) {
+            half8 k[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) k[t] = codes_f16(kr[t][i].x, kr[t][i].y);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], qh[2 * i], S[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[2 * i], S[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) k[t] = codes_f16(kr[t][i].z, kr[t][i].w);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], qh[2 * i + 1], S[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[2 * i + 1], S[t], 0, 0, 0);
         }
+        if constexpr (kAhead) fetch_k(step + kWaves);
         // Scores in powers of two with the exponent of the page's value scale
-        // added, so that weights times that scale are what is normalised.
-        const int e = __builtin_amdgcn_frexp_expf(vs);
-        float mant = __builtin_amdgcn_frexp_mantf(vs);
-        if (!__builtin_isfinite(vs)) mant = NAN;
-        const float scale = __builtin_isfinite(ks) ? ks * qscale : NAN;
-        const int from = vpage >= 0 ? first - vat : 16, to = vpage >= 0 ? last - vat : -1;
-        float w[16];
-        float top = -INFINITY;
+        // added, so that weights times that scale are what is normalised, by a
+        // whole power of two. A page that reads as NaN makes the rows that see
+        // it NaN by their sum alone.
+        const int at = kStep * step, pos = at + 16 * part;
+        const bool fine = __builtin_isfinite(ks) && __builtin_isfinite(vs);
+        const float scale = fine ? fmaxf(fabsf(ks) * qscale, 0x1p-126f) : 1.f;   // above 0: keeps minus infinity
+        const int e = fine ? __builtin_amdgcn_frexp_expf(vs) : 0;
+        const float mant = fine ? __builtin_amdgcn_frexp_mantf(vs) : 1.f;
+        if (there && !fine && first <= pos + 15 && last >= pos) l = NAN;
+        if (all_from > at || all_to < at + kStep - 1 || __builtin_amdgcn_ballot_w64(!there)) {
+            const int from = there ? max(first - pos, 0) : 16, to = min(last - pos, 15);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float s = S[i >> 2][i & 3] * scale;
-            w[i] = i >= from && i <= to ? s : -INFINITY;
-            top = fmaxf(top, w[i]);
+            for (int i = 0; i < 16; ++i) S[i >> 2][i & 3] = i >= from && i <= to ? S[i >> 2][i & 3] : -INFINITY;
         }
-        const float next = fmaxf(m, ceilf(column_max(top + e)));
-        const float base = next == -INFINITY ? 0.f : next;
-        const float alpha = __builtin_amdgcn_exp2f(m - base);
-        m = next;
-        float sum = 0.f;
+        float best = S[0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float s = __builtin_fmaf(S[i >> 2][i & 3], scale, e - base + 15.f);
-            const bool seen = i >= from && i <= to;
-            const float v = seen ? __builtin_amdgcn_exp2f(s) : 0.f;
-            sum += v;
-            w[i] = seen ? v * mant : 0.f;
+        for (int i = 1; i < 16; ++i) best = fmaxf(best, S[i >> 2][i & 3]);
+        const float top = best * scale + e;
+        if (__builtin_amdgcn_ballot_w64(top > m)) {
+            const float next = fmaxf(m, ceilf(column_max(top)));
+            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < D; ++d) O[d] *= alpha;
         }
-        l = l * alpha + ldexpf(sum, -e);
+        const float add = e - (m == -INFINITY ? 0.f : m) + 15.f;
         half8 ph[2], pl[2];
-        split_f16(w, ph[0], pl[0]);
-        split_f16(w + 8, ph[1], pl[1]);
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const half8 v0 = codes_f16(vr[d].x, vr[d].y), v1 = codes_f16(vr[d].z, vr[d].w);
-            f32x4 o = O[d] * alpha;
-            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], o, 0, 0, 0);
-            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], o, 0, 0, 0);
-            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], o, 0, 0, 0);
-            O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], o, 0, 0, 0);
+        for (int n = 0; n < 2; ++n) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * n + (i >> 2)][i & 3], scale, add));
+                sum[i & 1] += v;
+                w[i] = v * mant;
+            }
+            split_f16(w, ph[n], pl[n]);
+        }
+        l += ldexpf(sum[0] + sum[1], -e);
+#pragma unroll
+        for (int d0 = 0; d0 < D; d0 += 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[d] = kAhead ? vr[d0 + d] : *(const uint4 *)(vb + 256 * (d0 + d));
+            half8 x[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) x[d] = codes_f16(v[d].x, v[d].y);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) O[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[d], ph[0], O[d0 + d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) O[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[d], pl[0], O[d0 + d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) x[d] = codes_f16(v[d].z, v[d].w);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) O[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[d], ph[1], O[d0 + d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) O[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[d], pl[1], O[d0 + d], 0, 0, 0);
+        }
+        if constexpr (kAhead) {
+            fetch_v(step + kWaves);
+            look(step + 2 * kWaves);
         }
     }
     l = column_sum(l);
 
     // The wavefronts' partial softmaxes meet in LDS, 64 columns at a time.
-    __shared__ float ml[2][kWaves][kRows];
-    __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
     if (part == 0) {
         ml[0][wave][col] = m;
         ml[1][wave][col] = l;
@@ -270,6 +335,7 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     const int mrow = threadIdx.x >> 4, mcol = 4 * (threadIdx.x & 15);   // this thread's output: 4 columns of a row
     const int out_row = kRows * tile + mrow;
     const size_t prow = ((size_t)r * a.max_tokens * group + out_row) * c.kv_heads + kvh;
+    const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         if (i) __syncthreads();
@@ -290,19 +356,35 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
         if (out_row < rq.rows) {
             if (g.active > 1) {
                 *(f32x4 *)(partials + (prow * splits + sp) * W + 64 * i + mcol) = o;
-                if (i == 0 && mcol == 0) {
-                    float *pm = partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * (prow * splits + sp);
-                    pm[0] = top;
-                    pm[1] = total;
-                }
+                if (i == 0 && mcol == 0)
+                    *(float2 *)(partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W +
+                                2 * (prow * splits + sp)) = make_float2(top, total);
             } else {
                 float *out = a.out + (rq.begin + out_row / group) * a.out_stride +
                              (int64_t)(kvh * group + out_row % group) * W + 64 * i + mcol;
+                const float inverse = total == 0.f ? 0.f : 1.f / total;
+                o *= inverse;
+                if (aligned) {
+                    *(f32x4 *)out = o;
+                } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) out[k] = total == 0.f ? 0.f : o[k] / total;
+                    for (int k = 0; k < 4; ++k) out[k] = o[k];
+                }
             }
         }
     }
+}
+
+template <int W>
+__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Attention a, int splits, int least,
+    int most_rows, float *__restrict__ partials)
+{
+    __shared__ float ml[2][kWaves][kRows];
+    __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
+    int x = blockIdx.x;
+    const int kvh = x % a.cache.kv_heads;
+    x /= a.cache.kv_heads;
+    few_rows<W>(a, blockIdx.y, kvh, x % splits, x / splits, splits, least, most_rows, partials, ml, po);
 }
 
 // LDS writes and reads of the workgroup up to here; global loads stay in flight.
@@ -381,7 +463,8 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
     const int row = kWideRows * tile + 32 * wave + col, row_in = min(row, rq.rows - 1), token = row_in / group;
     const int head = kvh * group + row_in % group;
     const int64_t p = rq.first + token;
-    const int last = row < rq.rows ? (int)(p < g.highest ? p : g.highest) : -1;
+    // (Rows past the request's last repeat it and are not written.)
+    const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
     // Positions that all of the wavefront's rows see.
     int all_from = first, all_to = last;
@@ -658,9 +741,8 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
             for (int i = 0; i < 4; ++i)
                 *(float4 *)(to + 32 * d + 8 * i) = make_float4(O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]);
         if (h == 0) {
-            float *pm = partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * (prow * splits + sp);
-            pm[0] = m;
-            pm[1] = l;
+            *(float2 *)(partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * (prow * splits + sp)) =
+                make_float2(m, l);
         }
         return;
     }
@@ -698,28 +780,35 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, int splits, int 
     const Range g = range_of(a, rq, row / rows, rows, splits, rows == kRows ? least : 1);
     if (g.active <= 1) return;
     const size_t prow = ((size_t)r * a.max_tokens * group + row) * c.kv_heads + kvh;
-    const float *pm = partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * prow * splits;
-    constexpr int kCols = W / 4, kParts = 256 / kCols < 1 ? 1 : 256 / kCols;
+    const float2 *pm = (const float2 *)(partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W) + prow * splits;
+    constexpr int kCols = W / 4, kParts = 256 / kCols;
     __shared__ f32x4 po[kParts][kCols];
-    const int col = threadIdx.x % kCols, part = threadIdx.x / kCols;
-    float top = -INFINITY;
-    for (int s = 0; s < g.active; ++s) top = fmaxf(top, pm[2 * s]);
-    const float base = top == -INFINITY ? 0.f : top;
+    __shared__ float fs[kMostSplits];
+    const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, part = threadIdx.x / kCols;
+    // Shares' outputs are requested before their weights are known; lane s forms
+    // the weight of share s.
+    const f32x4 *po_at = (const f32x4 *)(partials + prow * splits * W) + col;
+    constexpr int kOnce = kMostSplits / kParts;
+    f32x4 v[kOnce];
+#pragma unroll
+    for (int k = 0; k < kOnce; ++k) v[k] = po_at[(size_t)min(part + kParts * k, g.active - 1) * kCols];
+    const float2 mine = lane < g.active ? pm[lane] : make_float2(-INFINITY, 0.f);
+    const float top = wave_reduce<true>(mine.x), base = top == -INFINITY ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(mine.x - base), total = wave_sum(mine.y * f);
+    if (threadIdx.x < kMostSplits) fs[lane] = f;
+    __syncthreads();
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
-    for (int s = part; s < g.active; s += kParts) {
-        const float f = __builtin_amdgcn_exp2f(pm[2 * s] - base);
-        o += *(const f32x4 *)(partials + (prow * splits + s) * W + 4 * col) * f;
-    }
-    for (int s = 0; s < g.active; ++s) total += pm[2 * s + 1] * __builtin_amdgcn_exp2f(pm[2 * s] - base);
+#pragma unroll
+    for (int k = 0; k < kOnce; ++k) o += v[k] * fs[part + kParts * k];   // (shares past the last weigh 0)
     po[part][col] = o;
     __syncthreads();
     if (part) return;
 #pragma unroll
     for (int k = 1; k < kParts; ++k) o += po[k][col];
     float *out = a.out + (rq.begin + row / group) * a.out_stride + (int64_t)(kvh * group + row % group) * W + 4 * col;
+    const float inverse = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = total == 0.f ? 0.f : o[k] / total;
+    for (int k = 0; k < 4; ++k) out[k] = o[k] * inverse;
 }
 
 // How the work is split: `splits` workgroups at most share a tile's
@@ -748,11 +837,20 @@ Plan plan_of(int requests, int max_tokens, int count, int max_length, int heads,
     int64_t range = max_length;
     if (window && (int64_t)window + max_tokens < range) range = (int64_t)window + max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    const int64_t wanted = tile == kRows ? 1024 : 256, least = tile == kRows ? kWaves : 4;
-    int64_t splits = wanted / groups;
-    if (splits > 64) splits = 64;
-    if (splits > steps / least) splits = steps / least;
-    p.splits = splits < 1 ? 1 : (int)splits;
+    // About 2048 shares of all the requests if each were as long as the longest:
+    // ragged batches then have shares of about equal length, and a few requests
+    // fill the chip. A share is at least a step per wavefront (wide tiles, which
+    // fill a CU each: two rounds of them).
+    int64_t splits;
+    if (tile == kRows) {
+        const int64_t share = (groups * steps + 2047) / 2048;
+        p.least = share < kWaves ? kWaves : (int)share;
+        splits = (steps + p.least - 1) / p.least;
+    } else {
+        splits = 256 / groups;
+        if (splits > steps / 4) splits = steps / 4;
+    }
+    p.splits = splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : (int)splits;
     return p;
 }
 
