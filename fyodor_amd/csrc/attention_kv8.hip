@@ -23,6 +23,11 @@ constexpr int kWideRows = 32 * kWaves;   // query rows per tile of many
 struct Range {
     int lowest, highest;   // positions, highest < 0: none
     int begin, chunk, active, end;
+
+    // Steps of share sp. The first one has what is left over: the grids begin
+    // with the last shares, so the shorter ones come where others have ended.
+    __device__ __forceinline__ int until(int sp) const { return end - (active - 1 - sp) * chunk; }
+    __device__ __forceinline__ int from(int sp) const { return max(begin, until(sp) - chunk); }
 };
 
 // Request r's rows, the first position and whether it brings any.
@@ -148,7 +153,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
 
     const int *table = a.table + (size_t)r * a.table_stride;
     const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
-    const int begin = g.begin + sp * g.chunk + wave, stop = min(g.begin + (sp + 1) * g.chunk, g.end);
+    const int begin = g.from(sp) + wave, stop = g.until(sp);
     // Lane l reads keys of the granule of 16 positions (l % 16) / 4 of a step and
     // holds scores and values of granule l / 16. Everything is read
     // unconditionally (positions past the last one lead to page 0).
@@ -381,10 +386,8 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
 {
     __shared__ float ml[2][kWaves][kRows];
     __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
-    int x = blockIdx.x;
-    const int kvh = x % a.cache.kv_heads;
-    x /= a.cache.kv_heads;
-    few_rows<W>(a, blockIdx.y, kvh, x % splits, x / splits, splits, least, most_rows, partials, ml, po);
+    few_rows<W>(a, blockIdx.y, blockIdx.x % a.cache.kv_heads, splits - 1 - (int)blockIdx.z, blockIdx.x / a.cache.kv_heads,
+                splits, least, most_rows, partials, ml, po);
 }
 
 // LDS writes and reads of the workgroup up to here; global loads stay in flight.
@@ -452,8 +455,8 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
     int x = blockIdx.x;
     const int kvh = x % c.kv_heads;
     x /= c.kv_heads;
-    const int sp = x % splits;
-    const TileOf at_tile = tile_of(a, most_rows, x / splits);
+    const int tiles = gridDim.x / (c.kv_heads * splits), sp = splits - 1 - x / tiles;
+    const TileOf at_tile = tile_of(a, most_rows, x % tiles);
     const int r = at_tile.request, tile = at_tile.tile;
     if (r < 0) return;
     const Request rq = request_of(a, r);
@@ -479,7 +482,7 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
     const int *table = a.table + (size_t)r * a.table_stride;
     const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
     // This group's steps: begin, begin + KS, ...
-    const int begin = g.begin + sp * g.chunk + ks, stop = min(g.begin + (sp + 1) * g.chunk, g.end);
+    const int begin = g.from(sp) + ks, stop = g.until(sp);
     const int rounds = (stop - (begin - ks) + KS - 1) / KS;   // the same for every group
     // Table entries are read a round before the codes they lead to, and
     // everything unconditionally (positions past the last one lead to page 0):
@@ -866,8 +869,8 @@ hipError_t launch_rows(const Kv8Attention &a, Plan p, float *partials, hipStream
     const int64_t each = (int64_t)p.splits * a.cache.kv_heads;
     if (p.most_rows) {
         const int64_t most = rows < p.most_rows ? rows : p.most_rows;
-        hipLaunchKernelGGL((kv8_rows<W>), dim3((unsigned)((most + kRows - 1) / kRows * each), (unsigned)a.requests),
-                           dim3(64 * kWaves), 0, s, a, p.splits, p.least, p.most_rows, partials);
+        hipLaunchKernelGGL((kv8_rows<W>), dim3((unsigned)((most + kRows - 1) / kRows * a.cache.kv_heads),
+                                               (unsigned)a.requests, (unsigned)p.splits), dim3(64 * kWaves), 0, s, a, p.splits, p.least, p.most_rows, partials);
     }
     if constexpr (W <= 256) {
         if (rows > p.most_rows) {
