@@ -206,8 +206,15 @@ NYA_HIP_EXPORT int nya_hip_kv8_attention_bytes(const nya_hip_kv8 *cache, size_t 
     size_t max_tokens, size_t max_length, size_t heads, size_t window, size_t *bytes)
 {
     if (!bytes || !attention_ok(cache, count, requests, max_tokens, max_length, heads, window)) return 1;
-    *bytes = kv8_attention_workspace((int)requests, (int)max_tokens, (int)count, (int)max_length, (int)heads,
-                                     (int)cache->kv_heads, (int)cache->width, (int)window);
+    Kv8Attention a = {};
+    a.cache = cache_of(cache);
+    a.count = (int)count;
+    a.requests = (int)requests;
+    a.max_tokens = (int)max_tokens;
+    a.max_length = (int)max_length;
+    a.heads = (int)heads;
+    a.window = (int)window;
+    *bytes = kv8_attention_workspace(a);
     return 0;
 }
 

@@ -30,6 +30,25 @@ struct Range {
     __device__ __forceinline__ int from(int sp) const { return max(begin, until(sp) - chunk); }
 };
 
+// How the positions of tiles are shared out: among `most` workgroups, at least
+// `least` steps each, which leave their rows in the workspace (room for `rows`
+// rows of every request and KV head).
+struct Share {
+    float *o;
+    float2 *ml;
+};
+struct Split {
+    int most, least, rows;
+    float *partials;
+
+    __device__ __forceinline__ Share share(const Kv8Attention &a, int r, int kvh, int row, int sp, int width) const
+    {
+        const size_t at = (((size_t)r * rows + row) * a.cache.kv_heads + kvh) * most + sp;
+        return {partials + at * width,
+                (float2 *)(partials + (size_t)a.requests * rows * a.cache.kv_heads * most * width) + at};
+    }
+};
+
 // Request r's rows, the first position and whether it brings any.
 struct Request {
     int begin, rows;   // first row; rows of one KV head: tokens x group
@@ -127,8 +146,8 @@ __device__ __forceinline__ float column_sum(float v)
 // step are requested as soon as the last step's are used up, pages a step
 // before that.
 template <int W>
-__device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, int sp, int tile, int splits, int least,
-    int most_rows, float *__restrict__ partials, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
+__device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, int sp, int tile, const Split &split,
+    int most_rows, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
 {
     constexpr int C = W / 64, D = W / 16;
     constexpr bool kAhead = W <= 256;   // room for a step's K and V in registers
@@ -138,7 +157,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
     const int group = a.heads / c.kv_heads;
     const Request rq = request_of(a, r);
     if (kRows * tile >= rq.rows || rq.rows > most_rows) return;
-    const Range g = range_of(a, rq, tile, kRows, splits, least);
+    const Range g = range_of(a, rq, tile, kRows, split.most, split.least);
     if (sp >= g.active) return;
 
     // Rows past the request's last repeat it and are not written.
@@ -339,7 +358,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
     }
     const int mrow = threadIdx.x >> 4, mcol = 4 * (threadIdx.x & 15);   // this thread's output: 4 columns of a row
     const int out_row = kRows * tile + mrow;
-    const size_t prow = ((size_t)r * a.max_tokens * group + out_row) * c.kv_heads + kvh;
+    const Share to = split.share(a, r, kvh, out_row, sp, W);
     const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -360,10 +379,8 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
         }
         if (out_row < rq.rows) {
             if (g.active > 1) {
-                *(f32x4 *)(partials + (prow * splits + sp) * W + 64 * i + mcol) = o;
-                if (i == 0 && mcol == 0)
-                    *(float2 *)(partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W +
-                                2 * (prow * splits + sp)) = make_float2(top, total);
+                *(f32x4 *)(to.o + 64 * i + mcol) = o;
+                if (i == 0 && mcol == 0) *to.ml = make_float2(top, total);
             } else {
                 float *out = a.out + (rq.begin + out_row / group) * a.out_stride +
                              (int64_t)(kvh * group + out_row % group) * W + 64 * i + mcol;
@@ -381,13 +398,12 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
 }
 
 template <int W>
-__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Attention a, int splits, int least,
-    int most_rows, float *__restrict__ partials)
+__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Attention a, Split split, int most_rows)
 {
     __shared__ float ml[2][kWaves][kRows];
     __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
-    few_rows<W>(a, blockIdx.y, blockIdx.x % a.cache.kv_heads, splits - 1 - (int)blockIdx.z, blockIdx.x / a.cache.kv_heads,
-                splits, least, most_rows, partials, ml, po);
+    few_rows<W>(a, blockIdx.y, blockIdx.x % a.cache.kv_heads, split.most - 1 - (int)blockIdx.z,
+                blockIdx.x / a.cache.kv_heads, split, most_rows, ml, po);
 }
 
 // LDS writes and reads of the workgroup up to here; global loads stay in flight.
@@ -438,7 +454,7 @@ __device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, 
 // wavefronts.
 template <int W, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
-void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ partials)
+void kv8_wide(Kv8Attention a, Split split, int most_rows)
 {
     constexpr int M = W / 16;       // MFMA steps of a score
     constexpr int D = W / 32;       // output tiles
@@ -455,12 +471,12 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
     int x = blockIdx.x;
     const int kvh = x % c.kv_heads;
     x /= c.kv_heads;
-    const int tiles = gridDim.x / (c.kv_heads * splits), sp = splits - 1 - x / tiles;
+    const int tiles = gridDim.x / (c.kv_heads * split.most), sp = split.most - 1 - x / tiles;
     const TileOf at_tile = tile_of(a, most_rows, x % tiles);
     const int r = at_tile.request, tile = at_tile.tile;
     if (r < 0) return;
     const Request rq = request_of(a, r);
-    const Range g = range_of(a, rq, tile, kWideRows, splits, 1);
+    const Range g = range_of(a, rq, tile, kWideRows, split.most, split.least);
     if (sp >= g.active) return;
 
     const int row = kWideRows * tile + 32 * wave + col, row_in = min(row, rq.rows - 1), token = row_in / group;
@@ -736,17 +752,14 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
     }
     if (row >= rq.rows) return;
     if (g.active > 1) {
-        const size_t prow = ((size_t)r * a.max_tokens * group + row) * c.kv_heads + kvh;
-        float *to = partials + (prow * splits + sp) * W + 4 * h;
+        const Share to = split.share(a, r, kvh, row, sp, W);
 #pragma unroll
         for (int d = 0; d < D; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *(float4 *)(to + 32 * d + 8 * i) = make_float4(O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]);
-        if (h == 0) {
-            *(float2 *)(partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W + 2 * (prow * splits + sp)) =
-                make_float2(m, l);
-        }
+                *(float4 *)(to.o + 32 * d + 8 * i + 4 * h) =
+                    make_float4(O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]);
+        if (h == 0) *to.ml = make_float2(m, l);
         return;
     }
     float *out = a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W + 4 * h;
@@ -770,32 +783,30 @@ void kv8_wide(Kv8Attention a, int splits, int most_rows, float *__restrict__ par
 }
 
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over a row's shares.
-// Workgroup (row of a KV head and request).
-template <int W>
-__global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, int splits, int least,
-    int most_rows, const float *__restrict__ partials)
+// Workgroup (row of a KV head and request) of the requests of the rows' kind.
+template <int W, bool WIDE>
+__global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split split, int most_rows)
 {
     const Kv8 &c = a.cache;
     const int group = a.heads / c.kv_heads, r = blockIdx.y, kvh = blockIdx.x % c.kv_heads, row = blockIdx.x / c.kv_heads;
     const Request rq = request_of(a, r);
-    if (row >= rq.rows) return;
-    const int rows = rq.rows > most_rows ? kWideRows : kRows;
-    const Range g = range_of(a, rq, row / rows, rows, splits, rows == kRows ? least : 1);
+    if (row >= rq.rows || WIDE != (rq.rows > most_rows)) return;
+    constexpr int kTile = WIDE ? kWideRows : kRows;
+    const Range g = range_of(a, rq, row / kTile, kTile, split.most, split.least);
     if (g.active <= 1) return;
-    const size_t prow = ((size_t)r * a.max_tokens * group + row) * c.kv_heads + kvh;
-    const float2 *pm = (const float2 *)(partials + (size_t)a.requests * a.max_tokens * a.heads * splits * W) + prow * splits;
+    const Share from = split.share(a, r, kvh, row, 0, W);
     constexpr int kCols = W / 4, kParts = 256 / kCols;
     __shared__ f32x4 po[kParts][kCols];
     __shared__ float fs[kMostSplits];
     const int lane = threadIdx.x & 63, col = threadIdx.x % kCols, part = threadIdx.x / kCols;
     // Shares' outputs are requested before their weights are known; lane s forms
     // the weight of share s.
-    const f32x4 *po_at = (const f32x4 *)(partials + prow * splits * W) + col;
+    const f32x4 *po_at = (const f32x4 *)from.o + col;
     constexpr int kOnce = kMostSplits / kParts;
     f32x4 v[kOnce];
 #pragma unroll
     for (int k = 0; k < kOnce; ++k) v[k] = po_at[(size_t)min(part + kParts * k, g.active - 1) * kCols];
-    const float2 mine = lane < g.active ? pm[lane] : make_float2(-INFINITY, 0.f);
+    const float2 mine = lane < g.active ? from.ml[lane] : make_float2(-INFINITY, 0.f);
     const float top = wave_reduce<true>(mine.x), base = top == -INFINITY ? 0.f : top;
     const float f = __builtin_amdgcn_exp2f(mine.x - base), total = wave_sum(mine.y * f);
     if (threadIdx.x < kMostSplits) fs[lane] = f;
@@ -814,13 +825,6 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, int splits, int 
     for (int k = 0; k < 4; ++k) out[k] = o[k] * inverse;
 }
 
-// How the work is split: `splits` workgroups at most share a tile's
-// positions, in tiles of a few rows at least `least` steps each; requests of
-// more than most_rows rows (of one KV head) run in wide tiles.
-struct Plan {
-    int splits, least, most_rows;
-};
-
 // Wide tiles that a step can have: every request's last one may be short.
 int64_t wide_tiles(int requests, int max_tokens, int count, int group)
 {
@@ -829,83 +833,113 @@ int64_t wide_tiles(int requests, int max_tokens, int count, int group)
     return each < all ? each : all;
 }
 
-Plan plan_of(int requests, int max_tokens, int count, int max_length, int heads, int kv_heads, int width, int window)
+// Requests of more than most_rows rows (of one KV head) run in wide tiles.
+struct Plan {
+    int most_rows;
+    bool any_few, any_wide;
+    Split few, wide;
+};
+
+size_t share_bytes(const Kv8Attention &a, const Split &s)
 {
-    const int64_t rows = (int64_t)max_tokens * (heads / kv_heads);
-    Plan p = {1, kWaves, INT32_MAX};
-    if (width <= 256 && rows > 32) p.most_rows = requests == 1 ? 0 : 32;
-    const int tile = rows > p.most_rows ? kWideRows : kRows;
-    const int64_t groups = (tile == kRows ? (rows + kRows - 1) / kRows * requests
-                                          : wide_tiles(requests, max_tokens, count, heads / kv_heads)) * kv_heads;
-    int64_t range = max_length;
-    if (window && (int64_t)window + max_tokens < range) range = (int64_t)window + max_tokens;
+    return (size_t)a.requests * s.rows * a.cache.kv_heads * (a.cache.width + 2) * sizeof(float);
+}
+
+Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
+{
+    const int group = a.heads / a.cache.kv_heads, width = a.cache.width;
+    const int64_t rows = (int64_t)a.max_tokens * group;
+    int64_t range = a.max_length;
+    if (a.window && (int64_t)a.window + a.max_tokens < range) range = (int64_t)a.window + a.max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    // About 2048 shares of all the requests if each were as long as the longest:
-    // ragged batches then have shares of about equal length, and a few requests
-    // fill the chip. A share is at least a step per wavefront (wide tiles, which
-    // fill a CU each: two rounds of them).
-    int64_t splits;
-    if (tile == kRows) {
-        const int64_t share = (groups * steps + 2047) / 2048;
-        p.least = share < kWaves ? kWaves : (int)share;
-        splits = (steps + p.least - 1) / p.least;
-    } else {
-        splits = 256 / groups;
-        if (splits > steps / 4) splits = steps / 4;
+    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, nullptr}, {1, 4, 0, nullptr}};
+    if (width <= 256 && rows > 32) {
+        // A single request of many rows is all wide.
+        p.most_rows = a.requests == 1 ? 0 : 32;
+        p.any_wide = true;
+        p.any_few = a.requests > 1;
     }
-    p.splits = splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : (int)splits;
+    if (p.any_few) {
+        p.few.rows = (int)(rows < p.most_rows ? rows : p.most_rows);
+        const int64_t tiles = (int64_t)(p.few.rows + kRows - 1) / kRows * a.requests * a.cache.kv_heads;
+        // Fewer tiles than CUs: shares for three workgroups per CU (one at widths
+        // that fill a CU's registers), at least a step per wavefront. Enough
+        // tiles: none, sharing costs about 6 us (32 requests of 2048 positions, 8
+        // heads of 128, us: whole 25, halves 31, quarters 34), but in long contexts,
+        // where the requests' lengths differ by more (64 of 500 to 8192: whole 105,
+        // 2048 shares were they all long 97).
+        const int64_t wanted = tiles < 256 ? (width <= 128 ? 768 : 256) : steps >= 96 ? 2048 : 0;
+        const int64_t share = wanted ? (tiles * steps + wanted - 1) / wanted : steps;
+        if (share > p.few.least) p.few.least = (int)share;
+        const int64_t most = (steps + p.few.least - 1) / p.few.least;
+        p.few.most = most > kMostSplits ? kMostSplits : (int)most;
+    }
+    if (p.any_wide) {
+        // Wide tiles fill a CU each; their rows are too many to be left in memory
+        // for less than a chip that is half empty.
+        p.wide.rows = (int)rows;
+        const int64_t tiles = wide_tiles(a.requests, a.max_tokens, a.count, group) * a.cache.kv_heads;
+        int64_t most = 256 / tiles;
+        if (most > steps / 4) most = steps / 4;
+        p.wide.most = most < 1 ? 1 : most > kMostSplits ? kMostSplits : (int)most;
+    }
+    size_t taken = 0;
+    for (Split *s : {&p.few, &p.wide}) {
+        if (s->most == 1) continue;
+        const size_t each = share_bytes(a, *s);
+        if (bytes / each < (size_t)s->most) s->most = bytes / each < 2 ? 1 : (int)(bytes / each);
+        if (s->most == 1) continue;
+        if (workspace) s->partials = workspace + taken;
+        taken += s->most * each / sizeof(float);
+        bytes -= s->most * each;
+    }
     return p;
 }
 
-size_t row_bytes(int requests, int max_tokens, int heads, int width)
-{
-    return (size_t)requests * max_tokens * heads * (width + 2) * sizeof(float);
-}
-
 template <int W>
-hipError_t launch_rows(const Kv8Attention &a, Plan p, float *partials, hipStream_t s)
+hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
 {
-    const int64_t rows = (int64_t)a.max_tokens * (a.heads / a.cache.kv_heads);
-    const int64_t each = (int64_t)p.splits * a.cache.kv_heads;
-    if (p.most_rows) {
-        const int64_t most = rows < p.most_rows ? rows : p.most_rows;
-        hipLaunchKernelGGL((kv8_rows<W>), dim3((unsigned)((most + kRows - 1) / kRows * a.cache.kv_heads),
-                                               (unsigned)a.requests, (unsigned)p.splits), dim3(64 * kWaves), 0, s, a, p.splits, p.least, p.most_rows, partials);
+    const int group = a.heads / a.cache.kv_heads;
+    const unsigned requests = a.requests, kv_heads = a.cache.kv_heads;
+    if (p.any_few) {
+        const unsigned tiles = (unsigned)((p.few.rows + kRows - 1) / kRows);
+        hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, requests, (unsigned)p.few.most), dim3(64 * kWaves), 0, s, a,
+                           p.few, p.most_rows);
+        if (p.few.most > 1)
+            hipLaunchKernelGGL((kv8_join<W, false>), dim3((unsigned)p.few.rows * kv_heads, requests), dim3(256), 0, s, a,
+                               p.few, p.most_rows);
     }
     if constexpr (W <= 256) {
-        if (rows > p.most_rows) {
+        if (p.any_wide) {
             constexpr int KS = W <= 128 ? 2 : 1;
-            hipLaunchKernelGGL((kv8_wide<W, KS>), dim3((unsigned)(wide_tiles(a.requests, a.max_tokens, a.count,
-                                                                             a.heads / a.cache.kv_heads) * each)),
-                               dim3(256 * KS), 0, s, a, p.splits, p.most_rows, partials);
+            const int64_t tiles = wide_tiles(a.requests, a.max_tokens, a.count, group);
+            hipLaunchKernelGGL((kv8_wide<W, KS>), dim3((unsigned)(tiles * p.wide.most * kv_heads)), dim3(256 * KS), 0, s, a,
+                               p.wide, p.most_rows);
+            if (p.wide.most > 1)
+                hipLaunchKernelGGL((kv8_join<W, true>), dim3((unsigned)p.wide.rows * kv_heads, requests), dim3(256), 0, s, a,
+                                   p.wide, p.most_rows);
         }
     }
-    if (p.splits > 1)
-        hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)(a.max_tokens * a.heads), (unsigned)a.requests), dim3(256), 0,
-                           s, a, p.splits, p.least, p.most_rows, partials);
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t kv8_attention_workspace(int requests, int max_tokens, int count, int max_length, int heads, int kv_heads,
-    int width, int window)
+size_t kv8_attention_workspace(const Kv8Attention &a)
 {
-    const Plan p = plan_of(requests, max_tokens, count, max_length, heads, kv_heads, width, window);
-    return p.splits > 1 ? p.splits * row_bytes(requests, max_tokens, heads, width) : 0;
+    const Plan p = plan_of(a, nullptr, SIZE_MAX);
+    return (p.few.most > 1 ? p.few.most * share_bytes(a, p.few) : 0) +
+           (p.wide.most > 1 ? p.wide.most * share_bytes(a, p.wide) : 0);
 }
 
 hipError_t launch_kv8_attention(const Kv8Attention &a, void *workspace, size_t workspace_bytes, hipStream_t s)
 {
-    Plan p = plan_of(a.requests, a.max_tokens, a.count, a.max_length, a.heads, a.cache.kv_heads, a.cache.width, a.window);
-    const size_t each = row_bytes(a.requests, a.max_tokens, a.heads, a.cache.width);
-    if (workspace_bytes / each < (size_t)p.splits) p.splits = (int)(workspace_bytes / each);
-    if (p.splits < 1) p.splits = 1;
+    const Plan p = plan_of(a, (float *)workspace, workspace ? workspace_bytes : 0);
     switch (a.cache.width) {
-    case 64: return launch_rows<64>(a, p, (float *)workspace, s);
-    case 128: return launch_rows<128>(a, p, (float *)workspace, s);
-    case 256: return launch_rows<256>(a, p, (float *)workspace, s);
-    default: return launch_rows<512>(a, p, (float *)workspace, s);
+    case 64: return launch_width<64>(a, p, s);
+    case 128: return launch_width<128>(a, p, s);
+    case 256: return launch_width<256>(a, p, s);
+    default: return launch_width<512>(a, p, s);
     }
 }
 

@@ -56,8 +56,8 @@ struct Kv8Attention {
     int table_stride, requests, max_tokens, max_length, heads, window;
     float scale;
 };
-size_t kv8_attention_workspace(int requests, int max_tokens, int count, int max_length, int heads, int kv_heads,
-    int width, int window);
+// Of the arguments' sizes alone.
+size_t kv8_attention_workspace(const Kv8Attention &a);
 hipError_t launch_kv8_attention(const Kv8Attention &a, void *workspace, size_t workspace_bytes, hipStream_t s);
 
 }  // namespace fy
