@@ -31,21 +31,20 @@ struct Range {
 };
 
 // How the positions of tiles are shared out: among `most` workgroups, at least
-// `least` steps each, which leave their rows in the workspace (room for `rows`
-// rows of every request and KV head).
+// `least` steps each, which leave their rows (and each row's maximum and sum)
+// in the workspace: room for `places` places of `tile` rows, for every KV head.
 struct Share {
     float *o;
     float2 *ml;
 };
 struct Split {
-    int most, least, rows;
+    int most, least, tile, places;
     float *partials;
 
-    __device__ __forceinline__ Share share(const Kv8Attention &a, int r, int kvh, int row, int sp, int width) const
+    __device__ __forceinline__ Share share(int kv_heads, int place, int kvh, int row, int sp, int width) const
     {
-        const size_t at = (((size_t)r * rows + row) * a.cache.kv_heads + kvh) * most + sp;
-        return {partials + at * width,
-                (float2 *)(partials + (size_t)a.requests * rows * a.cache.kv_heads * most * width) + at};
+        const size_t at = (((size_t)place * kv_heads + kvh) * tile + row) * most + sp;
+        return {partials + at * width, (float2 *)(partials + (size_t)places * kv_heads * tile * most * width) + at};
     }
 };
 
@@ -358,7 +357,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
     }
     const int mrow = threadIdx.x >> 4, mcol = 4 * (threadIdx.x & 15);   // this thread's output: 4 columns of a row
     const int out_row = kRows * tile + mrow;
-    const Share to = split.share(a, r, kvh, out_row, sp, W);
+    const Share to = split.share(c.kv_heads, r, kvh, out_row, sp, W);
     const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -752,7 +751,7 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
     }
     if (row >= rq.rows) return;
     if (g.active > 1) {
-        const Share to = split.share(a, r, kvh, row, sp, W);
+        const Share to = split.share(c.kv_heads, x % tiles, kvh, row - kWideRows * tile, sp, W);
 #pragma unroll
         for (int d = 0; d < D; ++d)
 #pragma unroll
@@ -783,18 +782,17 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
 }
 
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over a row's shares.
-// Workgroup (row of a KV head and request) of the requests of the rows' kind.
-template <int W, bool WIDE>
+// Requests of a few rows: workgroup (row of a KV head and request).
+template <int W>
 __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split split, int most_rows)
 {
     const Kv8 &c = a.cache;
     const int group = a.heads / c.kv_heads, r = blockIdx.y, kvh = blockIdx.x % c.kv_heads, row = blockIdx.x / c.kv_heads;
     const Request rq = request_of(a, r);
-    if (row >= rq.rows || WIDE != (rq.rows > most_rows)) return;
-    constexpr int kTile = WIDE ? kWideRows : kRows;
-    const Range g = range_of(a, rq, row / kTile, kTile, split.most, split.least);
+    if (row >= rq.rows || rq.rows > most_rows) return;
+    const Range g = range_of(a, rq, row / kRows, kRows, split.most, split.least);
     if (g.active <= 1) return;
-    const Share from = split.share(a, r, kvh, row, 0, W);
+    const Share from = split.share(c.kv_heads, r, kvh, row, 0, W);
     constexpr int kCols = W / 4, kParts = 256 / kCols;
     __shared__ f32x4 po[kParts][kCols];
     __shared__ float fs[kMostSplits];
@@ -825,6 +823,46 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split split, int
     for (int k = 0; k < 4; ++k) out[k] = o[k] * inverse;
 }
 
+// Wide tiles: workgroup (tile and KV head, 16 of its rows), a wavefront every
+// fourth row.
+template <int W>
+__global__ __launch_bounds__(256) void kv8_join_wide(Kv8Attention a, Split split, int most_rows)
+{
+    const Kv8 &c = a.cache;
+    const int kvh = blockIdx.x % c.kv_heads, lane = threadIdx.x & 63, group = a.heads / c.kv_heads;
+    const TileOf at = tile_of(a, most_rows, blockIdx.x / c.kv_heads);
+    if (at.request < 0) return;
+    const Request rq = request_of(a, at.request);
+    const Range g = range_of(a, rq, at.tile, kWideRows, split.most, split.least);
+    if (g.active <= 1) return;
+    constexpr int kCols = W / 64;   // columns per lane
+    const int first_row = kWideRows * at.tile + 16 * blockIdx.y;
+    for (int row = first_row + (threadIdx.x >> 6); row < min(first_row + 16, rq.rows); row += 4) {
+        const Share from = split.share(c.kv_heads, blockIdx.x / c.kv_heads, kvh, row - kWideRows * at.tile, 0, W);
+        const float2 mine = lane < g.active ? from.ml[lane] : make_float2(-INFINITY, 0.f);
+        const float top = wave_reduce<true>(mine.x), base = top == -INFINITY ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(mine.x - base), total = wave_sum(mine.y * f);
+        float o[kCols] = {};
+        for (int s = 0; s < g.active; s += 4) {
+            float v[4][kCols];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < kCols; ++e) v[n][e] = from.o[min(s + n, g.active - 1) * W + 64 * e + lane];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float weight = lane_value(f, s + n);   // 0 past the last share
+#pragma unroll
+                for (int e = 0; e < kCols; ++e) o[e] += v[n][e] * weight;
+            }
+        }
+        float *out = a.out + (rq.begin + row / group) * a.out_stride + (int64_t)(kvh * group + row % group) * W + lane;
+        const float inverse = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) out[64 * e] = o[e] * inverse;
+    }
+}
+
 // Wide tiles that a step can have: every request's last one may be short.
 int64_t wide_tiles(int requests, int max_tokens, int count, int group)
 {
@@ -842,7 +880,7 @@ struct Plan {
 
 size_t share_bytes(const Kv8Attention &a, const Split &s)
 {
-    return (size_t)a.requests * s.rows * a.cache.kv_heads * (a.cache.width + 2) * sizeof(float);
+    return (size_t)s.places * s.tile * a.cache.kv_heads * (a.cache.width + 2) * sizeof(float);
 }
 
 Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
@@ -852,16 +890,22 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
     int64_t range = a.max_length;
     if (a.window && (int64_t)a.window + a.max_tokens < range) range = (int64_t)a.window + a.max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, nullptr}, {1, 4, 0, nullptr}};
-    if (width <= 256 && rows > 32) {
-        // A single request of many rows is all wide.
+    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, 0, nullptr}, {1, 4, kWideRows, 0, nullptr}};
+    if (width <= 256 && rows > 64) {
+        // Up to 64 rows are fewer keys read again than wide tiles leave empty (8
+        // requests of 5 tokens of 32 heads over 4 of 64: 12 us, wide 18 to 23). In
+        // a batch with longer ones, which pays for every place of a tile that
+        // a request of a few rows might have, 32; a single request is all wide.
         p.most_rows = a.requests == 1 ? 0 : 32;
         p.any_wide = true;
         p.any_few = a.requests > 1;
     }
     if (p.any_few) {
-        p.few.rows = (int)(rows < p.most_rows ? rows : p.most_rows);
-        const int64_t tiles = (int64_t)(p.few.rows + kRows - 1) / kRows * a.requests * a.cache.kv_heads;
+        p.few.tile = (int)(rows < p.most_rows ? rows : p.most_rows);
+        p.few.places = a.requests;
+        // In a mixed batch most of these requests bring a token each.
+        const int64_t each = p.any_wide ? group : p.few.tile;
+        const int64_t tiles = (each + kRows - 1) / kRows * a.requests * a.cache.kv_heads;
         // Fewer tiles than CUs: shares for three workgroups per CU (one at widths
         // that fill a CU's registers), at least a step per wavefront. Enough
         // tiles: none, sharing costs about 6 us (32 requests of 2048 positions, 8
@@ -875,16 +919,17 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         p.few.most = most > kMostSplits ? kMostSplits : (int)most;
     }
     if (p.any_wide) {
-        // Wide tiles fill a CU each; their rows are too many to be left in memory
-        // for less than a chip that is half empty.
-        p.wide.rows = (int)rows;
-        const int64_t tiles = wide_tiles(a.requests, a.max_tokens, a.count, group) * a.cache.kv_heads;
-        int64_t most = 256 / tiles;
+        // Wide tiles fill a CU each, so they are split while they leave CUs idle: as
+        // many tiles as the rows make, short last ones left out (24 requests, two
+        // of them prompts of 256 tokens, 32 heads of 128: 65 us whole, in halves).
+        p.wide.places = (int)wide_tiles(a.requests, a.max_tokens, a.count, group);
+        const double tiles = (double)a.count * group / kWideRows * a.cache.kv_heads;
+        int64_t most = (int64_t)(256 / (tiles < 1 ? 1 : tiles) + 0.4);
         if (most > steps / 4) most = steps / 4;
         p.wide.most = most < 1 ? 1 : most > kMostSplits ? kMostSplits : (int)most;
     }
     size_t taken = 0;
-    for (Split *s : {&p.few, &p.wide}) {
+    for (Split *s : {&p.wide, &p.few}) {
         if (s->most == 1) continue;
         const size_t each = share_bytes(a, *s);
         if (bytes / each < (size_t)s->most) s->most = bytes / each < 2 ? 1 : (int)(bytes / each);
@@ -902,11 +947,11 @@ hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
     const int group = a.heads / a.cache.kv_heads;
     const unsigned requests = a.requests, kv_heads = a.cache.kv_heads;
     if (p.any_few) {
-        const unsigned tiles = (unsigned)((p.few.rows + kRows - 1) / kRows);
+        const unsigned tiles = (unsigned)((p.few.tile + kRows - 1) / kRows);
         hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, requests, (unsigned)p.few.most), dim3(64 * kWaves), 0, s, a,
                            p.few, p.most_rows);
         if (p.few.most > 1)
-            hipLaunchKernelGGL((kv8_join<W, false>), dim3((unsigned)p.few.rows * kv_heads, requests), dim3(256), 0, s, a,
+            hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)p.few.tile * kv_heads, requests), dim3(256), 0, s, a,
                                p.few, p.most_rows);
     }
     if constexpr (W <= 256) {
@@ -916,7 +961,7 @@ hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
             hipLaunchKernelGGL((kv8_wide<W, KS>), dim3((unsigned)(tiles * p.wide.most * kv_heads)), dim3(256 * KS), 0, s, a,
                                p.wide, p.most_rows);
             if (p.wide.most > 1)
-                hipLaunchKernelGGL((kv8_join<W, true>), dim3((unsigned)p.wide.rows * kv_heads, requests), dim3(256), 0, s, a,
+                hipLaunchKernelGGL((kv8_join_wide<W>), dim3((unsigned)(tiles * kv_heads), kWideRows / 16), dim3(256), 0, s, a,
                                    p.wide, p.most_rows);
         }
     }

@@ -146,19 +146,18 @@ __global__ __launch_bounds__(kPageThreads) void page_tables(PageStep p)
     }
 }
 
-__global__ __launch_bounds__(256) void page_rows(PageStep p)
+// The row's position and slot.
+__device__ __forceinline__ void place_row(const PageStep &p, int row, bool live, int r, int start, int length, int count,
+    int held)
 {
-    const int row = blockIdx.x * 256 + threadIdx.x;
-    if (row >= p.max_tokens) return;
     int position = -1, slot = -1;
-    if (row < p.starts[p.requests]) {
-        const int r = last_from((const uint32_t *)p.starts, p.requests, (uint32_t)row);
+    if (live) {
         // 64 bits: the lengths are the caller's.
-        const int64_t at = (int64_t)max(p.lengths[r], 0) - clamped(p.counts[r], p.max_tokens) + (row - p.starts[r]);
+        const int64_t at = (int64_t)length - count + (row - start);
         position = (int)at;
         if (at >= 0) {
             const int64_t j = at / p.page_tokens;
-            if (j < clamped(p.held[r], p.table_stride)) {
+            if (j < held) {
                 const int page = p.table[(size_t)r * p.table_stride + j];
                 if ((unsigned)page < (unsigned)p.pages) slot = page * p.page_tokens + (int)(at % p.page_tokens);
             }
@@ -166,6 +165,111 @@ __global__ __launch_bounds__(256) void page_rows(PageStep p)
     }
     p.positions[row] = position;
     p.slots[row] = slot;
+}
+
+// The whole step of up to 1024 requests and 8192 rows in one launch: a request
+// per thread, the three prefix sums together, rows from LDS. Bound by its chain
+// of waits (lengths, stack and table, rows).
+__global__ __launch_bounds__(kPageThreads) void page_small(PageStep p)
+{
+    constexpr int kWavesHere = kPageThreads / 64;
+    __shared__ uint32_t parts[3][kWavesHere], first[kPageThreads], starts[kPageThreads];
+    __shared__ int lengths[kPageThreads], counts[kPageThreads], helds[kPageThreads];
+    __shared__ uint32_t served, refused;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool mine = tid < p.requests;
+    const int length = mine ? max(p.lengths[tid], 0) : 0;
+    const uint32_t n = mine ? (uint32_t)clamped(p.counts[tid], p.max_tokens) : 0;
+    int held = mine ? clamped(p.held[tid], p.table_stride) : 0;
+    uint32_t top = (uint32_t)clamped(p.free_count[0], p.pages);
+    const int need = (int)(((uint32_t)length + p.page_tokens - 1) / p.page_tokens);
+    const bool beyond = need > p.table_stride;
+    const uint32_t back = !beyond && held > need ? (uint32_t)(held - need) : 0;
+    const uint32_t grow = !beyond && need > held ? (uint32_t)(need - held) : 0;
+    uint32_t sums[3] = {back, grow, n};
+    const uint32_t most[3] = {INT_MAX, INT_MAX, (uint32_t)p.max_tokens};
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t o = (uint32_t)__shfl_up((int)sums[k], d, 64);
+            if (lane >= d) sums[k] = min(sums[k] + o, most[k]);
+        }
+    if (lane == 63)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) parts[k][wave] = sums[k];
+    if (tid == 0) served = refused = 0;
+    __syncthreads();
+    uint32_t before[3], total[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        uint32_t all = 0, here = 0;
+#pragma unroll
+        for (int w = 0; w < kWavesHere; ++w) {
+            if (w == wave) here = all;
+            all = min(all + parts[k][w], most[k]);
+        }
+        const uint32_t own = (uint32_t)__shfl_up((int)sums[k], 1, 64);
+        before[k] = min(here + (lane ? own : 0), most[k]);
+        total[k] = all;
+    }
+    // 1. Pages past the need, back on the stack.
+    if (total[0]) {
+        first[tid] = before[0];
+        helds[tid] = need;
+        __syncthreads();
+        for (uint32_t i = tid; i < total[0]; i += kPageThreads) {
+            const int k = last_from(first, kPageThreads, i);
+            int *entry = p.table + (size_t)k * p.table_stride + helds[k] + (i - first[k]);
+            if (top + i < (uint32_t)p.pages) p.free_pages[top + i] = *entry;
+            *entry = -1;
+        }
+        top = min(top + total[0], (uint32_t)p.pages);
+        __syncthreads();
+    }
+    if (back) held = need;
+    // 2. Pages for the requests that grow; those served are a prefix of them.
+    const bool fits = before[1] + grow <= top;
+    first[tid] = before[1];
+    helds[tid] = held;
+    lengths[tid] = length;
+    counts[tid] = (int)n;
+    starts[tid] = before[2];
+    if (grow && fits) atomicMax(&served, before[1] + grow);
+    if (beyond || (grow && !fits)) atomicAdd(&refused, 1u);
+    if (grow && fits) held += (int)grow;
+    __syncthreads();
+    for (uint32_t i = tid; i < served; i += kPageThreads) {
+        const int k = last_from(first, kPageThreads, i);
+        p.table[(size_t)k * p.table_stride + helds[k] + (i - first[k])] = p.free_pages[top - 1 - i];
+    }
+    if (mine) {
+        if (back || grow) p.held[tid] = held;
+        p.starts[tid] = (int)before[2];
+    }
+    if (tid == 0) {
+        p.starts[p.requests] = (int)total[2];
+        p.free_count[0] = (int)(top - served);
+        p.free_count[1] = (int)refused;
+    }
+    __syncthreads();
+    helds[tid] = held;
+    __syncthreads();
+    // 3. The rows.
+    for (int row = tid; row < p.max_tokens; row += kPageThreads) {
+        const int r = last_from(starts, p.requests, (uint32_t)row);
+        place_row(p, row, row < (int)total[2], r, (int)starts[r], lengths[r], counts[r], helds[r]);
+    }
+}
+
+__global__ __launch_bounds__(256) void page_rows(PageStep p)
+{
+    const int row = blockIdx.x * 256 + threadIdx.x;
+    if (row >= p.max_tokens) return;
+    const bool live = row < p.starts[p.requests];
+    const int r = last_from((const uint32_t *)p.starts, p.requests, (uint32_t)row);
+    place_row(p, row, live, r, p.starts[r], max(p.lengths[r], 0), clamped(p.counts[r], p.max_tokens),
+              clamped(p.held[r], p.table_stride));
 }
 
 // ---- rotary positions -----------------------------------------------------
@@ -633,6 +737,10 @@ __global__ __launch_bounds__(256) void kv8_load(Kv8 c, const int *__restrict__ s
 
 hipError_t launch_page_step(const PageStep &p, hipStream_t s)
 {
+    if (p.requests <= kPageThreads && p.max_tokens <= 8 * kPageThreads) {
+        hipLaunchKernelGGL(page_small, dim3(1), dim3(kPageThreads), 0, s, p);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(page_tables, dim3(1), dim3(kPageThreads), 0, s, p);
     hipLaunchKernelGGL(page_rows, dim3((unsigned)((p.max_tokens + 255ll) / 256)), dim3(256), 0, s, p);
     return hipGetLastError();
