@@ -895,8 +895,8 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         // Up to 64 rows are fewer keys read again than wide tiles leave empty (8
         // requests of 5 tokens of 32 heads over 4 of 64: 12 us, wide 18 to 23). In
         // a batch with longer ones, which pays for every place of a tile that
-        // a request of a few rows might have, 32; a single request is all wide.
-        p.most_rows = a.requests == 1 ? 0 : 32;
+        // a request of a few rows might have, one tile; a single request is all wide.
+        p.most_rows = a.requests == 1 ? 0 : kRows;
         p.any_wide = true;
         p.any_few = a.requests > 1;
     }
