@@ -199,7 +199,7 @@ static bool attention_ok(const nya_hip_kv8 *cache, size_t count, size_t requests
 {
     return geometry_ok(cache) && rows_fit(count) && requests && requests <= 65535 && max_tokens && max_tokens <= count &&
            some(max_length) && heads_ok(heads, cache->width) && heads % cache->kv_heads == 0 &&
-           count <= ((size_t)1 << 28) / heads && requests <= ((size_t)1 << 21) / cache->kv_heads && window <= (size_t)INT_MAX;
+           count <= ((size_t)1 << 27) / heads && requests <= ((size_t)1 << 21) / cache->kv_heads && window <= (size_t)INT_MAX;
 }
 
 NYA_HIP_EXPORT int nya_hip_kv8_attention_bytes(const nya_hip_kv8 *cache, size_t count, size_t requests,

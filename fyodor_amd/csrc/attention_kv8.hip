@@ -57,7 +57,7 @@ struct Request {
 __device__ __forceinline__ Request request_of(const Kv8Attention &a, int r)
 {
     const int start = a.starts[r], stop = a.starts[r + 1];
-    const int begin = max(start, 0), end = min(stop, a.count), tokens = min(end - begin, a.max_tokens);
+    const int begin = max(start, 0), end = max(min(stop, a.count), 0), tokens = min(end - begin, a.max_tokens);
     return {begin, tokens > 0 ? tokens * (a.heads / a.cache.kv_heads) : 0,
             (int64_t)a.lengths[r] - ((int64_t)stop - begin)};
 }
@@ -137,6 +137,36 @@ __device__ __forceinline__ float column_sum(float v)
     const int b = __builtin_bit_cast(int, v);
     const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
     return halves_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
+}
+
+// The request and the tile of kTile rows of number `index` over the requests
+// of more than most_rows rows, in order (request < 0: past the last). Later
+// tokens see more: a request's last tile comes first.
+struct TileOf {
+    int request, tile;
+};
+
+template <int kTile>
+__device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, int index)
+{
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.requests; base += 64) {
+        const int r = base + lane, rows = r < a.requests ? request_of(a, r).rows : 0;
+        const int tiles = rows > most_rows ? (rows + kTile - 1) / kTile : 0;
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(sum > index);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            return {base + at, __builtin_amdgcn_readlane(sum, at) - 1 - index};
+        }
+        index -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return {-1, 0};
 }
 
 // Requests of a few rows: 16 rows per workgroup, whose wavefronts take every
@@ -401,8 +431,13 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
 {
     __shared__ float ml[2][kWaves][kRows];
     __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
-    few_rows<W>(a, blockIdx.y, blockIdx.x % a.cache.kv_heads, split.most - 1 - (int)blockIdx.z,
-                blockIdx.x / a.cache.kv_heads, split, most_rows, ml, po);
+    TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / a.cache.kv_heads)};
+    if constexpr (W > 256) {   // every request runs here, prompts too
+        if (gridDim.y == 1) at = tile_of<kRows>(a, 0, at.tile);
+        if (at.request < 0) return;
+    }
+    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, split.most - 1 - (int)blockIdx.z, at.tile, split,
+                most_rows, ml, po);
 }
 
 // LDS writes and reads of the workgroup up to here; global loads stay in flight.
@@ -413,35 +448,6 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     __builtin_amdgcn_sched_barrier(0);
-}
-
-// The request and the tile of number `index` over the requests that run in
-// wide tiles, in order (request < 0: past the last). Later tokens see more:
-// a request's last tile comes first.
-struct TileOf {
-    int request, tile;
-};
-
-__device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, int index)
-{
-    const int lane = threadIdx.x & 63;
-    for (int base = 0; base < a.requests; base += 64) {
-        const int r = base + lane, rows = r < a.requests ? request_of(a, r).rows : 0;
-        const int tiles = rows > most_rows ? (rows + kWideRows - 1) / kWideRows : 0;
-        int sum = tiles;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int v = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += v;
-        }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(sum > index);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            return {base + at, __builtin_amdgcn_readlane(sum, at) - 1 - index};
-        }
-        index -= __builtin_amdgcn_readlane(sum, 63);
-    }
-    return {-1, 0};
 }
 
 // Many rows of one request: 32 per wavefront, 128 per group of four
@@ -471,7 +477,7 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
     const int kvh = x % c.kv_heads;
     x /= c.kv_heads;
     const int tiles = gridDim.x / (c.kv_heads * split.most), sp = split.most - 1 - x / tiles;
-    const TileOf at_tile = tile_of(a, most_rows, x % tiles);
+    const TileOf at_tile = tile_of<kWideRows>(a, most_rows, x % tiles);
     const int r = at_tile.request, tile = at_tile.tile;
     if (r < 0) return;
     const Request rq = request_of(a, r);
@@ -830,7 +836,7 @@ __global__ __launch_bounds__(256) void kv8_join_wide(Kv8Attention a, Split split
 {
     const Kv8 &c = a.cache;
     const int kvh = blockIdx.x % c.kv_heads, lane = threadIdx.x & 63, group = a.heads / c.kv_heads;
-    const TileOf at = tile_of(a, most_rows, blockIdx.x / c.kv_heads);
+    const TileOf at = tile_of<kWideRows>(a, most_rows, blockIdx.x / c.kv_heads);
     if (at.request < 0) return;
     const Request rq = request_of(a, at.request);
     const Range g = range_of(a, rq, at.tile, kWideRows, split.most, split.least);
@@ -863,11 +869,11 @@ __global__ __launch_bounds__(256) void kv8_join_wide(Kv8Attention a, Split split
     }
 }
 
-// Wide tiles that a step can have: every request's last one may be short.
-int64_t wide_tiles(int requests, int max_tokens, int count, int group)
+// Tiles of `tile` rows that a step can have: every request's last one may be short.
+int64_t most_tiles(int requests, int max_tokens, int count, int group, int tile)
 {
-    const int64_t each = ((int64_t)max_tokens * group + kWideRows - 1) / kWideRows * requests;
-    const int64_t all = (int64_t)count * group / kWideRows + requests;
+    const int64_t each = ((int64_t)max_tokens * group + tile - 1) / tile * requests;
+    const int64_t all = (int64_t)count * group / tile + requests;
     return each < all ? each : all;
 }
 
@@ -904,8 +910,9 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         p.few.tile = (int)(rows < p.most_rows ? rows : p.most_rows);
         p.few.places = a.requests;
         // In a mixed batch most of these requests bring a token each.
-        const int64_t each = p.any_wide ? group : p.few.tile;
-        const int64_t tiles = (each + kRows - 1) / kRows * a.requests * a.cache.kv_heads;
+        const int64_t tiles = (p.any_wide ? (int64_t)(group + kRows - 1) / kRows * a.requests
+                                          : most_tiles(a.requests, a.max_tokens, a.count, group, kRows)) *
+                              a.cache.kv_heads;
         // Fewer tiles than CUs: shares for three workgroups per CU (one at widths
         // that fill a CU's registers), at least a step per wavefront. Enough
         // tiles: none, sharing costs about 6 us (32 requests of 2048 positions, 8
@@ -921,11 +928,15 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
     if (p.any_wide) {
         // Wide tiles fill a CU each, so they are split while they leave CUs idle: as
         // many tiles as the rows make, short last ones left out (24 requests, two
-        // of them prompts of 256 tokens, 32 heads of 128: 65 us whole, in halves).
-        p.wide.places = (int)wide_tiles(a.requests, a.max_tokens, a.count, group);
+        // of them prompts of 256 tokens, 32 heads over 8 of 128: 65 us whole, 42 and 9
+        // for the join in halves).
+        p.wide.places = (int)most_tiles(a.requests, a.max_tokens, a.count, group, kWideRows);
         const double tiles = (double)a.count * group / kWideRows * a.cache.kv_heads;
         int64_t most = (int64_t)(256 / (tiles < 1 ? 1 : tiles) + 0.4);
         if (most > steps / 4) most = steps / 4;
+        // Places that stay empty are launched and have their share of the workspace, too.
+        const int64_t places = (int64_t)p.wide.places * a.cache.kv_heads;
+        if (most > 16384 / places) most = 16384 / places;
         p.wide.most = most < 1 ? 1 : most > kMostSplits ? kMostSplits : (int)most;
     }
     size_t taken = 0;
@@ -947,9 +958,12 @@ hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
     const int group = a.heads / a.cache.kv_heads;
     const unsigned requests = a.requests, kv_heads = a.cache.kv_heads;
     if (p.any_few) {
-        const unsigned tiles = (unsigned)((p.few.tile + kRows - 1) / kRows);
-        hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, requests, (unsigned)p.few.most), dim3(64 * kWaves), 0, s, a,
-                           p.few, p.most_rows);
+        // Prompts among single tokens: as many tiles as the rows make.
+        const bool by_tile = W > 256 && p.few.tile > 64;
+        const unsigned tiles = by_tile ? (unsigned)most_tiles(a.requests, a.max_tokens, a.count, group, kRows)
+                                       : (unsigned)((p.few.tile + kRows - 1) / kRows);
+        hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, by_tile ? 1 : requests, (unsigned)p.few.most),
+                           dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
         if (p.few.most > 1)
             hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)p.few.tile * kv_heads, requests), dim3(256), 0, s, a,
                                p.few, p.most_rows);
@@ -957,7 +971,7 @@ hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
     if constexpr (W <= 256) {
         if (p.any_wide) {
             constexpr int KS = W <= 128 ? 2 : 1;
-            const int64_t tiles = wide_tiles(a.requests, a.max_tokens, a.count, group);
+            const int64_t tiles = most_tiles(a.requests, a.max_tokens, a.count, group, kWideRows);
             hipLaunchKernelGGL((kv8_wide<W, KS>), dim3((unsigned)(tiles * p.wide.most * kv_heads)), dim3(256 * KS), 0, s, a,
                                p.wide, p.most_rows);
             if (p.wide.most > 1)

@@ -18,8 +18,8 @@
  * aligned rows whose strides are multiples of 4 load and store faster.
  * Integers on the device (lengths, counts, tables, slots, positions) are
  * int32. A step has at most 2^22 rows (tokens), a row at most 2^22 floats;
- * count * kv_heads <= 2^25 where rows are stored or loaded, count * heads <=
- * 2^28 and requests * kv_heads <= 2^21 in attention.
+ * count * kv_heads <= 2^25 where rows are stored or loaded; in attention
+ * count * heads <= 2^27, requests <= 65535 and requests * kv_heads <= 2^21.
  * The integers are data of the step that no call can check beforehand:
  * an entry outside its range is taken as "nothing there", never followed.
  *
@@ -95,9 +95,9 @@ NYA_HIP_EXPORT int nya_hip_rope_frequencies(float *out, size_t rotated, double b
     unsigned scaling, double factor, double original, double low, double high, float *magnitude);
 
 /* angles[i][j] = (cos, sin)(positions[i] * frequencies[j]) * magnitude for
- * `count` positions and rotated / 2 (at most 512) frequencies: the table (8-byte aligned)
- * that every layer of a step reads. Formed in 64 bits, so far positions lose
- * nothing, and rounded once. */
+ * `count` positions and rotated / 2 (at most 512) frequencies: the
+ * table (8-byte aligned) that every layer of a step reads. Formed in 64 bits,
+ * so far positions lose nothing, and rounded once. */
 NYA_HIP_EXPORT int nya_hip_rope_angles(uintptr_t positions, size_t count, uintptr_t frequencies, size_t rotated,
     float magnitude, uintptr_t angles, uintptr_t stream);
 
@@ -129,7 +129,8 @@ typedef struct nya_hip_kv8 {
 
 /* Bytes of one of the code arrays and of one of the scale arrays; 1 for
  * geometries that the cache does not have (widths and page sizes as above,
- * kv_heads <= 16384, pages * page_tokens and pages * kv_heads <= INT_MAX). The addresses in `cache` are not looked at. */
+ * kv_heads <= 16384, pages * page_tokens and pages * kv_heads <= INT_MAX). The
+ * addresses in `cache` are not looked at. */
 NYA_HIP_EXPORT int nya_hip_kv8_bytes(const nya_hip_kv8 *cache, size_t *codes, size_t *scales);
 
 /* `count` rows of k and v (kv_heads heads of width, strides in floats) into
@@ -137,7 +138,7 @@ NYA_HIP_EXPORT int nya_hip_kv8_bytes(const nya_hip_kv8 *cache, size_t *codes, si
  * cache: the row is left out), k rotated by angles as nya_hip_rope does
  * (angles = 0: as it is); with q, the q rows are rotated into q_out as well
  * (all `count` of them; q_out may be q with the same stride), one launch for
- * both.
+ * both; q without angles is declined.
  *
  * Rows of one page stand together, in the order of their positions, and no
  * slot twice. Such a run takes wanted = max|x| * (1 / 127) (in fp32, at least
@@ -165,7 +166,8 @@ NYA_HIP_EXPORT int nya_hip_kv8_load(const nya_hip_kv8 *cache, uintptr_t slots, s
  * kv_heads): scores q.k * scale, a softmax, out = sum_t p_t v_t. A row that
  * sees nothing gives zeros; rows outside [starts[0], starts[requests]) stay
  * as they are. `count` rows of q and out there are (starts past it are cut
- * off), at most max_tokens of one request. Requests may bring one token, a
+ * off), at most max_tokens of one request, the rest of whose rows stay as
+ * they are. Requests may bring one token, a
  * few (drafts to check) or a prompt, in any mixture. max_length, the longest
  * request the caller expects, only says how finely to split the work; any
  * lengths[r] is attended in full.
@@ -175,8 +177,9 @@ NYA_HIP_EXPORT int nya_hip_kv8_load(const nya_hip_kv8 *cache, uintptr_t slots, s
  * runs goes by the arguments alone: the same call gives the same bits.
  *
  * `workspace` (16-byte aligned) is scratch for work split over several
- * workgroups: with less than nya_hip_kv8_attention_bytes says, or none, the
- * call runs with fewer of them, and slower. Calls that may overlap in time
+ * workgroups (nothing in it is kept, nor has to be cleared): with less than
+ * nya_hip_kv8_attention_bytes says, or none, the call runs with fewer of
+ * them, and slower; both calls with the same arguments. Calls that may overlap in time
  * need workspaces of their own. out must not overlap q. */
 NYA_HIP_EXPORT int nya_hip_kv8_attention_bytes(const nya_hip_kv8 *cache, size_t count, size_t requests,
     size_t max_tokens, size_t max_length, size_t heads, size_t window, size_t *bytes);

@@ -535,6 +535,46 @@ def test_attention_rows_cut_off(env, dev):
     assert np.all(np.abs(got[:2] - want[:2]).max(2) <= attention_bound(weight, top, 64, 80)[:2])
 
 
+def test_attention_starts_outside(env, dev):
+    """starts of the ends of int32: those requests bring nothing, and the rows stay."""
+    lengths = [50, 60, 70, 80]
+    cache, q, _, table = make_attention(env, dev, lengths, [5, 5, 5, 5], 16, 2, 64, 16, 7)
+    starts = np.array([2**31 - 1, -2**31, -2**31, 2**31 - 1, -2**31], np.int32)
+    for most in (1, 22):   # requests of a few rows, and wide tiles
+        got = run_attention(env, dev, cache, q, starts, [50, 60, -80, 80], table, most=most, count=22)
+        assert np.all(got[most:] == 0.25)
+        assert np.all(got[:most] == 0)   # request 2: rows from 0 on, before its first position
+
+
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 128), (4, 4, 64), (6, 2, 256), (4, 2, 512)])
+def test_attention_many_requests(env, dev, heads, kv_heads, width):
+    """A batch of 150 requests, most with one token, prompts among them (the 1st, 64th, 65th and last too), some with
+    nothing."""
+    rng = np.random.default_rng(12)
+    lengths, counts = rng.integers(1, 60, 150), np.ones(150, int)
+    for r, n in ((0, 40), (63, 150), (64, 17), (70, 90), (128, 33), (149, 130)):
+        counts[r], lengths[r] = n, n + int(rng.integers(0, 40))
+    counts[[1, 65, 100]] = 0
+    cache, q, starts, table = make_attention(env, dev, lengths.tolist(), counts.tolist(), heads, kv_heads, width, 32, 13)
+    got = run_attention(env, dev, cache, q, starts, lengths, table)
+    check_attention(cache, q, got, starts, lengths, table)
+
+
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 128), (8, 2, 64), (2, 2, 256), (4, 1, 512)])
+def test_attention_mixed_split(env, dev, heads, kv_heads, width):
+    """A prompt, a single token and drafts over long caches in one batch: work split with its workspace, with parts of
+    it and with none; the same bits twice."""
+    lengths, counts = [3000, 1500, 40, 2200], [100, 1, 30, 3]
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 64, 14)
+    size = env[1].kv8_attention_bytes(cache.arg, len(q), 4, 100, 3000, heads, 0)
+    first = run_attention(env, dev, cache, q, starts, lengths, table)
+    check_attention(cache, q, first, starts, lengths, table)
+    assert np.array_equal(first, run_attention(env, dev, cache, q, starts, lengths, table))
+    for workspace in (size // 2 & ~15, size // 5 & ~15, 0):
+        got = run_attention(env, dev, cache, q, starts, lengths, table, workspace=workspace)
+        check_attention(cache, q, got, starts, lengths, table)
+
+
 def test_attention_scales(env, dev):
     """A scale of 0, a negative one and a large one."""
     lengths, counts = [100, 64], [20, 1]

@@ -167,6 +167,24 @@ def test_kv8_attention_refusals(kernels):
            [{"cache": cache(**c)} for c in BAD_GEOMETRY] + sizes + [{"cache": None}, {"bytes": None}])
 
 
+def test_kv8_attention_limits(kernels):
+    """The largest steps are answered, larger ones declined; empty places do not make the workspace large."""
+    def ask(count, requests, heads, kv_heads, width=128, max_tokens=1, max_length=4096):
+        b = ctypes.c_size_t()
+        done = kernels.lib.nya_hip_kv8_attention_bytes(cache(kv_heads=kv_heads, width=width), count, requests,
+                                                       max_tokens, max_length, heads, 0, ctypes.byref(b))
+        return done, b.value
+    assert ask(1 << 22, 1, 32, 8, max_tokens=1 << 22)[0] == 0
+    assert ask(1 << 22, 1, 33, 3)[0] == 1
+    assert ask(1 << 22, 1, 33, 3, width=512)[0] == 1
+    assert ask(65535, 65535, 32, 32)[0] == 0
+    assert ask(65535, 65535, 33, 33)[0] == 1
+    # A prompt of 600 tokens somewhere among 65535 requests.
+    for width in (64, 128, 256, 512):
+        done, size = ask(700, 65535, 32, 32, width, max_tokens=600)
+        assert done == 0 and size < 1 << 32
+
+
 @pytest.mark.parametrize("seed", range(4))
 def test_page_statement(seed):
     """The statement the GPU is held to: no page is held twice or lost, and every slot is its request's."""
