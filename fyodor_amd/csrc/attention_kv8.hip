@@ -33,12 +33,14 @@ struct Range {
 // How the positions of tiles are shared out: among `most` workgroups, at least
 // `least` steps each, which leave their rows (and each row's maximum and sum)
 // in the workspace: room for `places` places of `tile` rows, for every KV head.
+// A place is a request, or (listed) a tile of the requests' rows by tile_of.
 struct Share {
     float *o;
     float2 *ml;
 };
 struct Split {
     int most, least, tile, places;
+    bool listed;
     float *partials;
 
     __device__ __forceinline__ Share share(int kv_heads, int place, int kvh, int row, int sp, int width) const
@@ -176,7 +178,7 @@ __device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, 
 // before that.
 template <int W>
 __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, int sp, int tile, const Split &split,
-    int most_rows, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
+    int place, int most_rows, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
 {
     constexpr int C = W / 64, D = W / 16;
     constexpr bool kAhead = W <= 256;   // room for a step's K and V in registers
@@ -387,7 +389,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
     }
     const int mrow = threadIdx.x >> 4, mcol = 4 * (threadIdx.x & 15);   // this thread's output: 4 columns of a row
     const int out_row = kRows * tile + mrow;
-    const Share to = split.share(c.kv_heads, r, kvh, out_row, sp, W);
+    const Share to = split.share(c.kv_heads, place, kvh, split.listed ? mrow : out_row, sp, W);
     const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -432,11 +434,15 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     __shared__ float ml[2][kWaves][kRows];
     __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
     TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / a.cache.kv_heads)};
+    int place = at.request;
     if constexpr (W > 256) {   // every request runs here, prompts too
-        if (gridDim.y == 1) at = tile_of<kRows>(a, 0, at.tile);
-        if (at.request < 0) return;
+        if (split.listed) {
+            place = at.tile;
+            at = tile_of<kRows>(a, 0, place);
+            if (at.request < 0) return;
+        }
     }
-    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, split.most - 1 - (int)blockIdx.z, at.tile, split,
+    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, split.most - 1 - (int)blockIdx.z, at.tile, split, place,
                 most_rows, ml, po);
 }
 
@@ -788,17 +794,27 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
 }
 
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over a row's shares.
-// Requests of a few rows: workgroup (row of a KV head and request).
+// Requests of a few rows: workgroup (place, row of a KV head).
 template <int W>
-__global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split split, int most_rows)
+__device__ __forceinline__ void join_row(const Kv8Attention &a, const Split &split, int most_rows, int index)
 {
     const Kv8 &c = a.cache;
-    const int group = a.heads / c.kv_heads, r = blockIdx.y, kvh = blockIdx.x % c.kv_heads, row = blockIdx.x / c.kv_heads;
+    const int group = a.heads / c.kv_heads, place = index / (split.tile * c.kv_heads), kvh = index % c.kv_heads,
+              within = index / c.kv_heads % split.tile;
+    int r = place, row = within;
+    if constexpr (W > 256) {
+        if (split.listed) {
+            const TileOf at = tile_of<kRows>(a, 0, place);
+            if (at.request < 0) return;
+            r = at.request;
+            row += kRows * at.tile;
+        }
+    }
     const Request rq = request_of(a, r);
     if (row >= rq.rows || rq.rows > most_rows) return;
     const Range g = range_of(a, rq, row / kRows, kRows, split.most, split.least);
     if (g.active <= 1) return;
-    const Share from = split.share(c.kv_heads, r, kvh, row, 0, W);
+    const Share from = split.share(c.kv_heads, place, kvh, within, 0, W);
     constexpr int kCols = W / 4, kParts = 256 / kCols;
     __shared__ f32x4 po[kParts][kCols];
     __shared__ float fs[kMostSplits];
@@ -829,22 +845,24 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split split, int
     for (int k = 0; k < 4; ++k) out[k] = o[k] * inverse;
 }
 
-// Wide tiles: workgroup (tile and KV head, 16 of its rows), a wavefront every
+// Wide tiles: workgroup (tile, 16 of its rows, KV head), a wavefront every
 // fourth row.
+constexpr int kJoinParts = kWideRows / 16;
 template <int W>
-__global__ __launch_bounds__(256) void kv8_join_wide(Kv8Attention a, Split split, int most_rows)
+__device__ __forceinline__ void join_wide(const Kv8Attention &a, const Split &split, int most_rows, int index)
 {
     const Kv8 &c = a.cache;
-    const int kvh = blockIdx.x % c.kv_heads, lane = threadIdx.x & 63, group = a.heads / c.kv_heads;
-    const TileOf at = tile_of<kWideRows>(a, most_rows, blockIdx.x / c.kv_heads);
+    const int kvh = index % c.kv_heads, lane = threadIdx.x & 63, group = a.heads / c.kv_heads;
+    const int part = index / c.kv_heads % kJoinParts, place = index / c.kv_heads / kJoinParts;
+    const TileOf at = tile_of<kWideRows>(a, most_rows, place);
     if (at.request < 0) return;
     const Request rq = request_of(a, at.request);
     const Range g = range_of(a, rq, at.tile, kWideRows, split.most, split.least);
     if (g.active <= 1) return;
     constexpr int kCols = W / 64;   // columns per lane
-    const int first_row = kWideRows * at.tile + 16 * blockIdx.y;
+    const int first_row = kWideRows * at.tile + 16 * part;
     for (int row = first_row + (threadIdx.x >> 6); row < min(first_row + 16, rq.rows); row += 4) {
-        const Share from = split.share(c.kv_heads, blockIdx.x / c.kv_heads, kvh, row - kWideRows * at.tile, 0, W);
+        const Share from = split.share(c.kv_heads, place, kvh, row - kWideRows * at.tile, 0, W);
         const float2 mine = lane < g.active ? from.ml[lane] : make_float2(-INFINITY, 0.f);
         const float top = wave_reduce<true>(mine.x), base = top == -INFINITY ? 0.f : top;
         const float f = __builtin_amdgcn_exp2f(mine.x - base), total = wave_sum(mine.y * f);
@@ -867,6 +885,15 @@ __global__ __launch_bounds__(256) void kv8_join_wide(Kv8Attention a, Split split
 #pragma unroll
         for (int e = 0; e < kCols; ++e) out[64 * e] = o[e] * inverse;
     }
+}
+
+// Both in one launch: `wide_blocks` workgroups of wide tiles, then those of few rows.
+template <int W>
+__global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split few, Split wide, int most_rows, int wide_blocks)
+{
+    const int index = blockIdx.x;
+    if (index >= wide_blocks) join_row<W>(a, few, most_rows, index - wide_blocks);
+    else join_wide<W>(a, wide, most_rows, index);
 }
 
 // Tiles of `tile` rows that a step can have: every request's last one may be short.
@@ -896,7 +923,7 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
     int64_t range = a.max_length;
     if (a.window && (int64_t)a.window + a.max_tokens < range) range = (int64_t)a.window + a.max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, 0, nullptr}, {1, 4, kWideRows, 0, nullptr}};
+    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, 0, false, nullptr}, {1, 4, kWideRows, 0, true, nullptr}};
     if (width <= 256 && rows > 64) {
         // Up to 64 rows are fewer keys read again than wide tiles leave empty (8
         // requests of 5 tokens of 32 heads over 4 of 64: 12 us, wide 18 to 23). In
@@ -909,6 +936,12 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
     if (p.any_few) {
         p.few.tile = (int)(rows < p.most_rows ? rows : p.most_rows);
         p.few.places = a.requests;
+        if (!p.any_wide && rows > 64) {
+            // Prompts of heads of 512: as many tiles as the rows make.
+            p.few.listed = true;
+            p.few.tile = kRows;
+            p.few.places = (int)most_tiles(a.requests, a.max_tokens, a.count, group, kRows);
+        }
         // In a mixed batch most of these requests bring a token each.
         const int64_t tiles = (p.any_wide ? (int64_t)(group + kRows - 1) / kRows * a.requests
                                           : most_tiles(a.requests, a.max_tokens, a.count, group, kRows)) *
@@ -955,30 +988,27 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
 template <int W>
 hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
 {
-    const int group = a.heads / a.cache.kv_heads;
     const unsigned requests = a.requests, kv_heads = a.cache.kv_heads;
     if (p.any_few) {
-        // Prompts among single tokens: as many tiles as the rows make.
-        const bool by_tile = W > 256 && p.few.tile > 64;
-        const unsigned tiles = by_tile ? (unsigned)most_tiles(a.requests, a.max_tokens, a.count, group, kRows)
-                                       : (unsigned)((p.few.tile + kRows - 1) / kRows);
-        hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, by_tile ? 1 : requests, (unsigned)p.few.most),
+        const bool listed = p.few.listed;
+        const unsigned tiles = listed ? (unsigned)p.few.places : (unsigned)((p.few.tile + kRows - 1) / kRows);
+        hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, listed ? 1 : requests, (unsigned)p.few.most),
                            dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
-        if (p.few.most > 1)
-            hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)p.few.tile * kv_heads, requests), dim3(256), 0, s, a,
-                               p.few, p.most_rows);
     }
+    int64_t wide_blocks = 0;
     if constexpr (W <= 256) {
         if (p.any_wide) {
             constexpr int KS = W <= 128 ? 2 : 1;
-            const int64_t tiles = most_tiles(a.requests, a.max_tokens, a.count, group, kWideRows);
+            const int64_t tiles = p.wide.places;
             hipLaunchKernelGGL((kv8_wide<W, KS>), dim3((unsigned)(tiles * p.wide.most * kv_heads)), dim3(256 * KS), 0, s, a,
                                p.wide, p.most_rows);
-            if (p.wide.most > 1)
-                hipLaunchKernelGGL((kv8_join_wide<W>), dim3((unsigned)(tiles * kv_heads), kWideRows / 16), dim3(256), 0, s, a,
-                                   p.wide, p.most_rows);
+            if (p.wide.most > 1) wide_blocks = tiles * kJoinParts * kv_heads;
         }
     }
+    const int64_t blocks = wide_blocks + (p.any_few && p.few.most > 1 ? (int64_t)p.few.tile * kv_heads * p.few.places : 0);
+    if (blocks)
+        hipLaunchKernelGGL((kv8_join<W>), dim3((unsigned)blocks), dim3(256), 0, s, a, p.few, p.wide, p.most_rows,
+                           (int)wide_blocks);
     return hipGetLastError();
 }
 
