@@ -1,4 +1,27 @@
 // Causal attention over a paged 8-bit cache (include/fyodor_hip_serving.h).
+//
+// For a KV head, its group's heads and the request's new tokens make the rows
+// of one product: row i is token i / group, head i % group of the group. With
+// codes K, V and the scales a_t, b_t of position t's page,
+//     s_it = (q_i . K_t) a_t scale,   out_i = sum_t e^(s_it) b_t V_t / sum_t e^(s_it).
+// One pass over the positions, 64 a step: S^T = K Q^T and O^T = V^T P^T on the
+// fp16 matrix cores, with the softmax's running maximum and sum (fp32, like S
+// and O) per column, so that a column of S^T is already laid out as the operand
+// P^T. The codes are exact in fp16. q and P go in as two fp16 pieces each
+// (22 bits, the error of fp32 sums of this length; one piece would be 2^-11),
+// which makes two matrix instructions of one: half the fp16 rate is this
+// kernel's ceiling. b_t is a power of two times a mantissa: the power joins the
+// exponent of e^s and the mantissa multiplies P, so P's fp16 pieces see what
+// is summed, not codes of a page of small values. The maximum is rounded up to
+// a whole power of two: rescaling by it is exact, and rare.
+//
+// A call of few rows reads each position once, 2 W bytes per KV head and position,
+// and is bound by that; one of many rows by the matrix cores and the
+// conversions and the softmax beside them. Hence two kernels, a workgroup of
+// 16 rows that loads straight into the operands' lanes (kv8_rows), and one of
+// 128 rows that convert each code once, in LDS (kv8_wide). What is too few
+// tiles for the chip is split over the positions and joined by a second
+// launch (kv8_join).
 #include <math.h>
 
 #include "device.h"
@@ -175,7 +198,11 @@ __device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, 
 // fourth step of its share of the positions and meet in LDS at the end. Keys
 // and values go from memory straight into the operands' lanes: K and V of a
 // step are requested as soon as the last step's are used up, pages a step
-// before that.
+// before that: with a load and its use in one step the wavefronts, two per SIMD,
+// waited for memory (64 requests of 500 to 8192 positions, 32 heads over 8 of
+// 128, 371 MB: 105 us with the join, so 95: 4.1 TB/s in these 90, of the 5.1
+// that a copy reaches; 1 of 32768, 67 MB: 28 us, so 20). Registers for three
+// wavefronts per SIMD measured slower.
 template <int W>
 __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, int sp, int tile, const Split &split,
     int place, int most_rows, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
@@ -462,7 +489,11 @@ __device__ __forceinline__ void lds_barrier()
 // end. Two groups run half a step apart: while one is in its MFMAs (last
 // step's outputs, this step's scores) the other does its softmax and stages
 // its next codes, so that the matrix cores of a SIMD always have one of its two
-// wavefronts.
+// wavefronts (1024 tokens at the end of 8192 positions, 32 heads over 8 of 128:
+// 345 us with one group, and copies of tiles around conditions, so 245: 528
+// TFLOP/s, 1056 as issued, where the library's product of 8192^3 in fp16 reaches
+// 1154). Heads of 256 fill the
+// registers with one group: 420 to 450 TFLOP/s in long prompts.
 template <int W, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
 void kv8_wide(Kv8Attention a, Split split, int most_rows)

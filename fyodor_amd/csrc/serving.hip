@@ -1,6 +1,9 @@
 // The steps around attention over a paged 8-bit cache
 // (include/fyodor_hip_serving.h): page tables from request lengths, rotary
-// positions, and the cache's store and load.
+// positions, and the cache's store and load. None of them does arithmetic worth
+// counting: in a decode step they are bound by launches and by the chains of
+// waits inside (the angles of 16 tokens take 2 us), for prompts by the
+// bytes of the rows at a copy's rate.
 #include <math.h>
 
 #include "device.h"
@@ -169,7 +172,9 @@ __device__ __forceinline__ void place_row(const PageStep &p, int row, bool live,
 
 // The whole step of up to 1024 requests and 8192 rows in one launch: a request
 // per thread, the three prefix sums together, rows from LDS. Bound by its chain
-// of waits (lengths, stack and table, rows).
+// of waits (lengths, stack and table, rows): 64 requests of a token each take 4.8 us
+// (page_tables and page_rows 7.0 and 3.1), 8192 rows of theirs 10.5, by when the
+// two are as fast; more rows want more than one CU.
 __global__ __launch_bounds__(kPageThreads) void page_small(PageStep p)
 {
     constexpr int kWavesHere = kPageThreads / 64;
@@ -379,7 +384,10 @@ __device__ __forceinline__ void rotate_heads(const Rows &t, int row, int first, 
     }
 }
 
-// Workgroup (row, part of its heads).
+// Workgroup (row, part of its heads). Rows of 24 heads of 256, a quarter of
+// each rotated: 2049 of them 24.5 us, 4.1 TB/s (a grid through the parts of a
+// row first: 6 us more). Angles in 64 bits per step, not per layer: 4 us for
+// 2049 x 32.
 __global__ __launch_bounds__(256) void rope_rows(Rows q, Rows k, int width, const float2 *__restrict__ angles,
     int rotated, bool halves, int q_parts, int each, bool quads)
 {
@@ -444,6 +452,8 @@ struct Store {
     int each;    // q heads per workgroup
     int parts;   // workgroups per row of q
     int rows;    // rows of a workgroup that stores
+    int apart;   // groups of rows that follow in the grid are this far apart ..
+    int lines;   // .. and `lines` of them go before the next ones
     int stores;  // workgroups that store
 };
 
@@ -664,7 +674,9 @@ __device__ __forceinline__ void store_run(const Store &args, int row, int head, 
 // that are multiples of 4 KB sent everything in flight to the same few channels
 // (4096 rows, 8 heads of 128, no q: 331 us, so 46). Most rows of a prompt begin
 // no run, and a workgroup that finds none costs 0.35 ns of the chip: rows go in
-// groups where there are many (those 46 us -> 27; the bytes alone take 8).
+// groups where there are many (those 46 us -> 27). Groups a page apart follow each other in the
+// grid: in the rows' order the ones with a run, one in page_tokens / rows, were
+// dealt to a part of the CUs only (27 us -> 17; the bytes alone take 8).
 template <int W>
 __global__ __launch_bounds__(256, 3) void kv8_store(Store s)
 {
@@ -676,8 +688,10 @@ __global__ __launch_bounds__(256, 3) void kv8_store(Store s)
                      s.quads_q);
         return;
     }
-    const int first_row = blockIdx.x / pairs * s.rows, part = blockIdx.x % pairs;
+    const int at = blockIdx.x / pairs, part = blockIdx.x % pairs;
+    const int first_row = (at % s.lines * s.apart + at / s.lines) * s.rows;
     const int lane = threadIdx.x & 63, rows = min(s.rows, s.count - first_row);
+    if (rows <= 0) return;
     const int row = first_row + min(lane, rows - 1), slot = s.slots[row], before = row ? s.slots[row - 1] : -2;
     uint64_t mask = __builtin_amdgcn_ballot_w64(lane < rows && (unsigned)slot < (unsigned)(s.c.pages * s.c.page_tokens) &&
                                                 (before != slot - 1 || (slot & (s.c.page_tokens - 1)) == 0));
@@ -775,9 +789,11 @@ hipError_t launch_kv8_store(const Kv8 &cache, const int *slots, int count, const
     const int each = q.heads ? heads_each(count, q.heads, cache.width) : 1, parts = (q.heads + each - 1) / each;
     const int64_t work = (int64_t)count * cache.kv_heads;
     const int rows = work <= 2048 ? 1 : work <= 8192 ? 4 : 8;
-    const int64_t stores = (int64_t)((count + rows - 1) / rows) * 2 * cache.kv_heads;
+    const int groups = (count + rows - 1) / rows, page = cache.page_tokens / rows;
+    const int apart = page < groups ? page : groups, lines = (groups + apart - 1) / apart;
+    const int64_t stores = (int64_t)lines * apart * 2 * cache.kv_heads;
     const Store args = {cache, slots, count, k, v, k_stride, v_stride, angles, rotated, halves, quads_k, quads_q, q, each,
-                        parts, rows, (int)stores};
+                        parts, rows, apart, lines, (int)stores};
     const dim3 grid((unsigned)(stores + (int64_t)count * parts));
     switch (cache.width) {
     case 64: hipLaunchKernelGGL(kv8_store<64>, grid, dim3(256), 0, s, args); break;
