@@ -57,13 +57,14 @@ struct Range {
 // `least` steps each, which leave their rows (and each row's maximum and sum)
 // in the workspace: room for `places` places of `tile` rows, for every KV head.
 // A place is a request, or (listed) a tile of the requests' rows by tile_of.
+// Packed: the grid counts the shares there are, by item_of.
 struct Share {
     float *o;
     float2 *ml;
 };
 struct Split {
     int most, least, tile, places;
-    bool listed;
+    bool listed, packed;
     float *partials;
 
     __device__ __forceinline__ Share share(int kv_heads, int place, int kvh, int row, int sp, int width) const
@@ -194,14 +195,50 @@ __device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, 
     return {-1, 0};
 }
 
+// The share of a tile of number `index` over the requests of a few rows, in
+// order (request < 0: past the last).
+struct ItemOf {
+    int request, tile, share;
+};
+
+__device__ __forceinline__ ItemOf item_of(const Kv8Attention &a, const Split &split, int most_rows, int index)
+{
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.requests; base += 64) {
+        const int r = base + lane;
+        int tiles = 0, n = 0;
+        if (r < a.requests) {
+            const Request rq = request_of(a, r);
+            if (rq.rows > 0 && rq.rows <= most_rows) {
+                tiles = (rq.rows + kRows - 1) / kRows;
+                n = tiles * range_of(a, rq, tiles - 1, kRows, split.most, split.least).active;
+            }
+        }
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(sum > index);
+        if (past) {
+            const int at = __builtin_ctzll(past), left = __builtin_amdgcn_readlane(sum, at) - 1 - index,
+                      each = __builtin_amdgcn_readlane(tiles, at);
+            return {base + at, left % each, left / each};
+        }
+        index -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return {-1, 0, 0};
+}
+
 // Requests of a few rows: 16 rows per workgroup, whose wavefronts take every
 // fourth step of its share of the positions and meet in LDS at the end. Keys
 // and values go from memory straight into the operands' lanes: K and V of a
 // step are requested as soon as the last step's are used up, pages a step
 // before that: with a load and its use in one step the wavefronts, two per SIMD,
 // waited for memory (64 requests of 500 to 8192 positions, 32 heads over 8 of
-// 128, 371 MB: 105 us with the join, so 95: 4.1 TB/s in these 90, of the 5.1
-// that a copy reaches; 1 of 32768, 67 MB: 28 us, so 20). Registers for three
+// 128, 371 MB: 105 us with the join, so 95; counted shares 86, 4.6 TB/s of the
+// 5.1 that a copy reaches; 1 of 32768, 67 MB: 28 us, so 20). Registers for three
 // wavefronts per SIMD measured slower.
 template <int W>
 __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, int sp, int tile, const Split &split,
@@ -461,7 +498,14 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     __shared__ float ml[2][kWaves][kRows];
     __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
     TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / a.cache.kv_heads)};
-    int place = at.request;
+    int place = at.request, share = split.most - 1 - (int)blockIdx.z;
+    if (split.packed) {
+        const ItemOf item = item_of(a, split, most_rows, at.tile);
+        if (item.request < 0) return;
+        at = {item.request, item.tile};
+        place = item.request;
+        share = item.share;
+    }
     if constexpr (W > 256) {   // every request runs here, prompts too
         if (split.listed) {
             place = at.tile;
@@ -469,8 +513,7 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
             if (at.request < 0) return;
         }
     }
-    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, split.most - 1 - (int)blockIdx.z, at.tile, split, place,
-                most_rows, ml, po);
+    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, share, at.tile, split, place, most_rows, ml, po);
 }
 
 // LDS writes and reads of the workgroup up to here; global loads stay in flight.
@@ -954,7 +997,7 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
     int64_t range = a.max_length;
     if (a.window && (int64_t)a.window + a.max_tokens < range) range = (int64_t)a.window + a.max_tokens;
     const int64_t steps = (range + kStep - 1) / kStep + 1;
-    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, 0, false, nullptr}, {1, 4, kWideRows, 0, true, nullptr}};
+    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, 0, false, false, nullptr}, {1, 4, kWideRows, 0, true, false, nullptr}};
     if (width <= 256 && rows > 64) {
         // Up to 64 rows are fewer keys read again than wide tiles leave empty (8
         // requests of 5 tokens of 32 heads over 4 of 64: 12 us, wide 18 to 23). In
@@ -988,6 +1031,11 @@ Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         if (share > p.few.least) p.few.least = (int)share;
         const int64_t most = (steps + p.few.least - 1) / p.few.least;
         p.few.most = most > kMostSplits ? kMostSplits : (int)most;
+        // Requests of unequal lengths leave gaps in a grid of all their shares,
+        // and the CUs get unequal work; counting them costs a look at
+        // every request, one for up to 64 (32 and 64 of 500 to 8192 positions: 53
+        // and 98 us, counted 50 and 91; 16, with 128 tiles, 28 and 29).
+        p.few.packed = p.few.most > 1 && tiles >= 256 && a.requests <= 64 && !p.few.listed;
     }
     if (p.any_wide) {
         // Wide tiles fill a CU each, so they are split while they leave CUs idle: as
@@ -1023,7 +1071,8 @@ hipError_t launch_width(const Kv8Attention &a, const Plan &p, hipStream_t s)
     if (p.any_few) {
         const bool listed = p.few.listed;
         const unsigned tiles = listed ? (unsigned)p.few.places : (unsigned)((p.few.tile + kRows - 1) / kRows);
-        hipLaunchKernelGGL((kv8_rows<W>), dim3(tiles * kv_heads, listed ? 1 : requests, (unsigned)p.few.most),
+        const unsigned most = p.few.most, packed = p.few.packed ? tiles * requests * most : 0;
+        hipLaunchKernelGGL((kv8_rows<W>), packed ? dim3(packed * kv_heads) : dim3(tiles * kv_heads, listed ? 1 : requests, most),
                            dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
     }
     int64_t wide_blocks = 0;

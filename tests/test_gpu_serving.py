@@ -575,6 +575,23 @@ def test_attention_mixed_split(env, dev, heads, kv_heads, width):
         check_attention(cache, q, got, starts, lengths, table)
 
 
+@pytest.mark.parametrize("heads,kv_heads,width,tokens", [(8, 8, 64, [1]), (32, 4, 64, [3, 1, 0, 2]), (8, 8, 128, [1]),
+                                                        (8, 8, 64, [40, 1, 90, 1])])
+def test_attention_ragged_split(env, dev, heads, kv_heads, width, tokens):
+    """Many requests of very unequal lengths, as a batch that expects long ones splits them; with less workspace."""
+    rng = np.random.default_rng(15)
+    n = 64 if tokens[0] == 3 else 40
+    lengths = rng.integers(1, 3000, n)
+    lengths[[3, 7]] = 0, 1
+    counts = np.where(np.arange(n) < 2 * len(tokens), np.resize(tokens, n), 1)
+    counts = np.minimum(counts, np.maximum(lengths, 1))
+    cache, q, starts, table = make_attention(env, dev, lengths.tolist(), counts.tolist(), heads, kv_heads, width, 32, 16)
+    size = env[1].kv8_attention_bytes(cache.arg, len(q), n, int(counts.max()), 9000, heads, 0)
+    for workspace in (size, size // 2 & ~15):
+        got = run_attention(env, dev, cache, q, starts, lengths, table, longest=9000, workspace=workspace)
+        check_attention(cache, q, got, starts, lengths, table)
+
+
 def test_attention_scales(env, dev):
     """A scale of 0, a negative one and a large one."""
     lengths, counts = [100, 64], [20, 1]
