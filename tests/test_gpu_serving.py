@@ -546,7 +546,8 @@ def test_attention_starts_outside(env, dev):
         assert np.all(got[:most] == 0)   # request 2: rows from 0 on, before its first position
 
 
-@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 128), (4, 4, 64), (6, 2, 256), (4, 2, 512)])
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 128), (4, 4, 64), (6, 2, 256), (4, 2, 512), (40, 1, 64),
+                                                  (70, 1, 64)])
 def test_attention_many_requests(env, dev, heads, kv_heads, width):
     """A batch of 150 requests, most with one token, prompts among them (the 1st, 64th, 65th and last too), some with
     nothing."""
