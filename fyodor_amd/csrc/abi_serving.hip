@@ -145,7 +145,12 @@ NYA_HIP_EXPORT int nya_hip_rope(uintptr_t q, size_t q_stride, uintptr_t q_out, s
     if (!rows_fit(count) || !heads_ok(heads, width) || !rows_ok(q, q_stride, q_out, q_out_stride, heads * width, count) ||
         !rotation_ok(angles, rotated, width, layout))
         return 1;
-    if (k && (!heads_ok(kv_heads, width) || !rows_ok(k, k_stride, k_out, k_out_stride, kv_heads * width, count)))
+    // No row that is written is another's input or output.
+    const size_t n = heads * width, kn = kv_heads * width;
+    if (k && (!heads_ok(kv_heads, width) || !rows_ok(k, k_stride, k_out, k_out_stride, kn, count) ||
+              !apart(q_out, q_out_stride, n, k, k_stride, kn, count) ||
+              !apart(q_out, q_out_stride, n, k_out, k_out_stride, kn, count) ||
+              !apart(k_out, k_out_stride, kn, q, q_stride, n, count)))
         return 1;
     const Rows qr = {(const float *)q, (float *)q_out, (int64_t)q_stride, (int64_t)q_out_stride, (int)heads};
     const Rows kr = {(const float *)k, (float *)k_out, (int64_t)k_stride, (int64_t)k_out_stride,
@@ -172,7 +177,9 @@ NYA_HIP_EXPORT int nya_hip_kv8_store(const nya_hip_kv8 *cache, uintptr_t slots, 
     if (angles && !rotation_ok(angles, rotated, cache->width, layout)) return 1;
     // Without angles there is nothing to do for q.
     if (q && (!angles || !heads_ok(heads, cache->width) ||
-              !rows_ok(q, q_stride, q_out, q_out_stride, heads * cache->width, count)))
+              !rows_ok(q, q_stride, q_out, q_out_stride, heads * cache->width, count) ||
+              !apart(q_out, q_out_stride, heads * cache->width, k, k_stride, n, count) ||
+              !apart(q_out, q_out_stride, heads * cache->width, v, v_stride, n, count)))
         return 1;
     const Rows qr = {(const float *)q, (float *)q_out, (int64_t)q_stride, (int64_t)q_out_stride, q ? (int)heads : 0};
     return status(launch_kv8_store(cache_of(cache), (const int *)slots, (int)count, (const float *)k,

@@ -63,7 +63,8 @@ extern "C" {
  *      the step.
  * Negative lengths and counts are taken as 0. Run again with the same
  * lengths it changes nothing. requests <= 65536, and
- * requests * table_stride, pages * page_tokens <= INT_MAX. */
+ * requests * table_stride, table_stride * page_tokens and
+ * pages * page_tokens <= INT_MAX. */
 NYA_HIP_EXPORT int nya_hip_page_step(uintptr_t lengths, uintptr_t counts, size_t requests, size_t page_tokens,
     uintptr_t table, size_t table_stride, uintptr_t held, uintptr_t free_pages, size_t pages, uintptr_t free_count,
     uintptr_t starts, uintptr_t positions, uintptr_t slots, size_t max_tokens, uintptr_t stream);
@@ -84,7 +85,7 @@ enum { NYA_HIP_ROPE_INTERLEAVED = 0, NYA_HIP_ROPE_HALVES = 1 };
  *           `high` (0 <= low < high);
  *   RAMP    the same with g going linearly in j instead, from 1 at the
  *           (rounded down) pair that turns `high` times to 0 at the (rounded
- *           up) one that turns `low` times, and *magnitude =
+ *           up) one that turns `low` (> 0) times, and *magnitude =
  *           1 + 0.1 ln(factor).
  * *magnitude, which multiplies (cos, sin), is 1 otherwise. factors (or
  * null): rotated / 2 floats that divide the base frequencies first, a
@@ -104,8 +105,8 @@ NYA_HIP_EXPORT int nya_hip_rope_angles(uintptr_t positions, size_t count, uintpt
 /* The rotary step of `count` rows of q (`heads` heads of `width`) and of k
  * (kv_heads heads; k = 0: none) by angles ([count][rotated / 2] pairs as
  * above): q_out and k_out receive the whole rows, and may be q and k
- * themselves with the same stride, but not overlap them otherwise. Strides
- * in floats. */
+ * themselves with the same stride, but not overlap them or each other
+ * otherwise. Strides in floats. */
 NYA_HIP_EXPORT int nya_hip_rope(uintptr_t q, size_t q_stride, uintptr_t q_out, size_t q_out_stride, size_t heads,
     uintptr_t k, size_t k_stride, uintptr_t k_out, size_t k_out_stride, size_t kv_heads, size_t width, size_t count,
     uintptr_t angles, size_t rotated, unsigned layout, uintptr_t stream);
@@ -137,8 +138,8 @@ NYA_HIP_EXPORT int nya_hip_kv8_bytes(const nya_hip_kv8 *cache, size_t *codes, si
  * the cache slots slots[i] (as nya_hip_page_step numbers them; outside the
  * cache: the row is left out), k rotated by angles as nya_hip_rope does
  * (angles = 0: as it is); with q, the q rows are rotated into q_out as well
- * (all `count` of them; q_out may be q with the same stride), one launch for
- * both; q without angles is declined.
+ * (all `count` of them; q_out may be q with the same stride, and does not
+ * overlap k or v), one launch for both; q without angles is declined.
  *
  * Rows of one page stand together, in the order of their positions, and no
  * slot twice. Such a run takes wanted = max|x| * (1 / 127) (in fp32, at least

@@ -147,6 +147,24 @@ def test_kv8_store_and_load_refusals(kernels):
             {"k_stride": 768, "v_stride": 768, "v": A + 1020}])
 
 
+def test_rows_that_overlap(kernels):
+    """A row that a call writes is no other row's input or output; parts of common rows are apart."""
+    far, L = 1 << 28, kernels.lib
+    rope = dict(q=A, q_stride=512, q_out=A + far, q_out_stride=512, heads=4, k=A + 2 * far, k_stride=256,
+                k_out=A + 3 * far, k_out_stride=256, kv_heads=2, width=128, count=5, angles=A, rotated=64, layout=0,
+                stream=0)
+    refuse(L.nya_hip_rope, rope,
+           [{"k": A + far}, {"k": A + far + 2048}, {"k_out": A + far + 4 * 2047}, {"k": A + far, "k_out": A + far},
+            {"k": A, "k_out": A}, {"k": A + 2044, "k_stride": 512, "k_out": A, "q_out": A, "k_out_stride": 512},
+            # q | k in common rows of 768 in place, k one float too early
+            {"q_out": A, "q_stride": 768, "q_out_stride": 768, "k": A + 2044, "k_out": A + 2044, "k_stride": 768,
+             "k_out_stride": 768}])
+    store = dict(cache=cache(), slots=A, count=4, k=A + 2 * far, k_stride=256, v=A + 3 * far, v_stride=256, angles=A,
+                 rotated=64, layout=1, q=A, q_stride=512, q_out=A + far, q_out_stride=512, heads=4, stream=0)
+    refuse(L.nya_hip_kv8_store, store,
+           [{"k": A + far}, {"v": A + far + 4096}, {"v": A + far - 4}, {"q_out": A + 2 * far}, {"q_out": A + 3 * far - 4}])
+
+
 def test_kv8_attention_refusals(kernels):
     far = 1 << 28
     good = dict(cache=cache(), q=A, q_stride=512, out=A + far, out_stride=512, count=4, starts=A, lengths=A, table=A,
