@@ -25,7 +25,7 @@
 #include <math.h>
 
 #include "device.h"
-#include "serving.h"
+#include "kv8_shares.h"
 
 namespace fy {
 namespace {
@@ -34,77 +34,6 @@ typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-constexpr int kStep = 64;   // positions per step of a wavefront
-constexpr int kRows = 16;   // query rows per tile of a few
-constexpr int kWaves = 4;
-constexpr int kMostSplits = 64;   // a lane each where they are joined
-constexpr int kWideRows = 32 * kWaves;   // query rows per tile of many
-
-// The positions that a tile of query rows sees and how they are split: steps
-// [begin, end) of 64 positions in `active` shares of `chunk`.
-struct Range {
-    int lowest, highest;   // positions, highest < 0: none
-    int begin, chunk, active, end;
-
-    // Steps of share sp. The first one has what is left over: the grids begin
-    // with the last shares, so the shorter ones come where others have ended.
-    __device__ __forceinline__ int until(int sp) const { return end - (active - 1 - sp) * chunk; }
-    __device__ __forceinline__ int from(int sp) const { return max(begin, until(sp) - chunk); }
-};
-
-// How the positions of tiles are shared out: among `most` workgroups, at least
-// `least` steps each, which leave their rows (and each row's maximum and sum)
-// in the workspace: room for `places` places of `tile` rows, for every KV head.
-// A place is a request, or (listed) a tile of the requests' rows by tile_of.
-// Packed: the grid counts the shares there are, by item_of.
-struct Share {
-    float *o;
-    float2 *ml;
-};
-struct Split {
-    int most, least, tile, places;
-    bool listed, packed;
-    float *partials;
-
-    __device__ __forceinline__ Share share(int kv_heads, int place, int kvh, int row, int sp, int width) const
-    {
-        const size_t at = (((size_t)place * kv_heads + kvh) * tile + row) * most + sp;
-        return {partials + at * width, (float2 *)(partials + (size_t)places * kv_heads * tile * most * width) + at};
-    }
-};
-
-// Request r's rows, the first position and whether it brings any.
-struct Request {
-    int begin, rows;   // first row; rows of one KV head: tokens x group
-    int64_t first;     // position of its first token
-};
-
-__device__ __forceinline__ Request request_of(const Kv8Attention &a, int r)
-{
-    const int start = a.starts[r], stop = a.starts[r + 1];
-    const int begin = max(start, 0), end = max(min(stop, a.count), 0), tokens = min(end - begin, a.max_tokens);
-    return {begin, tokens > 0 ? tokens * (a.heads / a.cache.kv_heads) : 0,
-            (int64_t)a.lengths[r] - ((int64_t)stop - begin)};
-}
-
-__device__ __forceinline__ Range range_of(const Kv8Attention &a, const Request &q, int tile, int rows, int splits,
-    int least)
-{
-    const int group = a.heads / a.cache.kv_heads;
-    // Positions of the steps looked up past the last one still fit 31 bits.
-    const int64_t most = min((int64_t)a.table_stride * a.cache.page_tokens - 1, (int64_t)INT32_MAX - 64 * kStep);
-    const int64_t low = q.first + rows * tile / group, high = q.first + (min(rows * tile + rows, q.rows) - 1) / group;
-    Range g;
-    g.highest = (int)(high < 0 ? -1 : high < most ? high : most);
-    g.lowest = (int)(a.window && low >= a.window ? (low - a.window < most ? low - a.window + 1 : most) : 0);
-    g.begin = g.lowest / kStep;
-    g.end = g.highest < 0 ? g.begin : g.highest / kStep + 1;
-    const int steps = g.end - g.begin;
-    g.chunk = max(least, (steps + splits - 1) / splits);
-    g.active = steps > 0 ? (steps + g.chunk - 1) / g.chunk : 1;
-    return g;
-}
 
 // 8 codes as fp16, exactly: the byte with its sign bit flipped under the
 // exponent of 1024 is 1152 + code.
@@ -195,10 +124,11 @@ __device__ __forceinline__ TileOf tile_of(const Kv8Attention &a, int most_rows, 
     return {-1, 0};
 }
 
-// The share of a tile of number `index` over the requests of a few rows, in
-// order (request < 0: past the last).
+// The item of number `index` over the requests of a few rows, in order (request
+// < 0: past the last). The shares that its tile does not have are no work.
 struct ItemOf {
-    int request, tile, share;
+    int request;
+    Item item;
 };
 
 __device__ __forceinline__ ItemOf item_of(const Kv8Attention &a, const Split &split, int most_rows, int index)
@@ -206,15 +136,8 @@ __device__ __forceinline__ ItemOf item_of(const Kv8Attention &a, const Split &sp
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < a.requests; base += 64) {
         const int r = base + lane;
-        int tiles = 0, n = 0;
-        if (r < a.requests) {
-            const Request rq = request_of(a, r);
-            if (rq.rows > 0 && rq.rows <= most_rows) {
-                tiles = (rq.rows + kRows - 1) / kRows;
-                n = tiles * range_of(a, rq, tiles - 1, kRows, split.most, split.least).active;
-            }
-        }
-        int sum = n;
+        const Items items = r < a.requests ? items_of(a, split, request_of(a, r), most_rows) : Items{0, 0};
+        int sum = items.tiles * items.shares;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const int v = __shfl_up(sum, o, 64);
@@ -222,13 +145,13 @@ __device__ __forceinline__ ItemOf item_of(const Kv8Attention &a, const Split &sp
         }
         const uint64_t past = __builtin_amdgcn_ballot_w64(sum > index);
         if (past) {
-            const int at = __builtin_ctzll(past), left = __builtin_amdgcn_readlane(sum, at) - 1 - index,
-                      each = __builtin_amdgcn_readlane(tiles, at);
-            return {base + at, left % each, left / each};
+            const int at = __builtin_ctzll(past);
+            return {base + at, item_at(__builtin_amdgcn_readlane(items.tiles, at),
+                                       __builtin_amdgcn_readlane(sum, at) - 1 - index)};
         }
         index -= __builtin_amdgcn_readlane(sum, 63);
     }
-    return {-1, 0, 0};
+    return {-1, {0, 0}};
 }
 
 // Requests of a few rows: 16 rows per workgroup, whose wavefronts take every
@@ -500,11 +423,11 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv8_rows(Kv8Att
     TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / a.cache.kv_heads)};
     int place = at.request, share = split.most - 1 - (int)blockIdx.z;
     if (split.packed) {
-        const ItemOf item = item_of(a, split, most_rows, at.tile);
-        if (item.request < 0) return;
-        at = {item.request, item.tile};
-        place = item.request;
-        share = item.share;
+        const ItemOf it = item_of(a, split, most_rows, at.tile);
+        if (it.request < 0) return;
+        at = {it.request, it.item.tile};
+        place = it.request;
+        share = it.item.share;
     }
     if constexpr (W > 256) {   // every request runs here, prompts too
         if (split.listed) {
@@ -968,103 +891,6 @@ __global__ __launch_bounds__(256) void kv8_join(Kv8Attention a, Split few, Split
     const int index = blockIdx.x;
     if (index >= wide_blocks) join_row<W>(a, few, most_rows, index - wide_blocks);
     else join_wide<W>(a, wide, most_rows, index);
-}
-
-// Tiles of `tile` rows that a step can have: every request's last one may be short.
-int64_t most_tiles(int requests, int max_tokens, int count, int group, int tile)
-{
-    const int64_t each = ((int64_t)max_tokens * group + tile - 1) / tile * requests;
-    const int64_t all = (int64_t)count * group / tile + requests;
-    return each < all ? each : all;
-}
-
-// Requests of more than most_rows rows (of one KV head) run in wide tiles.
-struct Plan {
-    int most_rows;
-    bool any_few, any_wide;
-    Split few, wide;
-};
-
-size_t share_bytes(const Kv8Attention &a, const Split &s)
-{
-    return (size_t)s.places * s.tile * a.cache.kv_heads * (a.cache.width + 2) * sizeof(float);
-}
-
-Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
-{
-    const int group = a.heads / a.cache.kv_heads, width = a.cache.width;
-    const int64_t rows = (int64_t)a.max_tokens * group;
-    int64_t range = a.max_length;
-    if (a.window && (int64_t)a.window + a.max_tokens < range) range = (int64_t)a.window + a.max_tokens;
-    const int64_t steps = (range + kStep - 1) / kStep + 1;
-    Plan p = {INT32_MAX, true, false, {1, kWaves, 0, 0, false, false, nullptr}, {1, 4, kWideRows, 0, true, false, nullptr}};
-    if (width <= 256 && rows > 64) {
-        // Up to 64 rows are fewer keys read again than wide tiles leave empty (8
-        // requests of 5 tokens of 32 heads over 4 of 64: 12 us, wide 18 to 23). In
-        // a batch with longer ones, which pays for every place of a tile that
-        // a request of a few rows might have, the tiles that one token takes (a
-        // prompt of 512 among 64 requests, 32 heads over 8 of 128: 176 us, with
-        // two tiles 188; 64 over 2 of 64: 107 with the two tiles of a token, 149
-        // with it in wide ones); a single request is all wide.
-        p.most_rows = a.requests == 1 ? 0 : group > 64 ? kRows : (group + kRows - 1) / kRows * kRows;
-        p.any_wide = true;
-        p.any_few = a.requests > 1;
-    }
-    if (p.any_few) {
-        p.few.tile = (int)(rows < p.most_rows ? rows : p.most_rows);
-        p.few.places = a.requests;
-        if (!p.any_wide && rows > 64) {
-            // Prompts of heads of 512: as many tiles as the rows make.
-            p.few.listed = true;
-            p.few.tile = kRows;
-            p.few.places = (int)most_tiles(a.requests, a.max_tokens, a.count, group, kRows);
-        }
-        // In a mixed batch most of these requests bring a token each.
-        const int64_t tiles = (p.any_wide ? (int64_t)(group + kRows - 1) / kRows * a.requests
-                                          : most_tiles(a.requests, a.max_tokens, a.count, group, kRows)) *
-                              a.cache.kv_heads;
-        // Fewer tiles than CUs: shares for three workgroups per CU (one at widths
-        // that fill a CU's registers), at least a step per wavefront. Enough
-        // tiles: none, sharing costs about 6 us (32 requests of 2048 positions, 8
-        // heads of 128, us: whole 25, halves 31, quarters 34), but in long contexts,
-        // where the requests' lengths differ by more (64 of 500 to 8192: whole 105,
-        // 2048 shares were they all long 97).
-        const int64_t wanted = tiles < 256 ? (width <= 128 ? 768 : 256) : steps >= 96 ? 2048 : 0;
-        const int64_t share = wanted ? (tiles * steps + wanted - 1) / wanted : steps;
-        if (share > p.few.least) p.few.least = (int)share;
-        const int64_t most = (steps + p.few.least - 1) / p.few.least;
-        p.few.most = most > kMostSplits ? kMostSplits : (int)most;
-        // Requests of unequal lengths leave gaps in a grid of all their shares,
-        // and the CUs get unequal work; counting them costs a look at
-        // every request, one for up to 64 (32 and 64 of 500 to 8192 positions: 53
-        // and 98 us, counted 50 and 91; 16, with 128 tiles, 28 and 29).
-        p.few.packed = p.few.most > 1 && tiles >= 256 && a.requests <= 64 && !p.few.listed;
-    }
-    if (p.any_wide) {
-        // Wide tiles fill a CU each, so they are split while they leave CUs idle: as
-        // many tiles as the rows make, short last ones left out (24 requests, two
-        // of them prompts of 256 tokens, 32 heads over 8 of 128: 65 us whole, 42 and 9
-        // for the join in halves).
-        p.wide.places = (int)most_tiles(a.requests, a.max_tokens, a.count, group, kWideRows);
-        const double tiles = (double)a.count * group / kWideRows * a.cache.kv_heads;
-        int64_t most = (int64_t)(256 / (tiles < 1 ? 1 : tiles) + 0.4);
-        if (most > steps / 4) most = steps / 4;
-        // Places that stay empty are launched and have their share of the workspace, too.
-        const int64_t places = (int64_t)p.wide.places * a.cache.kv_heads;
-        if (most > 16384 / places) most = 16384 / places;
-        p.wide.most = most < 1 ? 1 : most > kMostSplits ? kMostSplits : (int)most;
-    }
-    size_t taken = 0;
-    for (Split *s : {&p.wide, &p.few}) {
-        if (s->most == 1) continue;
-        const size_t each = share_bytes(a, *s);
-        if (bytes / each < (size_t)s->most) s->most = bytes / each < 2 ? 1 : (int)(bytes / each);
-        if (s->most == 1) continue;
-        if (workspace) s->partials = workspace + taken;
-        taken += s->most * each / sizeof(float);
-        bytes -= s->most * each;
-    }
-    return p;
 }
 
 template <int W>
