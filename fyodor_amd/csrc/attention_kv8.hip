@@ -13,7 +13,8 @@
 // kernel's ceiling. b_t is a power of two times a mantissa: the power joins the
 // exponent of e^s and the mantissa multiplies P, so P's fp16 pieces see what
 // is summed, not codes of a page of small values. The maximum is rounded up to
-// a whole power of two: rescaling by it is exact, and rare.
+// a whole power of two: rescaling by it is exact, and rare. From 2^22 on (kFar)
+// the scores are rounded first, and their distances from the maximum taken after.
 //
 // A call of few rows reads each position once, 2 W bytes per KV head and position,
 // and is bound by that; one of many rows by the matrix cores and the
@@ -22,6 +23,7 @@
 // 128 rows that convert each code once, in LDS (kv8_wide). What is too few
 // tiles for the chip is split over the positions and joined by a second
 // launch (kv8_join).
+#include <float.h>
 #include <math.h>
 
 #include "device.h"
@@ -92,6 +94,19 @@ __device__ __forceinline__ float column_sum(float v)
     const int b = __builtin_bit_cast(int, v);
     const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
     return halves_sum(__builtin_bit_cast(float, (int)r[0]) + __builtin_bit_cast(float, (int)r[1]));
+}
+
+// A score times its scale less the maximum, rounded once at the end, may be above
+// 0 by half the last place of the maximum. From this maximum on that is more than
+// weights in fp16, up to 2^15 of the 2^16 they hold, have room for.
+constexpr float kFar = 0x1p22f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
+
+// What a row's sum of weights makes of its outputs. Without weights the row saw
+// nothing (no maximum) and gives zeros, or its scores were beyond fp32.
+__device__ __forceinline__ float inverse_of(float total, float top)
+{
+    return total == 0.f ? (top == -INFINITY ? 0.f : NAN) : 1.f / total;
 }
 
 // The request and the tile of kTile rows of number `index` over the requests
@@ -273,6 +288,8 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
 #pragma unroll
     for (int d = 0; d < D; ++d) O[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
+    bool far = false;
+    uint64_t saw = 0;   // lanes that had a score
     for (int step = begin; step < stop; step += kWaves) {
         const int8_t *vb = nullptr;
         if constexpr (!kAhead) {
@@ -307,7 +324,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
         // it NaN by their sum alone.
         const int at = kStep * step, pos = at + 16 * part;
         const bool fine = __builtin_isfinite(ks) && __builtin_isfinite(vs);
-        const float scale = fine ? fmaxf(fabsf(ks) * qscale, 0x1p-126f) : 1.f;   // above 0: keeps minus infinity
+        float scale = fine ? fmaxf(fabsf(ks) * qscale, 0x1p-126f) : 1.f;   // above 0: keeps minus infinity
         const int e = fine ? __builtin_amdgcn_frexp_expf(vs) : 0;
         const float mant = fine ? __builtin_amdgcn_frexp_mantf(vs) : 1.f;
         if (there && !fine && first <= pos + 15 && last >= pos) l = NAN;
@@ -319,7 +336,8 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
         float best = S[0][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) best = fmaxf(best, S[i >> 2][i & 3]);
-        const float top = best * scale + e;
+        saw |= __builtin_amdgcn_ballot_w64(best > -INFINITY);
+        const float top = __builtin_fmaf(best, scale, e);
         if (__builtin_amdgcn_ballot_w64(top > m)) {
             const float next = fmaxf(m, ceilf(column_max(top)));
             const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
@@ -327,8 +345,16 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < D; ++d) O[d] *= alpha;
+            far = __builtin_amdgcn_ballot_w64(is_far(m));
         }
-        const float add = e - (m == -INFINITY ? 0.f : m) + 15.f;
+        const float base = m == -INFINITY ? 0.f : m;
+        float add = e - base + 15.f;
+        if (far) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) S[i >> 2][i & 3] = __builtin_fmaf(S[i >> 2][i & 3], scale, e) - base;
+            scale = 1.f;
+            add = 15.f;
+        }
         half8 ph[2], pl[2];
         float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -368,6 +394,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
         }
     }
     l = column_sum(l);
+    if (m == -INFINITY && (saw >> col & 0x0001000100010001u)) m = -FLT_MAX;   // scores, none in fp32
 
     // The wavefronts' partial softmaxes meet in LDS, 64 columns at a time.
     if (part == 0) {
@@ -402,8 +429,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
             } else {
                 float *out = a.out + (rq.begin + out_row / group) * a.out_stride +
                              (int64_t)(kvh * group + out_row % group) * W + 64 * i + mcol;
-                const float inverse = total == 0.f ? 0.f : 1.f / total;
-                o *= inverse;
+                o *= inverse_of(total, top);
                 if (aligned) {
                     *(f32x4 *)out = o;
                 } else {
@@ -605,6 +631,8 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
     for (int d = 0; d < D; ++d) O[d] = (f32x16){};
     half8 ph[2][2], pl[2][2];
     float m = -INFINITY, l = 0.f;
+    bool far = false;
+    uint64_t saw = 0;   // lanes that had a score
     auto outputs = [&]() {
         const uint8_t *vs = vsm + 16 * lane;
 #pragma unroll
@@ -666,14 +694,16 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
                 for (int n = 0; n < 16; ++n) S[t][n] = seen >> n & 1 ? S[t][n] : -INFINITY;
             }
         }
-        float top = -INFINITY;
+        float top = -INFINITY, any = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             float best = S[t][0];
 #pragma unroll
             for (int n = 1; n < 16; ++n) best = fmaxf(best, S[t][n]);
-            top = fmaxf(top, best * scale[t] + e[t]);
+            any = fmaxf(any, best);
+            top = fmaxf(top, __builtin_fmaf(best, scale[t], e[t]));
         }
+        saw |= __builtin_amdgcn_ballot_w64(any > -INFINITY);
         if (__builtin_amdgcn_ballot_w64(top > m)) {
             const float next = fmaxf(m, ceilf(halves_max(top)));
             const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
@@ -681,18 +711,28 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < D; ++d) O[d] *= alpha;
+            far = __builtin_amdgcn_ballot_w64(is_far(m));
         }
         const float base = m == -INFINITY ? 0.f : m;
+        float add[2] = {e[0] - base + 15.f, e[1] - base + 15.f};
+        if (far) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int n = 0; n < 16; ++n) S[t][n] = __builtin_fmaf(S[t][n], scale[t], e[t]) - base;
+                scale[t] = 1.f;
+                add[t] = 15.f;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             float sum[2] = {0.f, 0.f};
-            const float add = e[t] - base + 15.f;
 #pragma unroll
             for (int n = 0; n < 16; n += 8) {
                 float w[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][n + i], scale[t], add));
+                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][n + i], scale[t], add[t]));
                     sum[i & 1] += v;
                     w[i] = v * mant[t];
                 }
@@ -735,6 +775,7 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
         __syncthreads();
     }
     l = halves_sum(l);
+    if (m == -INFINITY && (saw >> col & 0x0000000100000001u)) m = -FLT_MAX;   // scores, none in fp32
     if constexpr (KS == 2) {
         // The second group's rows through LDS, as they lie in its registers.
         float *po = (float *)&smem[0][0][0] + wave * (16 * D * 64) + lane;
@@ -771,7 +812,7 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
         return;
     }
     float *out = a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W + 4 * h;
-    const float inverse = l == 0.f ? 0.f : 1.f / l;
+    const float inverse = inverse_of(l, m);
     const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
 #pragma unroll
     for (int d = 0; d < D; ++d)
@@ -837,7 +878,7 @@ __device__ __forceinline__ void join_row(const Kv8Attention &a, const Split &spl
 #pragma unroll
     for (int k = 1; k < kParts; ++k) o += po[k][col];
     float *out = a.out + (rq.begin + row / group) * a.out_stride + (int64_t)(kvh * group + row % group) * W + 4 * col;
-    const float inverse = total == 0.f ? 0.f : 1.f / total;
+    const float inverse = inverse_of(total, top);
 #pragma unroll
     for (int k = 0; k < 4; ++k) out[k] = o[k] * inverse;
 }
@@ -878,7 +919,7 @@ __device__ __forceinline__ void join_wide(const Kv8Attention &a, const Split &sp
             }
         }
         float *out = a.out + (rq.begin + row / group) * a.out_stride + (int64_t)(kvh * group + row % group) * W + lane;
-        const float inverse = total == 0.f ? 0.f : 1.f / total;
+        const float inverse = inverse_of(total, top);
 #pragma unroll
         for (int e = 0; e < kCols; ++e) out[64 * e] = o[e] * inverse;
     }

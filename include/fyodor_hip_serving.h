@@ -174,7 +174,9 @@ NYA_HIP_EXPORT int nya_hip_kv8_load(const nya_hip_kv8 *cache, uintptr_t slots, s
  * lengths[r] is attended in full.
  *
  * q (and the softmax's weights) enter the matrix cores as two fp16 pieces,
- * 22 bits each, the codes exactly; all sums are fp32. Which kernel and split
+ * 22 bits each, the codes exactly; all sums are fp32. A score above
+ * 2^128 / log2(e) (2.3e38), or nothing but scores below minus that, gives NaN.
+ * Which kernel and split
  * runs goes by the arguments alone: the same call gives the same bits.
  *
  * `workspace` (16-byte aligned) is scratch for work split over several

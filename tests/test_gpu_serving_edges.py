@@ -3,8 +3,8 @@ the statements in serving_check.py."""
 import numpy as np
 import pytest
 
-from serving_check import attention_bound
-from test_gpu_serving import dev, env, make_attention, run_attention   # noqa: F401 (fixtures)
+from serving_check import F32_HALF, attention_bound
+from test_gpu_serving import check_attention, dev, env, make_attention, run_attention   # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,81 @@ def test_drafts_under_a_long_window(env, dev, requests, tokens, heads, kv_heads,
                             longest=32768, workspace=workspace)
         off = np.abs(got - want).max(2)
         assert np.all(off <= bound), (workspace, np.argwhere(~(off <= bound))[:5].tolist())
+
+
+# ---- attention: scores at the ends of fp32 ----------------------------------
+
+SCORE_BATCHES = [([300], [1]), ([80], [80]), ([300, 80, 9], [1, 80, 4]), ([9000], [1])]
+
+
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 64), (8, 2, 128), (4, 2, 256), (2, 1, 512)])
+@pytest.mark.parametrize("lengths,counts", SCORE_BATCHES)
+@pytest.mark.parametrize("size", [1e7, 3e8, 1e20, 1e33])
+def test_far_scores(env, dev, heads, kv_heads, width, lengths, counts, size):
+    """Scores of `size`, where fp32 has no fractions left: one position takes a row (all but those whose best two
+    scores fp32 does not tell apart)."""
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 64, 33, spread=0.1)
+    q *= np.float32(size ** 0.5)
+    cache.k.scales[table[table >= 0][table[table >= 0] < cache.pages]] *= np.float32(size ** 0.5)
+    cache.put()
+    got = run_attention(env, dev, cache, q, starts, lengths, table)
+    scale, clear = np.float32(width ** -0.5), 0
+    for r, n in enumerate(lengths):
+        t = np.arange(n)
+        page = table[r, t // 64]
+        for h in range(heads):
+            k, v = (c.values()[page, h * kv_heads // heads, t % 64] for c in (cache.k, cache.v))
+            for row in range(starts[r], starts[r + 1]):
+                last = n - (starts[r + 1] - row) + 1
+                x = q[row, h].astype(np.float64)
+                s = k[:last] @ x * scale
+                top = np.abs(v[:last]).max()
+                assert np.all(np.abs(got[row, h]) <= top * (1 + 2.0 ** -16))
+                # Off by this much each (attention_bound's part of the scores), another position weighs e^-50.
+                off = (np.abs(k[:last]) @ np.abs(x)).max() * scale * (2.0 ** -22 + (width / 16 + 12) * F32_HALF)
+                order = np.argsort(s)
+                if last == 1 or s[order[-1]] - s[order[-2]] > 2 * off + 50:
+                    clear += 1
+                    assert np.abs(got[row, h] - v[order[-1]]).max() <= attention_bound(0, top, width, n), (row, h)
+    assert clear > heads * sum(counts) // 2
+
+
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 64), (8, 2, 128), (4, 2, 256), (2, 1, 512)])
+@pytest.mark.parametrize("lengths,counts", SCORE_BATCHES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_beyond_fp32(env, dev, heads, kv_heads, width, lengths, counts, sign):
+    """Scores of about 1e42, of either sign or all of one: no answer in fp32, and none that looks like one. What sees
+    nothing still gives zeros."""
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 64, 34, spread=0.1)
+    used = table[table >= 0][table[table >= 0] < cache.pages]
+    q *= np.float32(1e21)
+    cache.k.scales[used] *= np.float32(1e21)
+    cache.put()
+    got = run_attention(env, dev, cache, q, starts, lengths, table)
+    assert np.all(np.isnan(got[:starts[-1]]))
+    # All scores far above, or far below.
+    q = np.abs(q)
+    cache.k.codes[:] = sign * np.maximum(np.abs(cache.k.codes), 1)
+    cache.put()
+    got = run_attention(env, dev, cache, q, starts, lengths, table)
+    assert np.all(np.isnan(got[:starts[-1]]))
+    table[:] = -1
+    got = run_attention(env, dev, cache, q, starts, lengths, table)
+    assert np.all(got[:starts[-1]] == 0)
+
+
+def test_some_scores_below_fp32(env, dev):
+    """A position whose score is below fp32's range weighs nothing beside others."""
+    for heads, kv_heads, width in ((8, 2, 64), (4, 2, 256)):
+        for tokens in (1, 40):
+            lengths = [200]
+            cache, q, starts, table = make_attention(env, dev, lengths, [tokens], heads, kv_heads, width, 64, 35)
+            q = np.abs(q)
+            far = table[0, 1]
+            cache.k.codes[far] = -np.maximum(np.abs(cache.k.codes[far]), 1)
+            cache.k.scales[far] = 1e38
+            cache.put()
+            got = run_attention(env, dev, cache, q, starts, lengths, table)
+            hole = table.copy()
+            hole[0, 1] = -1
+            check_attention(cache, q, got, starts, lengths, hole)
