@@ -18,17 +18,18 @@ namespace {
 
 constexpr int kPageThreads = 1024;
 
-// Exclusive prefix sums over the workgroup's threads, saturating at `most`
-// (a + b of two values up to INT_MAX fits 32 bits); *total over all of them.
+constexpr uint32_t kMost = INT_MAX;   // where sums saturate: two such values add up within 32 bits
+
+// Exclusive prefix sums over the workgroup's threads; *total over all of them.
 // `parts`: one word per wavefront.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t most, uint32_t *parts, uint32_t *total)
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *parts, uint32_t *total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t s = v;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const uint32_t o = (uint32_t)__shfl_up((int)s, d, 64);
-        if (lane >= d) s = min(s + o, most);
+        if (lane >= d) s = min(s + o, kMost);
     }
     __syncthreads();   // the last call's parts are read
     if (lane == 63) parts[wave] = s;
@@ -37,11 +38,11 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t most, uint
 #pragma unroll
     for (int w = 0; w < kPageThreads / 64; ++w) {
         if (w == wave) before = all;
-        all = min(all + parts[w], most);
+        all = min(all + parts[w], kMost);
     }
     *total = all;
     const uint32_t own = (uint32_t)__shfl_up((int)s, 1, 64);
-    return min(before + (lane ? own : 0), most);
+    return min(before + (lane ? own : 0), kMost);
 }
 
 __device__ __forceinline__ int clamped(int v, int most) { return v < 0 ? 0 : v > most ? most : v; }
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(kPageThreads) void page_tables(PageStep p)
             }
         }
         uint32_t total;
-        first[tid] = block_prefix(back, INT_MAX, parts, &total);
+        first[tid] = block_prefix(back, parts, &total);
         base[tid] = need;
         __syncthreads();
         for (uint32_t i = tid; i < total; i += kPageThreads) {
@@ -112,12 +113,12 @@ __global__ __launch_bounds__(kPageThreads) void page_tables(PageStep p)
             if (!beyond && need > held) grow = (uint32_t)(need - held);
         }
         uint32_t total, served;
-        const uint32_t before = min(asked + block_prefix(grow, INT_MAX, parts, &total), (uint32_t)INT_MAX);
+        const uint32_t before = min(asked + block_prefix(grow, parts, &total), kMost);
         const bool fits = before + grow <= top;
         const uint32_t mine = fits ? grow : 0;
         // A request that is not served, and with it every later one that
         // needs pages, takes nothing: those served are a prefix.
-        first[tid] = block_prefix(mine, INT_MAX, parts, &served);
+        first[tid] = block_prefix(mine, parts, &served);
         base[tid] = held;
         if (mine) p.held[r] = held + (int)mine;
         __syncthreads();
@@ -126,21 +127,22 @@ __global__ __launch_bounds__(kPageThreads) void page_tables(PageStep p)
             p.table[(size_t)(c * kPageThreads + k) * p.table_stride + base[k] + (i - first[k])] =
                 p.free_pages[top - 1 - given - i];
         }
-        asked = min(asked + total, (uint32_t)INT_MAX);
+        asked = min(asked + total, kMost);
         given += served;
         uint32_t left;
-        block_prefix(beyond || (grow && !fits) ? 1 : 0, INT_MAX, parts, &left);
+        block_prefix(beyond || (grow && !fits) ? 1 : 0, parts, &left);
         refused += left;
     }
-    // 3. The rows' starts.
+    // 3. The rows' starts, those past max_tokens too: attention takes a
+    // request's positions from them.
     uint32_t rows = 0;
     for (int c = 0; c < chunks; ++c) {
         const int r = c * kPageThreads + tid;
-        const uint32_t n = r < p.requests ? (uint32_t)clamped(p.counts[r], p.max_tokens) : 0;
+        const uint32_t n = r < p.requests ? (uint32_t)max(p.counts[r], 0) : 0;
         uint32_t total;
-        const uint32_t before = block_prefix(n, (uint32_t)p.max_tokens, parts, &total);
-        if (r < p.requests) p.starts[r] = (int)min(rows + before, (uint32_t)p.max_tokens);
-        rows = min(rows + total, (uint32_t)p.max_tokens);
+        const uint32_t before = block_prefix(n, parts, &total);
+        if (r < p.requests) p.starts[r] = (int)min(rows + before, kMost);
+        rows = min(rows + total, kMost);
     }
     if (tid == 0) {
         p.starts[p.requests] = (int)rows;
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(kPageThreads) void page_small(PageStep p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool mine = tid < p.requests;
     const int length = mine ? max(p.lengths[tid], 0) : 0;
-    const uint32_t n = mine ? (uint32_t)clamped(p.counts[tid], p.max_tokens) : 0;
+    const uint32_t n = mine ? (uint32_t)max(p.counts[tid], 0) : 0;
     int held = mine ? clamped(p.held[tid], p.table_stride) : 0;
     uint32_t top = (uint32_t)clamped(p.free_count[0], p.pages);
     const int need = (int)(((uint32_t)length + p.page_tokens - 1) / p.page_tokens);
@@ -192,13 +194,12 @@ __global__ __launch_bounds__(kPageThreads) void page_small(PageStep p)
     const uint32_t back = !beyond && held > need ? (uint32_t)(held - need) : 0;
     const uint32_t grow = !beyond && need > held ? (uint32_t)(need - held) : 0;
     uint32_t sums[3] = {back, grow, n};
-    const uint32_t most[3] = {INT_MAX, INT_MAX, (uint32_t)p.max_tokens};
 #pragma unroll
     for (int d = 1; d < 64; d *= 2)
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
             const uint32_t o = (uint32_t)__shfl_up((int)sums[k], d, 64);
-            if (lane >= d) sums[k] = min(sums[k] + o, most[k]);
+            if (lane >= d) sums[k] = min(sums[k] + o, kMost);
         }
     if (lane == 63)
 #pragma unroll
@@ -212,10 +213,10 @@ __global__ __launch_bounds__(kPageThreads) void page_small(PageStep p)
 #pragma unroll
         for (int w = 0; w < kWavesHere; ++w) {
             if (w == wave) here = all;
-            all = min(all + parts[k][w], most[k]);
+            all = min(all + parts[k][w], kMost);
         }
         const uint32_t own = (uint32_t)__shfl_up((int)sums[k], 1, 64);
-        before[k] = min(here + (lane ? own : 0), most[k]);
+        before[k] = min(here + (lane ? own : 0), kMost);
         total[k] = all;
     }
     // 1. Pages past the need, back on the stack.
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(256) void page_rows(PageStep p)
     if (row >= p.max_tokens) return;
     const bool live = row < p.starts[p.requests];
     const int r = last_from((const uint32_t *)p.starts, p.requests, (uint32_t)row);
-    place_row(p, row, live, r, p.starts[r], max(p.lengths[r], 0), clamped(p.counts[r], p.max_tokens),
+    place_row(p, row, live, r, p.starts[r], max(p.lengths[r], 0), max(p.counts[r], 0),
               clamped(p.held[r], p.table_stride));
 }
 

@@ -59,8 +59,10 @@ extern "C" {
  *      table[r][p / page_tokens] * page_tokens + p % page_tokens of the
  *      cache, or -1 where the request holds no such page. Rows from
  *      starts[requests] to max_tokens: position -1, slot -1 (a batch padded
- *      for a captured graph). Rows past max_tokens are cut off: size it for
- *      the step.
+ *      for a captured graph). Rows past max_tokens are cut off, a request's
+ *      last ones: they have a place in `starts` (starts[requests] >
+ *      max_tokens says so; it ends at INT_MAX) but no position and slot, and
+ *      the others keep theirs, here and in attention.
  * Negative lengths and counts are taken as 0. Run again with the same
  * lengths it changes nothing. requests <= 65536, and
  * requests * table_stride, table_stride * page_tokens and

@@ -73,16 +73,15 @@ class Pages:
         positions, slots = np.full(max_tokens, -1, np.int32), np.full(max_tokens, -1, np.int32)
         row = 0
         for r in range(requests):
-            starts[r] = row
-            for j in range(max(int(counts[r]), 0)):
-                if row == max_tokens:
-                    break
-                p = max(int(lengths[r]), 0) - min(int(counts[r]), max_tokens) + j
-                positions[row] = p
+            starts[r] = min(row, 2**31 - 1)
+            count = max(int(counts[r]), 0)
+            for j in range(min(count, max(max_tokens - row, 0))):
+                p = max(int(lengths[r]), 0) - count + j
+                positions[row + j] = p
                 if p >= 0 and p // self.page_tokens < self.held[r]:
-                    slots[row] = self.table[r, p // self.page_tokens] * self.page_tokens + p % self.page_tokens
-                row += 1
-        starts[requests] = row
+                    slots[row + j] = self.table[r, p // self.page_tokens] * self.page_tokens + p % self.page_tokens
+            row += count
+        starts[requests] = min(row, 2**31 - 1)
         return starts, positions, slots
 
 

@@ -3,10 +3,54 @@ the statements in serving_check.py."""
 import numpy as np
 import pytest
 
-from serving_check import F32_HALF, attention_bound
-from test_gpu_serving import check_attention, dev, env, make_attention, run_attention   # noqa: F401 (fixtures)
+from serving_check import F32_HALF, Pages, attention_bound
+from test_gpu_serving import (DevicePages, Server, check_attention, dev, env, make_attention,   # noqa: F401 (fixtures)
+                              run_attention)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- steps that do not fit --------------------------------------------------
+
+@pytest.mark.parametrize("requests", [3, 1027])
+def test_rows_cut_off(env, dev, requests):
+    """Rows past max_tokens are the step's last ones; the others keep position lengths - counts + j and their slots,
+    whether a request brings more than fits by itself or the ones before it took the room."""
+    table = np.full((requests, 4), -1, np.int32)
+    table[:3] = np.arange(12).reshape(3, 4)
+    none = [0] * (requests - 3)
+    for counts, room, want in (([5, 6, 9], 8, [35, 36, 37, 38, 39, 24, 25, 26]),
+                               ([30, 1, 1], 4, [10, 11, 12, 13]),
+                               ([0, 6, 2], 7, [24, 25, 26, 27, 28, 29, 7]),
+                               ([40, 2**31 - 1, 2**31 - 1], 3, [0, 1, 2])):
+        state = Pages(requests, 4, 20, 16, np.arange(20))
+        state.table[:], state.held[:3], state.free_count[0] = table, [3, 2, 1], 8
+        lengths = [40, 30, 9] + none
+        device = DevicePages(env, dev, state, room)
+        device.step(lengths, counts + none)
+        starts = dev.get(device.starts, np.empty(requests + 1, np.int32))
+        assert np.array_equal(starts[:4], np.minimum(np.cumsum([0] + counts), 2**31 - 1))
+        assert np.all(starts[3:] == starts[3])
+        positions, slots = (dev.get(p, np.empty(room + 1, np.int32)) for p in (device.positions, device.slots))
+        assert positions.tolist() == want + [-7]
+        request = np.repeat([0, 1, 2], np.minimum(counts, 50))[:room]
+        assert np.array_equal(slots[:-1], table[request, np.array(want) // 16] * 16 + np.array(want) % 16)
+        assert slots[-1] == -7
+        # What the statement of the page step gives.
+        device.check(*state.step(lengths, counts + none, room))
+
+
+@pytest.mark.parametrize("max_tokens", [7, 48])
+def test_steps_cut_off(env, dev, max_tokens):
+    """Page step, store and attention agree on the positions of a step's rows when not all of them fit: no row sees
+    one that comes later or was never stored."""
+    server = Server(env, dev, max_tokens=max_tokens)
+    for lengths, counts in [([40, 30, 0, 0, 0], [40, 30, 0, 0, 0]), ([5, 20, 3, 0, 0], [5, 20, 3, 0, 0]),
+                            ([300, 21, 4, 9, 0], [300, 1, 1, 9, 0]), ([6, 28, 11, 16, 12], [1, 7, 7, 7, 12])]:
+        server.inputs(lengths, counts)
+        server.launch()
+        env[0].sync(env[2])
+        server.check(lengths, counts)
 
 
 # ---- attention: work split over the positions ------------------------------
