@@ -627,20 +627,24 @@ __device__ __forceinline__ void store_run(const Store &args, int row, int head, 
         }
     }
     const float inverse = 1.f / scale;
+    // Under an infinite scale every code is 0, so that code * scale is NaN.
+    const uint32_t keep = __builtin_isfinite(scale) ? ~0u : 0u;
     if (tid == 0) *scale_at = scale;
     if (brief) {
 #pragma unroll
         for (int p = 0; p < kShort; ++p) {
             const int i = tid + 256 * p, t = at + i / W, d = i % W;
-            if (i < n * W) bytes[kind ? value_at(t, d, W) : key_at(t, d, page_tokens)] = code_of(few[p], scale, inverse);
+            if (i < n * W)
+                bytes[kind ? value_at(t, d, W) : key_at(t, d, page_tokens)] = (int8_t)(code_of(few[p], scale, inverse) & keep);
         }
 #pragma unroll 1
         for (int i = tid + 256 * kShort; i < n * W; i += 256)
-            bytes[key_at(at + i / W, i % W, page_tokens)] = code_of(element(i), scale, inverse);
+            bytes[key_at(at + i / W, i % W, page_tokens)] = (int8_t)(code_of(element(i), scale, inverse) & keep);
         return;
     }
     auto put = [&](int i, const float (&x)[16]) {
-        const uint4 w = codes_of(x, scale, inverse);
+        uint4 w = codes_of(x, scale, inverse);
+        w = make_uint4(w.x & keep, w.y & keep, w.z & keep, w.w & keep);
         if (kind) {
             // Positions of the granule outside the run keep their codes.
             const int g = g0 + i / W, from = at - 16 * g, to = at + n - 16 * g;

@@ -3,9 +3,9 @@ the statements in serving_check.py."""
 import numpy as np
 import pytest
 
-from serving_check import F32_HALF, Pages, attention_bound
-from test_gpu_serving import (DevicePages, Server, check_attention, dev, env, make_attention,   # noqa: F401 (fixtures)
-                              run_attention)
+from serving_check import F32_HALF, Pages, angles_of, attention_bound
+from test_gpu_serving import (DeviceCache, DevicePages, Server, check_attention, dev, env,   # noqa: F401 (fixtures)
+                              make_attention, run_attention, run_store)
 
 pytestmark = pytest.mark.gpu
 
@@ -51,6 +51,66 @@ def test_steps_cut_off(env, dev, max_tokens):
         server.launch()
         env[0].sync(env[2])
         server.check(lengths, counts)
+
+
+# ---- the cache: elements that are not finite ---------------------------------
+
+@pytest.mark.parametrize("page_tokens,width,heads,rotated,shift", [(16, 64, 2, 64, 0), (64, 128, 2, 20, 0),
+                                                                   (128, 512, 0, 0, 0), (32, 256, 0, 0, 4)])
+def test_loads_of_what_is_not_finite(env, dev, page_tokens, width, heads, rotated, shift):
+    """A head's rows of a page with an infinite or NaN element read as NaN, all of them, from a long run and from a
+    single token, and still after a finite token; other heads read as stored."""
+    rt, kern, stream = env
+    rng = np.random.default_rng(width)
+    kv_heads = 4
+    cache = DeviceCache(env, dev, 3, page_tokens, kv_heads, width, rng)
+    frequencies, _ = kern.rope_frequencies(max(rotated, 2), 10000.0)
+
+    def read(slots):
+        n = kv_heads * width
+        rows = dev.put(np.zeros((len(slots), 2 * n), np.float32))
+        kern.kv8_load(cache.arg, dev.put(np.array(slots, np.int32)), len(slots), rows, 2 * n, rows + 4 * n, 2 * n, stream)
+        rt.sync(stream)
+        return dev.get(rows, np.empty((len(slots), 2, kv_heads, width), np.float32))
+
+    def store(slots, bad):
+        """Rows into these slots; bad: the values at element `width - 3` of the last row's K and V heads 0, 1, ..."""
+        x = rng.standard_normal((len(slots), heads + 2 * kv_heads, width)).astype(np.float32)
+        for h, b in enumerate(bad):
+            x[-1, heads + h, width - 3] = x[-1, heads + kv_heads + h, width - 3] = b
+        angles = angles_of(np.array(slots) % page_tokens, frequencies, 1.0).astype(np.float32)
+        with np.errstate(invalid="ignore"):
+            run_store(env, dev, cache, slots, x, heads, rotated, False, angles, shift)
+        cache.check()
+
+    def check(slots, bad):
+        got = read(slots)
+        assert np.all(np.isnan(got[:, :, bad]))
+        fine = [h for h in range(kv_heads) if h not in bad]
+        for kind, c in enumerate((cache.k, cache.v)):
+            page, t = np.array(slots) // page_tokens, np.array(slots) % page_tokens
+            want = c.codes[page, :, t].astype(np.float32) * c.scales[page][..., None]
+            assert np.array_equal(got[:, kind, fine], want[:, fine])
+
+    # A run from a page's first slot on, a token more, a finite one after it.
+    run = list(range(page_tokens, page_tokens + page_tokens - 3))
+    store(run, [np.inf, -np.inf, np.nan])
+    check(run, [0, 1, 2])
+    store([run[-1] + 1], [])
+    check(run + [run[-1] + 1], [0, 1, 2])
+    # A page that was fine; then infinity after NaN and NaN after infinity.
+    run = list(range(2 * page_tokens, 2 * page_tokens + 5))
+    store(run, [])
+    check(run, [])
+    store([run[-1] + 1], [np.inf, np.nan, -np.inf])
+    store([run[-1] + 2], [np.nan, np.inf, -np.inf])
+    run += [run[-1] + 1, run[-1] + 2]
+    check(run, [0, 1, 2])
+    # A whole page, and anew.
+    store(list(range(page_tokens)), [-np.inf, np.inf, np.nan])
+    check(list(range(page_tokens)), [0, 1, 2])
+    store([0], [])
+    check([0], [])
 
 
 # ---- attention: work split over the positions ------------------------------
