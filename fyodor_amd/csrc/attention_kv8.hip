@@ -102,7 +102,14 @@ __device__ __forceinline__ float column_sum(float v)
 constexpr float kFar = 0x1p22f;
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
 
-// What a row's sum of weights makes of its outputs. Without weights the row saw
+// Sums of weights are held without the exponent e of the value scales (-99 to 122,
+// as stored): up to 2^(15 - e) for a position where outputs hold 2^15. Times kLess
+// they stay in fp32 at both ends, for up to 2^30 positions; kLess joins the outputs
+// at the end.
+constexpr int kLessBits = -18;
+constexpr float kLess = 0x1p-18f;
+
+// What a row's sum of weights makes of its outputs (times kLess). Without weights the row saw
 // nothing (no maximum) and gives zeros, or its scores were beyond fp32.
 __device__ __forceinline__ float inverse_of(float total, float top)
 {
@@ -368,7 +375,7 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
             }
             split_f16(w, ph[n], pl[n]);
         }
-        l += ldexpf(sum[0] + sum[1], -e);
+        l += ldexpf(sum[0] + sum[1], kLessBits - e);
 #pragma unroll
         for (int d0 = 0; d0 < D; d0 += 4) {
             uint4 v[4];
@@ -429,7 +436,8 @@ __device__ __forceinline__ void few_rows(const Kv8Attention &a, int r, int kvh, 
             } else {
                 float *out = a.out + (rq.begin + out_row / group) * a.out_stride +
                              (int64_t)(kvh * group + out_row % group) * W + 64 * i + mcol;
-                o *= inverse_of(total, top);
+                const float inverse = inverse_of(total, top);
+                o = o * kLess * inverse;
                 if (aligned) {
                     *(f32x4 *)out = o;
                 } else {
@@ -738,7 +746,7 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
                 }
                 split_f16(w, ph[t][n / 8], pl[t][n / 8]);
             }
-            l += ldexpf(sum[0] + sum[1], -e[t]);
+            l += ldexpf(sum[0] + sum[1], kLessBits - e[t]);
         }
     };
     // The next codes set out before the MFMAs and are there after them. A
@@ -818,8 +826,8 @@ void kv8_wide(Kv8Attention a, Split split, int most_rows)
     for (int d = 0; d < D; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float4 o = make_float4(O[d][4 * i] * inverse, O[d][4 * i + 1] * inverse, O[d][4 * i + 2] * inverse,
-                                         O[d][4 * i + 3] * inverse);
+            const float4 o = make_float4(O[d][4 * i] * kLess * inverse, O[d][4 * i + 1] * kLess * inverse,
+                                         O[d][4 * i + 2] * kLess * inverse, O[d][4 * i + 3] * kLess * inverse);
             if (aligned) {
                 *(float4 *)(out + 32 * d + 8 * i) = o;
             } else {
@@ -880,7 +888,7 @@ __device__ __forceinline__ void join_row(const Kv8Attention &a, const Split &spl
     float *out = a.out + (rq.begin + row / group) * a.out_stride + (int64_t)(kvh * group + row % group) * W + 4 * col;
     const float inverse = inverse_of(total, top);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) out[k] = o[k] * inverse;
+    for (int k = 0; k < 4; ++k) out[k] = o[k] * kLess * inverse;
 }
 
 // Wide tiles: workgroup (tile, 16 of its rows, KV head), a wavefront every
@@ -921,7 +929,7 @@ __device__ __forceinline__ void join_wide(const Kv8Attention &a, const Split &sp
         float *out = a.out + (rq.begin + row / group) * a.out_stride + (int64_t)(kvh * group + row % group) * W + lane;
         const float inverse = inverse_of(total, top);
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) out[64 * e] = o[e] * inverse;
+        for (int e = 0; e < kCols; ++e) out[64 * e] = o[e] * kLess * inverse;
     }
 }
 

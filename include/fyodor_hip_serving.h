@@ -178,7 +178,8 @@ NYA_HIP_EXPORT int nya_hip_kv8_load(const nya_hip_kv8 *cache, uintptr_t slots, s
  * q (and the softmax's weights) enter the matrix cores as two fp16 pieces,
  * 22 bits each, the codes exactly; all sums are fp32. A score above
  * 2^128 / log2(e) (2.3e38), or nothing but scores below minus that, gives NaN.
- * Which kernel and split
+ * Positions whose value scale is below 2^-116 of the largest one that a row
+ * sees may be missing from its sum of weights. Which kernel and split
  * runs goes by the arguments alone: the same call gives the same bits.
  *
  * `workspace` (16-byte aligned) is scratch for work split over several

@@ -238,3 +238,39 @@ def test_some_scores_below_fp32(env, dev):
             hole = table.copy()
             hole[0, 1] = -1
             check_attention(cache, q, got, starts, lengths, hole)
+
+
+@pytest.mark.parametrize("heads,kv_heads,width,counts", [(4, 2, 64, [1, 1, 1]), (2, 1, 128, [20, 1, 2]),
+                                                        (2, 2, 256, [1, 70, 3]), (2, 1, 512, [1, 2, 1])])
+@pytest.mark.parametrize("workspace", [None, 0])
+def test_small_and_large_values(env, dev, heads, kv_heads, width, counts, workspace):
+    """Equal scores over many positions whose values are as small as a page's scale can be (which a head of zeros
+    stores, too), alone and before larger values, and over the largest ones."""
+    lengths = [70000, 40000, 3]
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 128, 36, spread=0.0)
+    q[:] = 0
+    small, large = 2.0 ** -100, 2.0 ** 120
+    codes = cache.v.codes.copy()
+    for base, tail in ((small, small), (large, large), (small, 1 / 90), (small, 2.0 ** 15)):
+        cache.v.codes[:] = codes
+        for r, n in enumerate(lengths):
+            need = -(-n // 128)
+            few = 2 * need // 3
+            cache.v.scales[table[r, :few]], cache.v.scales[table[r, few:need]] = base, tail
+            if tail != base:
+                cache.v.codes[table[r, :few]] = 0
+        cache.put()
+        got = run_attention(env, dev, cache, q, starts, lengths, table, workspace=workspace)
+        values = cache.v.values()
+        for r, n in enumerate(lengths):
+            t = np.arange(n)
+            for h in range(kv_heads):
+                v = values[table[r, t // 128], h, t % 128]
+                total, top = np.cumsum(v, 0), np.abs(v).max()
+                bound = attention_bound(0, top, width, n)   # all scores are 0 exactly
+                for row in range(starts[r], starts[r + 1]):
+                    last = n - (starts[r + 1] - row) + 1
+                    want = total[last - 1] / last
+                    assert np.abs(want).max() > 2 * bound
+                    off = np.abs(got[row, h * heads // kv_heads:(h + 1) * heads // kv_heads] - want)
+                    assert np.all(off <= bound), (base, tail, row)
