@@ -525,13 +525,33 @@ __device__ __forceinline__ uint4 codes_of(const float (&x)[16], float scale, flo
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The nearest row in the cache of the 128 from `row` on (step 1) or back (-1): it
+// if it is of this page, else -1.
+__device__ __forceinline__ int page_goes_on(const Store &s, int row, int step, int page, int shift)
+{
+    const int lane = threadIdx.x & 63;
+    for (int k = 0; k < 128; k += 64) {
+        const int at = row + step * (k + lane), slot = s.slots[min(max(at, 0), s.count - 1)];
+        const uint64_t live = __builtin_amdgcn_ballot_w64(at >= 0 && at < s.count &&
+                                                          (unsigned)slot < (unsigned)(s.c.pages * s.c.page_tokens));
+        if (live) {
+            const int first = __builtin_ctzll(live);
+            return __builtin_amdgcn_readlane(slot, first) >> shift == page ? row + step * (k + first) : -1;
+        }
+    }
+    return -1;
+}
+
 // The run of rows that begins at `row`: its head's keys (kind 0) or values. In
 // a long run a thread forms 16 codes that lie together: of one position's key, or
 // of 16 positions of one element of the values; in a short one (decoding) single
 // codes. Bound by its chain of waits (slots, rows and the old scale, codes) for a
 // few rows, by the rows' bytes for many.
+//
+// Returns the row where the page's next run begins, -1 where there is none: runs of
+// one page share its scale, so one workgroup takes them in turn.
 template <int W>
-__device__ __forceinline__ void store_run(const Store &args, int row, int head, int kind, uint32_t *top)
+__device__ __forceinline__ int store_run(const Store &args, int row, int head, int kind, uint32_t *top)
 {
     constexpr int kChunks = W / 16, kShort = 4;   // elements per thread of a short run
     Store s = args;
@@ -551,6 +571,14 @@ __device__ __forceinline__ void store_run(const Store &args, int row, int head, 
         if (off0) n = __builtin_ctzll(off0);
         else if (off1) n = 64 + __builtin_ctzll(off1);
     }
+    // The next run's row: mostly the slot after this run says that there is none;
+    // else it is looked for when the stores have set out.
+    bool last = at + n == page_tokens || row + n == s.count;
+    if (!last) {
+        const unsigned then = __builtin_amdgcn_readlane(n < 64 ? next0 : next1, n & 63);
+        last = then < (unsigned)(c.pages * page_tokens) && (int)then >> shift != page;
+    }
+    auto next_run = [&]() { return last ? -1 : page_goes_on(s, row + n, 1, page, shift); };
     const size_t place = (size_t)page * c.kv_heads + head;
     uint4 *codes = (uint4 *)((kind ? c.values : c.keys) + place * page_tokens * W);
     int8_t *bytes = (int8_t *)codes;
@@ -640,7 +668,7 @@ __device__ __forceinline__ void store_run(const Store &args, int row, int head, 
 #pragma unroll 1
         for (int i = tid + 256 * kShort; i < n * W; i += 256)
             bytes[key_at(at + i / W, i % W, page_tokens)] = (int8_t)(code_of(element(i), scale, inverse) & keep);
-        return;
+        return next_run();
     }
     auto put = [&](int i, const float (&x)[16]) {
         uint4 w = codes_of(x, scale, inverse);
@@ -671,6 +699,7 @@ __device__ __forceinline__ void store_run(const Store &args, int row, int head, 
         piece_at(i, x);
         put(i, x);
     }
+    return next_run();
 }
 
 // Workgroup (group of rows, 2 head + kind): the runs that begin in its rows;
@@ -698,12 +727,21 @@ __global__ __launch_bounds__(256, 3) void kv8_store(Store s)
     const int lane = threadIdx.x & 63, rows = min(s.rows, s.count - first_row);
     if (rows <= 0) return;
     const int row = first_row + min(lane, rows - 1), slot = s.slots[row], before = row ? s.slots[row - 1] : -2;
-    uint64_t mask = __builtin_amdgcn_ballot_w64(lane < rows && (unsigned)slot < (unsigned)(s.c.pages * s.c.page_tokens) &&
-                                                (before != slot - 1 || (slot & (s.c.page_tokens - 1)) == 0));
-    for (; mask; mask &= mask - 1) {
-        store_run<W>(s, first_row + __builtin_ctzll(mask), part >> 1, part & 1, top);
-        __syncthreads();   // `top` is read
+    // The rows that are the first of their page: the row before is of another one. (If that
+    // is not in the cache, the nearest one before it says.)
+    const unsigned slots = (unsigned)(s.c.pages * s.c.page_tokens);
+    const int shift = 31 - __builtin_clz(s.c.page_tokens), page = slot >> shift;
+    const bool here = lane < rows && (unsigned)slot < slots, begins = row == 0 || (slot & (s.c.page_tokens - 1)) == 0;
+    uint64_t mask = __builtin_amdgcn_ballot_w64(here && (begins || ((unsigned)before < slots && before >> shift != page)));
+    for (uint64_t look = __builtin_amdgcn_ballot_w64(here && !begins && (unsigned)before >= slots); look; look &= look - 1) {
+        const int at = __builtin_ctzll(look);
+        if (page_goes_on(s, first_row + at - 1, -1, __builtin_amdgcn_readlane(page, at), shift) < 0) mask |= 1ull << at;
     }
+    for (; mask; mask &= mask - 1)
+        for (int run = first_row + __builtin_ctzll(mask); run >= 0;) {
+            run = store_run<W>(s, run, part >> 1, part & 1, top);
+            __syncthreads();   // `top` is read, the page's codes and scale are written
+        }
 }
 
 // Workgroup (rows, 1024 columns of heads x width): a thread 4 columns of each

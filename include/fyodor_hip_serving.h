@@ -144,8 +144,10 @@ NYA_HIP_EXPORT int nya_hip_kv8_bytes(const nya_hip_kv8 *cache, size_t *codes, si
  * overlap k or v), one launch for both; q without angles is declined.
  *
  * Rows of one page stand together, in the order of their positions, and no
- * slot twice. Such a run takes wanted = max|x| * (1 / 127) (in fp32, at least
- * 2^-100) of its rows in a head. A run from the page's first slot sets the
+ * slot twice; between two of them fewer than 128 rows may stand that are left
+ * out. Positions that follow each other in rows that do are a run; a page's
+ * runs are taken in their order. A run takes wanted = max|x| * (1 / 127) (in
+ * fp32, at least 2^-100) of its rows in a head. A run from the page's first slot sets the
  * scale to that; a later one raises it to that if it is lower, and the
  * page's codes are rounded again to the new step, code = round(code * old /
  * new). Codes are round(x / scale), exactly (ties to even), of fp32 values

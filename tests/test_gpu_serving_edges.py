@@ -113,6 +113,50 @@ def test_loads_of_what_is_not_finite(env, dev, page_tokens, width, heads, rotate
     check([0], [])
 
 
+# ---- the cache: pages whose rows have gaps ------------------------------------
+
+@pytest.mark.parametrize("page_tokens,kv_heads,width,pages,rotated", [
+    (16, 2, 64, 9, 32), (32, 8, 64, 60, 64), (64, 1, 128, 5, 0), (128, 2, 256, 4, 256), (128, 8, 128, 12, 128),
+    (64, 2, 512, 3, 30)])
+def test_store_with_gaps(env, dev, page_tokens, kv_heads, width, pages, rotated):
+    """Pages of which some positions are not stored, as rows that are left out or without rows at all: their runs share
+    the page's scale, which grows from run to run."""
+    rng = np.random.default_rng(pages)
+    cache = DeviceCache(env, dev, pages, page_tokens, kv_heads, width, rng)
+    frequencies, _ = env[1].rope_frequencies(max(rotated, 2), 10000.0)
+    for kept, rows_of_others in ((0.5, True), (0.8, False), (0.05, True), (0.95, False)):
+        slots, sizes = [], []
+        for page in rng.permutation(pages):
+            positions = np.arange(page_tokens)
+            keep = rng.random(page_tokens) < kept
+            if rng.random() < 0.5:
+                keep[0] = True
+            here = page * page_tokens + positions
+            here = np.where(keep, here, rng.choice([-1, pages * page_tokens, -2**31])) if rows_of_others else here[keep]
+            slots += here.tolist()
+            sizes += (1 + np.arange(len(here)) * rng.choice([0, 0.3, -0.9 / page_tokens])).tolist()
+            if rng.random() < 0.3:
+                slots += [-1] * 5
+                sizes += [1.0] * 5
+        x = rng.standard_normal((len(slots), 2 * kv_heads, width)) * np.array(sizes)[:, None, None]
+        angles = angles_of(np.array(slots) % page_tokens, frequencies, 1.0).astype(np.float32)
+        run_store(env, dev, cache, np.array(slots, np.int64).astype(np.int32), x.astype(np.float32), 0, rotated, True,
+                  angles)
+        cache.check()
+
+
+def test_store_with_far_gaps(env, dev):
+    """Two rows of a page with 127 left out between them, and single positions of a page in turn."""
+    rng = np.random.default_rng(5)
+    cache = DeviceCache(env, dev, 3, 128, 2, 64, rng)
+    for slots in ([0] + [-1] * 127 + [127] + [-1] * 127 + [128] + [-1] * 40 + [200], list(range(256, 384, 2)),
+                  [-1] * 300 + [383] + [-1] * 300):
+        x = rng.standard_normal((len(slots), 4, 64)).astype(np.float32)
+        x *= (1 + np.arange(len(slots), dtype=np.float32))[:, None, None]
+        run_store(env, dev, cache, slots, x, 0, 0, False, np.zeros((len(slots), 32, 2), np.float32))
+        cache.check()
+
+
 # ---- attention: work split over the positions ------------------------------
 
 def dense_attention(cache, table, q, first, counts, window, scale):
