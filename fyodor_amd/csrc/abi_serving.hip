@@ -107,6 +107,8 @@ NYA_HIP_EXPORT int nya_hip_rope_frequencies(float *out, size_t rotated, double b
     if (scaling != NYA_HIP_ROPE_NONE && (!(factor >= 1) || !isfinite(factor))) return 1;
     if (bands && (!(original > 0) || !isfinite(original) || !(low >= 0) || !(high > low) || !isfinite(high))) return 1;
     if (scaling == NYA_HIP_ROPE_RAMP && !(low > 0)) return 1;
+    for (size_t j = 0; factors && j < rotated / 2; ++j)
+        if (!isfinite(factors[j]) || factors[j] == 0) return 1;
     const double turn = 2 * M_PI, r = (double)rotated;
     // The pair that turns n times within `original` positions: base^(-2j/r) original / 2 pi = n.
     const auto pair_of = [&](double n) { return r * log(original / (turn * n)) / (2 * log(base)); };

@@ -90,8 +90,8 @@ enum { NYA_HIP_ROPE_INTERLEAVED = 0, NYA_HIP_ROPE_HALVES = 1 };
  *           up) one that turns `low` (> 0) times, and *magnitude =
  *           1 + 0.1 ln(factor).
  * *magnitude, which multiplies (cos, sin), is 1 otherwise. factors (or
- * null): rotated / 2 floats that divide the base frequencies first, a
- * model's own rope factors. On the host: `out` receives rotated / 2 floats,
+ * null): rotated / 2 floats, finite and not 0, that divide the base
+ * frequencies first, a model's own rope factors. On the host: `out` receives rotated / 2 floats,
  * each the 64-bit result rounded once. */
 enum { NYA_HIP_ROPE_NONE = 0, NYA_HIP_ROPE_LINEAR = 1, NYA_HIP_ROPE_BANDS = 2, NYA_HIP_ROPE_RAMP = 3 };
 NYA_HIP_EXPORT int nya_hip_rope_frequencies(float *out, size_t rotated, double base, const float *factors,
