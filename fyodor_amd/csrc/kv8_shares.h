@@ -140,7 +140,9 @@ inline Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         // a request of a few rows might have, the tiles that one token takes (a
         // prompt of 512 among 64 requests, 32 heads over 8 of 128: 176 us, with
         // two tiles 188; 64 over 2 of 64: 107 with the two tiles of a token, 149
-        // with it in wide ones); a single request is all wide.
+        // with it in wide ones); a single request is all wide. It loses where single
+        // tokens are many and take many tiles: 130 requests with a prompt among
+        // them, 32 heads over 1 of 128: 83, in wide tiles 67.
         p.most_rows = a.requests == 1 ? 0 : group > 64 ? kRows : (group + kRows - 1) / kRows * kRows;
         p.any_wide = true;
         p.any_few = a.requests > 1;
@@ -163,7 +165,9 @@ inline Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         // tiles: none, sharing costs about 6 us (32 requests of 2048 positions, 8
         // heads of 128, us: whole 25, halves 31, quarters 34), but in long contexts,
         // where the requests' lengths differ by more (64 of 500 to 8192: whole 105,
-        // 2048 shares were they all long 97).
+        // 2048 shares were they all long 97). The border, 96 steps, is on the side of
+        // whole ones (64 requests of 300 to n positions, whole and in shares: n 1500
+        // 25 and 37, 3000 46 and 50, 4500 63 and 59, 5900 77 and 68).
         const int64_t wanted = tiles < 256 ? (width <= 128 ? 768 : 256) : steps >= 96 ? 2048 : 0;
         const int64_t share = wanted ? (tiles * steps + wanted - 1) / wanted : steps;
         if (share > p.few.least) p.few.least = (int)share;
@@ -172,7 +176,9 @@ inline Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
         // Requests of unequal lengths leave gaps in a grid of all their shares,
         // and the CUs get unequal work; counting them costs a look at
         // every request, one for up to 64 (32 and 64 of 500 to 8192 positions: 53
-        // and 98 us, counted 50 and 91; 16, with 128 tiles, 28 and 29).
+        // and 98 us, counted 50 and 91; 16, with 128 tiles, 28 and 29; past 64
+        // it gains nothing: 65 requests 94 both, 96 128 and 130, 192 of up to
+        // 6500 209 and 213).
         p.few.packed = p.few.most > 1 && tiles >= 256 && a.requests <= 64 && !p.few.listed;
     }
     if (p.any_wide) {

@@ -99,8 +99,9 @@ NYA_HIP_EXPORT int nya_hip_rope_frequencies(float *out, size_t rotated, double b
 
 /* angles[i][j] = (cos, sin)(positions[i] * frequencies[j]) * magnitude for
  * `count` positions and rotated / 2 (at most 512) frequencies: the
- * table (8-byte aligned) that every layer of a step reads. Formed in 64 bits,
- * so far positions lose nothing, and rounded once. */
+ * table (8-byte aligned) that every layer of a step reads. Formed in 64 bits
+ * and rounded once; the phase is right to p f 2^-51 (2^-27 at position 2^24,
+ * 2^-20 at the last one). */
 NYA_HIP_EXPORT int nya_hip_rope_angles(uintptr_t positions, size_t count, uintptr_t frequencies, size_t rotated,
     float magnitude, uintptr_t angles, uintptr_t stream);
 
@@ -122,8 +123,10 @@ NYA_HIP_EXPORT int nya_hip_rope(uintptr_t q, size_t q_stride, uintptr_t q_out, s
  * attention's loads: element d of position t
  *     of a key at    (d / 16 * page_tokens + t) * 16 + d % 16,
  *     of a value at  (t / 16 * width + d) * 16 + t % 16.
- * Scales at page * kv_heads + head. Codes 16-byte aligned. Nothing needs to
- * be cleared: a page's scale begins with its first position. */
+ * Scales at page * kv_heads + head; a page's, once its first position is
+ * stored, is from 2^-100 to FLT_MAX / 127, infinite or NaN. Codes 16-byte
+ * aligned. Nothing needs to be cleared: a page's scale begins with its first
+ * position. */
 typedef struct nya_hip_kv8 {
     uintptr_t keys, values;               /* nya_hip_kv8_bytes' *codes each */
     uintptr_t key_scales, value_scales;   /* *scales each */
