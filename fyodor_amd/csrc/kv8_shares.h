@@ -1,6 +1,7 @@
-// How attention over the paged 8-bit cache (attention_kv8.hip) is divided: the
-// positions that a tile of query rows sees, their shares, and the grids of a
-// call. Plain arithmetic, the same on the host and in the kernels.
+// How attention over a paged cache (attention_kv8.hip, attention_kv4.hip: A is its
+// arguments) is divided: the positions that a tile of query rows sees, their
+// shares, and the grids of a call. Plain arithmetic, the same on the host and
+// in the kernels.
 #pragma once
 #include "serving.h"
 
@@ -52,7 +53,8 @@ struct Request {
     int64_t first;     // position of its first token
 };
 
-__host__ __device__ __forceinline__ Request request_of(const Kv8Attention &a, int r)
+template <class A>
+__host__ __device__ __forceinline__ Request request_of(const A &a, int r)
 {
     const int start = a.starts[r], stop = a.starts[r + 1];
     const int begin = max(start, 0), end = max(min(stop, a.count), 0), tokens = min(end - begin, a.max_tokens);
@@ -60,7 +62,8 @@ __host__ __device__ __forceinline__ Request request_of(const Kv8Attention &a, in
             (int64_t)a.lengths[r] - ((int64_t)stop - begin)};
 }
 
-__host__ __device__ __forceinline__ Range range_of(const Kv8Attention &a, const Request &q, int tile, int rows, int splits,
+template <class A>
+__host__ __device__ __forceinline__ Range range_of(const A &a, const Request &q, int tile, int rows, int splits,
     int least)
 {
     const int group = a.heads / a.cache.kv_heads;
@@ -85,7 +88,8 @@ struct Items {
     int tiles, shares;
 };
 
-__host__ __device__ __forceinline__ Items items_of(const Kv8Attention &a, const Split &split, const Request &q,
+template <class A>
+__host__ __device__ __forceinline__ Items items_of(const A &a, const Split &split, const Request &q,
     int most_rows)
 {
     Items items = {0, 0};
@@ -120,12 +124,14 @@ struct Plan {
     Split few, wide;
 };
 
-inline size_t share_bytes(const Kv8Attention &a, const Split &s)
+template <class A>
+inline size_t share_bytes(const A &a, const Split &s)
 {
     return (size_t)s.places * s.tile * a.cache.kv_heads * (a.cache.width + 2) * sizeof(float);
 }
 
-inline Plan plan_of(const Kv8Attention &a, float *workspace, size_t bytes)
+template <class A>
+inline Plan plan_of(const A &a, float *workspace, size_t bytes)
 {
     const int group = a.heads / a.cache.kv_heads, width = a.cache.width;
     const int64_t rows = (int64_t)a.max_tokens * group;

@@ -46,6 +46,7 @@ hipError_t launch_kv8_load(const Kv8 &cache, const int *slots, int count, float 
     int64_t v_stride, hipStream_t s);
 
 struct Kv8Attention {
+    static constexpr float kLess = 0x1p-18f;   // sums of weights are held this much smaller
     Kv8 cache;
     const float *q;
     int64_t q_stride;
