@@ -21,7 +21,7 @@ LIB = ROOT / "lib"
 CSRC = ROOT / "csrc"
 HIP_SOURCES = ["abi.hip", "dense.hip", "smalln.hip", "matvec.hip", "rows_tokens.hip", "prefill.hip", "prefill_f16.hip",
                "resident.hip", "attention_tile.hip", "prefill_tile.hip", "abi_serving.hip", "serving.hip",
-               "attention_kv8.hip", "pack.cpp"]
+               "attention_kv8.hip", "abi_kv4.hip", "kv4.hip", "attention_kv4.hip", "logprobs.hip", "pack.cpp"]
 C_SOURCES = ["core/compute.c", "core/vendor.c", "rocm/rocm.c"]
 
 HIPCC_FLAGS = [
@@ -33,7 +33,7 @@ HIPCC_FLAGS = [
 # once in VALU code: results in VGPRs (not AGPRs) save a copy per register.
 EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("smalln.hip", "matvec.hip", "prefill_f16.hip",
                                                                 "attention_tile.hip", "prefill_tile.hip",
-                                                                "rows_tokens.hip", "attention_kv8.hip")}
+                                                                "rows_tokens.hip", "attention_kv8.hip", "attention_kv4.hip")}
 C_FLAGS = [
     "-std=c17", "-O2", "-fPIC", "-Wall", "-Wextra", "-Wpedantic", "-Wshadow",
     "-D_POSIX_C_SOURCE=200809L",

@@ -203,6 +203,25 @@ hipError_t launch_gelu_pairs(const float *gu, float *out, int n, int count, hipS
 hipError_t launch_greedy(const float *logits, int n, int count, const uint32_t *mask, uint32_t *ids,
     hipStream_t stream);
 
+// Log probabilities of given tokens, entropies and the most likely tokens of
+// rows of logits (include/fyodor_hip_logprobs.h).
+struct Logprobs {
+    const float *logits;
+    int64_t stride;
+    int n, count;
+    const uint32_t *mask;
+    float scale;
+    const int *tokens;
+    float *logprobs;
+    int *ranks;
+    float *entropies;
+    int top;
+    int *top_ids;
+    float *top_logprobs;
+};
+size_t logprobs_workspace(int n, int count, int top);
+hipError_t launch_logprobs(const Logprobs &a, void *workspace, size_t workspace_bytes, hipStream_t s);
+
 // Compute units of the current device (counted once per device).
 int device_cu_count();
 

@@ -105,12 +105,18 @@ class Kv8(ctypes.Structure):
                 ("page_tokens", _sz), ("kv_heads", _sz), ("width", _sz)]
 
 
+class Kv4(ctypes.Structure):
+    """nya_hip_kv4 (include/fyodor_hip_kv4.h)."""
+    _fields_ = [("keys", _up), ("values", _up), ("key_steps", _up), ("value_steps", _up), ("pages", _sz),
+                ("page_tokens", _sz), ("kv_heads", _sz), ("width", _sz)]
+
+
 ROPE_INTERLEAVED, ROPE_HALVES = 0, 1
 ROPE_SCALINGS = {"none": 0, "linear": 1, "bands": 2, "ramp": 3}
 
 
 class Kernels:
-    """libfyodor_hip.so (include/fyodor_hip.h, include/fyodor_hip_serving.h)."""
+    """libfyodor_hip.so (include/fyodor_hip.h, fyodor_hip_serving.h, fyodor_hip_kv4.h, fyodor_hip_logprobs.h)."""
 
     def __init__(self, path: Path = KERNEL_LIBRARY):
         if not Path(path).exists():
@@ -142,6 +148,15 @@ class Kernels:
         L.nya_hip_kv8_attention_bytes.argtypes = [cache, _sz, _sz, _sz, _sz, _sz, _sz, ctypes.POINTER(_sz)]
         L.nya_hip_kv8_attention.argtypes = [cache, _up, _sz, _up, _sz, _sz, _up, _up, _up, _sz, _sz, _sz, _sz, _sz,
                                             _sz, ctypes.c_float, _up, _sz, _up]
+        cache = ctypes.POINTER(Kv4)
+        L.nya_hip_kv4_bytes.argtypes = [cache, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]
+        L.nya_hip_kv4_store.argtypes = [cache] + L.nya_hip_kv8_store.argtypes[1:]
+        L.nya_hip_kv4_load.argtypes = [cache] + L.nya_hip_kv8_load.argtypes[1:]
+        L.nya_hip_kv4_attention_bytes.argtypes = [cache] + L.nya_hip_kv8_attention_bytes.argtypes[1:]
+        L.nya_hip_kv4_attention.argtypes = [cache] + L.nya_hip_kv8_attention.argtypes[1:]
+        L.nya_hip_logprobs_bytes.argtypes = [_sz, _sz, _sz, ctypes.POINTER(_sz)]
+        L.nya_hip_logprobs.argtypes = [_up, _sz, _sz, _sz, _up, ctypes.c_float, _up, _up, _up, _up, _sz, _up, _up, _up,
+                                       _sz, _up]
 
     def device_weights(self, w: np.ndarray, type_id: int, rows: int, cols: int) -> np.ndarray:
         """GGUF bytes -> the device layout (host side)."""
@@ -288,6 +303,75 @@ class Kernels:
                                                 window, scale, workspace, workspace_bytes, stream)
         if status != 0:
             raise HipError(f"nya_hip_kv8_attention returned {status}")
+
+    # ---- the cache in 4 bits (include/fyodor_hip_kv4.h) ----------------------
+
+    def kv4(self, keys: int, values: int, key_steps: int, value_steps: int, pages: int, page_tokens: int,
+            kv_heads: int, width: int) -> Kv4:
+        """The 4-bit paged cache at these device addresses."""
+        return Kv4(keys, values, key_steps, value_steps, pages, page_tokens, kv_heads, width)
+
+    def kv4_bytes(self, pages: int, page_tokens: int, kv_heads: int, width: int) -> tuple[int, int]:
+        """Bytes of each code array and of each step array."""
+        codes, steps = _sz(), _sz()
+        cache = Kv4(0, 0, 0, 0, pages, page_tokens, kv_heads, width)
+        if self.lib.nya_hip_kv4_bytes(ctypes.byref(cache), ctypes.byref(codes), ctypes.byref(steps)):
+            raise ValueError("cache geometry unsupported")
+        return codes.value, steps.value
+
+    def kv4_store(self, cache: Kv4, slots: int, count: int, k: int, k_stride: int, v: int, v_stride: int, angles: int,
+                  rotated: int, layout: int, q: int, q_stride: int, q_out: int, q_out_stride: int, heads: int,
+                  stream: int) -> None:
+        """Rows of k (rotated, with angles) and v into the cache, q rotated into q_out (q 0: none)."""
+        status = self.lib.nya_hip_kv4_store(ctypes.byref(cache), slots, count, k, k_stride, v, v_stride, angles,
+                                            rotated, layout, q, q_stride, q_out, q_out_stride, heads, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_kv4_store returned {status}")
+
+    def kv4_load(self, cache: Kv4, slots: int, count: int, k: int, k_stride: int, v: int, v_stride: int,
+                 stream: int) -> None:
+        """Cache rows back as fp32."""
+        status = self.lib.nya_hip_kv4_load(ctypes.byref(cache), slots, count, k, k_stride, v, v_stride, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_kv4_load returned {status}")
+
+    def kv4_attention_bytes(self, cache: Kv4, count: int, requests: int, max_tokens: int, max_length: int, heads: int,
+                            window: int) -> int:
+        """The workspace with which kv4_attention splits the work as it wants to."""
+        b = _sz()
+        if self.lib.nya_hip_kv4_attention_bytes(ctypes.byref(cache), count, requests, max_tokens, max_length, heads,
+                                                window, ctypes.byref(b)):
+            raise ValueError("request unsupported")
+        return b.value
+
+    def kv4_attention(self, cache: Kv4, q: int, q_stride: int, out: int, out_stride: int, count: int, starts: int,
+                      lengths: int, table: int, table_stride: int, requests: int, max_tokens: int, max_length: int,
+                      heads: int, window: int, scale: float, workspace: int, workspace_bytes: int,
+                      stream: int) -> None:
+        """Causal attention of a step's rows over their requests' pages."""
+        status = self.lib.nya_hip_kv4_attention(ctypes.byref(cache), q, q_stride, out, out_stride, count, starts,
+                                                lengths, table, table_stride, requests, max_tokens, max_length, heads,
+                                                window, scale, workspace, workspace_bytes, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_kv4_attention returned {status}")
+
+    # ---- answers (include/fyodor_hip_logprobs.h) -----------------------------
+
+    def logprobs_bytes(self, n: int, count: int, top: int) -> int:
+        """The workspace with which logprobs splits the rows as it wants to."""
+        b = _sz()
+        if self.lib.nya_hip_logprobs_bytes(n, count, top, ctypes.byref(b)):
+            raise ValueError("request unsupported")
+        return b.value
+
+    def logprobs(self, logits: int, stride: int, n: int, count: int, mask: int, scale: float, tokens: int,
+                 logprobs: int, ranks: int, entropies: int, top: int, top_ids: int, top_logprobs: int, workspace: int,
+                 workspace_bytes: int, stream: int) -> None:
+        """Of rows of logits: given tokens' log probabilities and ranks, entropies, the `top` most likely tokens."""
+        status = self.lib.nya_hip_logprobs(logits, stride, n, count, mask, scale, tokens, logprobs, ranks, entropies,
+                                           top, top_ids, top_logprobs, workspace, workspace_bytes, stream)
+        if status != 0:
+            raise HipError(f"nya_hip_logprobs returned {status}")
 
 
 class Graph:
