@@ -1,88 +1,788 @@
 // Causal attention over a paged 4-bit cache (include/fyodor_hip_kv4.h).
+//
+// For a KV head, its group's heads and the request's new tokens make the rows
+// of one product: row i is token i / group, head i % group of the group,
+//     s_it = q_i . K_t scale,   out_i = sum_t e^(s_it) V_t / sum_t e^(s_it).
+// One pass over the positions, 64 a step: S^T = K Q^T and O^T = V^T P^T on the
+// fp16 matrix cores, with the softmax's running maximum and sum (fp32, like S
+// and O) per column, so that a column of S^T is already laid out as the operand
+// P^T. A code times its step of 8 bits is an fp16 number, so keys and values
+// enter exactly; q and P go in as two fp16 pieces each (22 bits, the error of
+// fp32 sums of this length; one piece would be 2^-11), which makes two matrix
+// instructions of one: half the fp16 rate is this kernel's ceiling. The maximum
+// is rounded up to a whole power of two: rescaling by it is exact, and rare.
+// From 2^22 on (kFar) the scores are rounded first, and their distances from the
+// maximum taken after.
+//
+// A call of few rows reads each position once, 1.125 W bytes per KV head and
+// position, and is bound by that and by the conversion: 13 instructions for a
+// word of 8 codes, against 8 for 8 bytes of the 8-bit cache. One of many rows is
+// bound by the matrix cores and by the softmax beside them. Hence two kernels, a
+// workgroup of 16 rows that converts straight into the operands' lanes (kv4_rows),
+// and one of 128 rows that convert each code once, in LDS (kv4_wide). What is
+// too few tiles for the chip is split over the positions and joined by a second
+// launch (kv4_join).
 #include "paged_attention.h"
 
 namespace fy {
 namespace {
 
-// Workgroup (token and head, request) of one wavefront: a lane scores every
-// 64th position and has every 64th element of the output.
-template <int W>
-__global__ __launch_bounds__(64) void kv4_simple(Kv4Attention a)
+constexpr int kBlock = 32;   // elements that share a step
+
+// The four nibbles i of a word's halves' bytes as codes from -8 to 7: under the exponent of
+// 1024 the low nibbles of a half, under that of 64 the high ones, are that plus n.
+__device__ __forceinline__ half2 low_codes(uint32_t w)
 {
+    const half2 bias = {(_Float16)1032.f, (_Float16)1032.f};
+    return __builtin_bit_cast(half2, (w & 0x000F000Fu) | 0x64006400u) - bias;
+}
+__device__ __forceinline__ half2 high_codes(uint32_t w)
+{
+    const half2 bias = {(_Float16)72.f, (_Float16)72.f};
+    return __builtin_bit_cast(half2, (w & 0x00F000F0u) | 0x54005400u) - bias;
+}
+
+// 8 elements of a key.
+__device__ __forceinline__ half8 key_word(uint32_t w, _Float16 step)
+{
+    const half2 s = {step, step};
+    union { half8 v; half2 p[4]; } u;
+    u.p[0] = low_codes(w) * s;
+    u.p[1] = high_codes(w) * s;
+    u.p[2] = low_codes(w >> 8) * s;
+    u.p[3] = high_codes(w >> 8) * s;
+    return u.v;
+}
+
+// 8 positions of 4 elements of the values: a word of codes, and of steps, has two positions.
+__device__ __forceinline__ void value_words(const uint4 &w, const uint4 &steps, half8 *x)
+{
+    union { half8 v; half2 p[4]; } u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t n = word_of(w, i);
+        const half2 s = __builtin_bit_cast(half2, word_of(steps, i));
+        u[0].p[i] = low_codes(n) * s;
+        u[1].p[i] = high_codes(n) * s;
+        u[2].p[i] = low_codes(n >> 8) * s;
+        u[3].p[i] = high_codes(n >> 8) * s;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = u[e].v;
+}
+
+// Steps of the first `limit` of 8 positions, 0 for the others: what memory holds there
+// may be NaN, and a weight of 0 would not hide it.
+__device__ __forceinline__ uint4 first_steps(const uint4 &s, int limit)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = limit > 2 * i + 1 ? word_of(s, i) : limit > 2 * i ? word_of(s, i) & 0xFFFFu : 0u;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Requests of a few rows: 16 rows per workgroup, whose wavefronts take every
+// fourth step of its share of the positions and meet in LDS at the end. Keys
+// and values go from memory straight into the operands' lanes: K and V of a
+// step are requested as soon as the last step's are used up, pages a step
+// before that.
+template <int W>
+__device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, int sp, int tile, const Split &split,
+    int place, int most_rows, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
+{
+    // A lane has, of 16 positions of a step, 4 elements x U of the values, and of 4 positions B blocks of
+    // the keys (half a block of heads of 64) in J words.
+    constexpr int U = W / 64, D = W / 16, B = W < 128 ? 1 : W / 128, J = W / 32, kBlocks = W / kBlock;
+    constexpr bool kAhead = W <= 256;   // room for a step's K and V in registers
     const Kv4 &c = a.cache;
-    const int r = blockIdx.y, token = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x;
-    const int group = a.heads / c.kv_heads, kvh = head / group;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, part = lane >> 4;
+    const int group = a.heads / c.kv_heads;
     const Request rq = request_of(a, r);
-    if (token >= rq.rows / group) return;
-    __shared__ float q[W];
-    for (int d = lane; d < W; d += 64) q[d] = a.q[(rq.begin + token) * a.q_stride + (int64_t)head * W + d];
-    __syncthreads();
-    const int64_t p = rq.first + token, limit = min((int64_t)a.table_stride * c.page_tokens - 1, (int64_t)INT32_MAX - 128);
-    const int last = (int)(p < 0 ? -1 : min(p, limit));
-    const int first = (int)(a.window && p >= a.window ? min(p - a.window + 1, limit + 1) : 0);
-    float m = -INFINITY, l = 0.f, o[W / 64] = {};
-    bool saw = false;
-    for (int at = first; at <= last; at += 64) {
-        const int pos = at + lane, page = pos <= last ? a.table[(size_t)r * a.table_stride + pos / c.page_tokens] : -1;
-        const bool there = (unsigned)page < (unsigned)c.pages;
-        const int t = pos & (c.page_tokens - 1);
-        const size_t place = (size_t)(there ? page : 0) * c.kv_heads + kvh;
-        const uint8_t *keys = c.keys + place * (c.page_tokens * (W / 2));
-        const uint16_t *steps = c.key_steps + place * (c.page_tokens * (W / 32));
-        float s = 0.f;
-        for (int b = 0; b < W / 32; ++b) {
-            float sum = 0.f;
-            for (int w = 0; w < 4; ++w) {
-                const uint32_t word = *(const uint32_t *)(keys + (b * c.page_tokens + t) * 16 + 4 * w);
-                for (int e = 0; e < 8; ++e)
-                    sum += q[32 * b + 8 * w + e] * (float)((int)(word >> (e % 2 * 16 + e / 2 * 4) & 15u) - 8);
-            }
-            s += sum * f16_to_f32(steps[(t / 16 * (W / 32) + b) * 16 + t % 4 * 4 + t % 16 / 4]);
+    if (kRows * tile >= rq.rows || rq.rows > most_rows) return;
+    const Range g = range_of(a, rq, tile, kRows, split.most, split.least);
+    if (sp >= g.active) return;
+
+    // Rows past the request's last repeat it and are not written.
+    const int row = min(kRows * tile + col, rq.rows - 1), token = row / group, head = kvh * group + row % group;
+    const int64_t p = rq.first + token;
+    const int last = (int)(p < g.highest ? p : g.highest);
+    const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
+    // Positions that all rows see: up to the first row's last, from the last row's first.
+    const int64_t p0 = rq.first + kRows * tile / group, p1 = rq.first + min(kRows * tile + kRows - 1, rq.rows - 1) / group;
+    const int all_to = (int)(p0 < g.highest ? p0 : g.highest);
+    const int all_from = (int)(a.window && p1 >= a.window ? (p1 - a.window < g.highest ? p1 - a.window + 1 : g.highest + 1) : 0);
+
+    const int *table = a.table + (size_t)r * a.table_stride;
+    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
+    const int begin = g.from(sp) + wave, stop = g.until(sp);
+    // Lane l reads keys of the granule of 16 positions (l % 16) / 4 of a step and
+    // holds scores and values of granule l / 16. Everything is read
+    // unconditionally (positions past the last one lead to page 0).
+    auto entry_of = [&](int at) {
+        const int entry = table[min(at >> shift, a.table_stride - 1)];
+        return at <= g.highest ? entry : -1;
+    };
+    auto place_of = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + kvh; };
+    const size_t plane = (size_t)c.page_tokens * (W / 2), steps = (size_t)c.page_tokens * kBlocks;
+    int kpage, vpage;
+    auto look = [&](int step) {
+        kpage = entry_of(kStep * step + 16 * (col >> 2));
+        vpage = entry_of(kStep * step + 16 * part);
+    };
+    // (Half a block each of two lanes in heads of 64.)
+    const int block = W == 64 ? part >> 1 : part;
+    typedef uint32_t words __attribute__((ext_vector_type(W == 64 ? 2 : 4)));
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    words kr[4][B];
+    half4 ks[B];
+    uint4 vr[2][U], vs[2][U];
+    bool there;
+    auto fetch_k = [&](int step) {
+        const int at = kStep * step + 16 * (col >> 2);
+        const size_t page = place_of(kpage);
+        const uint8_t *kb = c.keys + page * plane + (block * c.page_tokens + (at & within) + (col & 3)) * 16 +
+                            (W == 64 ? 8 * (part & 1) : 0);
+        const uint16_t *sb = c.key_steps + page * steps + (((at & within) >> 4) * kBlocks + block) * 16 + 4 * (col & 3);
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            ks[b] = *(const half4 *)(sb + 64 * b);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) kr[t][b] = *(const words *)(kb + (size_t)64 * c.page_tokens * b + 64 * t);
         }
-        saw |= there;
-        s = there ? s * a.scale : -INFINITY;
-        const float top = fmaxf(m, wave_reduce<true>(s)), base = top == -INFINITY ? 0.f : top;
-        const float alpha = expf(m - base), e = expf(s - base);
-        m = top;
-        l = l * alpha + e;
-        for (int i = 0; i < W / 64; ++i) o[i] *= alpha;
-        for (int j = 0; j < 64 && at + j <= last; ++j) {
-            const int pg = __builtin_amdgcn_readlane(page, j);
-            if ((unsigned)pg >= (unsigned)c.pages) continue;
-            const float w = lane_value(e, j);
-            const int tj = (at + j) & (c.page_tokens - 1);
-            const size_t pl = (size_t)pg * c.kv_heads + kvh;
-            for (int i = 0; i < W / 64; ++i) {
-                const int d = 64 * i + lane;
-                const uint32_t n = *(const uint16_t *)(c.values + pl * (c.page_tokens * (W / 2)) + ((tj / 8 * (W / 4) + d / 4) * 8 + tj % 8) * 2);
-                o[i] += w * (float)((int)(n >> (4 * (d % 4)) & 15u) - 8) *
-                        f16_to_f32(c.value_steps[pl * (c.page_tokens * (W / 32)) + d / 32 * c.page_tokens + tj]);
+    };
+    const uint8_t *vb;
+    const uint16_t *wb;
+    auto value_codes = [&](int n, int u) { return *(const uint4 *)(vb + ((W / 4) * n + 16 * u) * 16); };
+    auto value_steps = [&](int n, int u) { return *(const uint4 *)(wb + 2 * u * c.page_tokens + 8 * n); };
+    auto fetch_v = [&](int step) {
+        const int at = kStep * step + 16 * part;
+        const size_t page = place_of(vpage);
+        vb = c.values + page * plane + (((at & within) >> 3) * (W / 4) + col) * 16;
+        wb = c.value_steps + page * steps + (col >> 3) * c.page_tokens + (at & within);
+        there = (unsigned)vpage < (unsigned)c.pages;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    vr[n][u] = value_codes(n, u);
+                    vs[n][u] = value_steps(n, u);
+                }
+        }
+    };
+    look(begin);
+
+    // The row's q in two pieces, scaled by a power of two; the scale's sign goes with it. Word j's
+    // elements are 8 j.. of a lane's block (of its half block).
+    half8 qh[J], ql[J];
+    float qscale;
+    {
+        const float *q = a.q + (rq.begin + token) * a.q_stride + (int64_t)head * W + (W == 64 ? 16 : kBlock) * part;
+        auto place_in = [](int i) { return W == 64 ? 4 * i : 128 * (i / 8) + 4 * (i % 8); };
+        float v[8 * J];
+        if (((uintptr_t)a.q & 15) == 0 && a.q_stride % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < 2 * J; ++i) *(float4 *)(v + 4 * i) = *(const float4 *)(q + place_in(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * J; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * i + e] = q[place_in(i) + e];
+        }
+        if constexpr (kAhead) {
+            fetch_k(begin);
+            fetch_v(begin);
+            look(begin + kWaves);
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8 * J; ++i) top = fmaxf(top, fabsf(v[i]));
+        const int e = 14 - __builtin_amdgcn_frexp_expf(column_max(top));
+#pragma unroll
+        for (int i = 0; i < 8 * J; ++i) v[i] = ldexpf(a.scale < 0.f ? -v[i] : v[i], e);
+#pragma unroll
+        for (int j = 0; j < J; ++j) split_f16(v + 8 * j, qh[j], ql[j]);
+        // exp(s) = exp2(s log2 e), q back to its size; above 0, so that it keeps minus infinity.
+        qscale = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504f, -e), 0x1p-126f);
+    }
+
+    f32x4 O[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) O[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool far = false;
+    uint64_t saw = 0;   // lanes that had a score
+    for (int step = begin; step < stop; step += kWaves) {
+        if constexpr (!kAhead) {
+            fetch_k(step);
+            fetch_v(step);
+            look(step + kWaves);
+        }
+        f32x4 S[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) S[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            half8 k[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) k[t] = key_word(kr[t][j / 4][j % 4], ks[j / 4][t]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], qh[j], S[t], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[j], S[t], 0, 0, 0);
+        }
+        if constexpr (kAhead) fetch_k(step + kWaves);
+        const int at = kStep * step, pos = at + 16 * part;
+        int limit = 16;
+        if (all_from > at || all_to < at + kStep - 1 || __builtin_amdgcn_ballot_w64(!there)) {
+            const int from = there ? max(first - pos, 0) : 16, to = min(last - pos, 15);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) S[i >> 2][i & 3] = i >= from && i <= to ? S[i >> 2][i & 3] : -INFINITY;
+            limit = there ? min(g.highest - pos + 1, 16) : 0;
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) vs[n][u] = first_steps(vs[n][u], limit - 8 * n);
+            }
+        }
+        float best = S[0][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) best = fmaxf(best, S[i >> 2][i & 3]);
+        saw |= __builtin_amdgcn_ballot_w64(best > -INFINITY);
+        const float top = best * qscale;
+        if (__builtin_amdgcn_ballot_w64(top > m)) {
+            const float next = fmaxf(m, ceilf(column_max(top)));
+            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < D; ++d) O[d] *= alpha;
+            far = __builtin_amdgcn_ballot_w64(is_far(m));
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float scale = qscale, add = 15.f - base;
+        if (far) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) S[i >> 2][i & 3] = S[i >> 2][i & 3] * qscale - base;
+            scale = 1.f;
+            add = 15.f;
+        }
+        half8 ph[2], pl[2];
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * n + (i >> 2)][i & 3], scale, add));
+                sum[i & 1] += w[i];
+            }
+            split_f16(w, ph[n], pl[n]);
+        }
+        l += sum[0] + sum[1];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                half8 x[4];
+                if constexpr (kAhead) value_words(vr[n][u], vs[n][u], x);
+                else value_words(value_codes(n, u), first_steps(value_steps(n, u), limit - 8 * n), x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[e], ph[n], O[4 * u + e], 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[e], pl[n], O[4 * u + e], 0, 0, 0);
+            }
+        if constexpr (kAhead) {
+            fetch_v(step + kWaves);
+            look(step + 2 * kWaves);
+        }
+    }
+    l = column_sum(l);
+    if (m == -INFINITY && (saw >> col & 0x0001000100010001u)) m = -FLT_MAX;   // scores, none in fp32
+
+    // The wavefronts' partial softmaxes meet in LDS, 64 columns at a time.
+    if (part == 0) {
+        ml[0][wave][col] = m;
+        ml[1][wave][col] = l;
+    }
+    const int mrow = threadIdx.x >> 4, mcol = 4 * (threadIdx.x & 15);   // this thread's output: 4 columns of a row
+    const int out_row = kRows * tile + mrow;
+    const Share to = split.share(c.kv_heads, place, kvh, split.listed ? mrow : out_row, sp, W);
+    const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        if (i) __syncthreads();
+        // Row 4 part + k of tile 4 i + e is element 64 i + 16 part + 4 k + e.
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            *(f32x4 *)&po[wave][col][16 * part + 4 * k] =
+                (f32x4){O[4 * i][k], O[4 * i + 1][k], O[4 * i + 2][k], O[4 * i + 3][k]};
+        __syncthreads();
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml[0][w][mrow]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(ml[0][w][mrow] - base);
+            total += ml[1][w][mrow] * f;
+            o += *(const f32x4 *)&po[w][mrow][mcol] * f;
+        }
+        if (out_row < rq.rows) {
+            if (g.active > 1) {
+                *(f32x4 *)(to.o + 64 * i + mcol) = o;
+                if (i == 0 && mcol == 0) *to.ml = make_float2(top, total);
+            } else {
+                float *out = a.out + (rq.begin + out_row / group) * a.out_stride +
+                             (int64_t)(kvh * group + out_row % group) * W + 64 * i + mcol;
+                const float inverse = inverse_of(total, top);
+                o = o * inverse;
+                if (aligned) {
+                    *(f32x4 *)out = o;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) out[k] = o[k];
+                }
             }
         }
     }
-    l = wave_sum(l);
-    if (m == -INFINITY && __builtin_amdgcn_ballot_w64(saw)) m = -FLT_MAX;
-    float *out = a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W + lane;
-    for (int i = 0; i < W / 64; ++i) out[64 * i] = o[i] * inverse_of(l, m);
+}
+
+template <int W>
+__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv4_rows(Kv4Attention a, Split split, int most_rows)
+{
+    __shared__ float ml[2][kWaves][kRows];
+    __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
+    TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / a.cache.kv_heads)};
+    int place = at.request, share = split.most - 1 - (int)blockIdx.z;
+    if (split.packed) {
+        const ItemOf it = item_of(a, split, most_rows, at.tile);
+        if (it.request < 0) return;
+        at = {it.request, it.item.tile};
+        place = it.request;
+        share = it.item.share;
+    }
+    if constexpr (W > 256) {   // every request runs here, prompts too
+        if (split.listed) {
+            place = at.tile;
+            at = tile_of<kRows>(a, 0, place);
+            if (at.request < 0) return;
+        }
+    }
+    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, share, at.tile, split, place, most_rows, ml, po);
+}
+
+// Many rows of one request: 32 per wavefront, 128 per group of four
+// wavefronts, which share every step's keys and values, converted to fp16 in
+// LDS once. KS groups take every KS-th step of the same rows and meet at the
+// end. Two groups run half a step apart: while one is in its MFMAs (last
+// step's outputs, this step's scores) the other does its softmax and stages
+// its next codes, so that the matrix cores of a SIMD always have one of its two
+// wavefronts. Heads of 256 fill the registers with one group.
+template <int W, int KS>
+__global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
+void kv4_wide(Kv4Attention a, Split split, int most_rows)
+{
+    constexpr int M = W / 16;       // MFMA steps of a score
+    constexpr int D = W / 32;       // output tiles
+    constexpr int N = W < 128 ? 1 : W / 128;   // 16-byte pieces of K, and of V, per thread and step
+    constexpr int kBlocks = W / kBlock, kBytes = 2 * kStep * W;
+    constexpr int kQuads = W / 4;   // pieces of V per 8 positions
+    __shared__ __align__(16) uint8_t smem[KS][2][kBytes];   // [group][K, V]
+    __shared__ int theres[KS][2][4];                        // whether 16 positions have a page
+    __shared__ float2 smem_ml[4][32];
+    const Kv4 &c = a.cache;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
+    const int ks = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), tid = threadIdx.x & 255;
+    const int col = lane & 31, h = lane >> 5;
+    const int group = a.heads / c.kv_heads;
+    int x = blockIdx.x;
+    const int kvh = x % c.kv_heads;
+    x /= c.kv_heads;
+    const int tiles = gridDim.x / (c.kv_heads * split.most), sp = split.most - 1 - x / tiles;
+    const TileOf at_tile = tile_of<kWideRows>(a, most_rows, x % tiles);
+    const int r = at_tile.request, tile = at_tile.tile;
+    if (r < 0) return;
+    const Request rq = request_of(a, r);
+    const Range g = range_of(a, rq, tile, kWideRows, split.most, split.least);
+    if (sp >= g.active) return;
+
+    const int row = kWideRows * tile + 32 * wave + col, row_in = min(row, rq.rows - 1), token = row_in / group;
+    const int head = kvh * group + row_in % group;
+    const int64_t p = rq.first + token;
+    // (Rows past the request's last repeat it and are not written.)
+    const int last = (int)(p < g.highest ? p : g.highest);
+    const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
+    // Positions that all of the wavefront's rows see.
+    int all_from = first, all_to = last;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        all_from = max(all_from, __shfl_xor(all_from, o, 64));
+        all_to = min(all_to, __shfl_xor(all_to, o, 64));
+    }
+    all_from = __builtin_amdgcn_readfirstlane(all_from);
+    all_to = __builtin_amdgcn_readfirstlane(all_to);
+
+    const int *table = a.table + (size_t)r * a.table_stride;
+    const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
+    // This group's steps: begin, begin + KS, ...
+    const int begin = g.from(sp) + ks, stop = g.until(sp);
+    const int rounds = (stop - (begin - ks) + KS - 1) / KS;   // the same for every group
+    // Table entries are read a round before the codes they lead to, and
+    // everything unconditionally (positions past the last one lead to page 0):
+    // loads under a condition would be waited for where it ends.
+    const int until = min(g.highest, kStep * stop - 1);   // this workgroup's last position
+    auto entry_of = [&](int at) {
+        const int entry = table[min(at >> shift, a.table_stride - 1)];
+        return at <= until ? entry : -1;
+    };
+    auto place_of = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + kvh; };
+    const size_t plane = (size_t)c.page_tokens * (W / 2), steps = (size_t)c.page_tokens * kBlocks;
+    int kpage, vpage[N], spage;
+    // This thread's piece i of K is block wave + 4 i of position `lane` of the
+    // step, of V the elements 4 quad.. of 8 positions. Heads of 64 have half as many:
+    // two of the wavefronts stage those of K, two of V.
+    const int kblock = W < 128 ? wave & 1 : wave, vpiece = W < 128 ? tid & 127 : tid;
+    auto look_k = [&](int step) {
+        kpage = entry_of(kStep * step + (lane & 48));
+        spage = entry_of(kStep * step + 16 * (tid & 3));
+    };
+    auto look_v = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) vpage[i] = entry_of(kStep * step + 8 * ((vpiece + 256 * i) / kQuads));
+    };
+    uint4 kreg[N], vreg[N], vstep[N];
+    _Float16 kstep[N];
+    int vpage_at[N];   // the pages that vreg is of
+    bool sthere;
+    auto fetch_k = [&](int step) {
+        const int t = (kStep * step + lane) & within;
+        const size_t page = place_of(kpage);
+        const uint8_t *kb = c.keys + page * plane + (kblock * c.page_tokens + t) * 16;
+        const uint16_t *sb = c.key_steps + page * steps + ((t >> 4) * kBlocks + kblock) * 16 + (t & 3) * 4 + (t >> 2 & 3);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            kreg[i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i);
+            kstep[i] = __builtin_bit_cast(_Float16, sb[64 * i]);
+        }
+        sthere = (unsigned)spage < (unsigned)c.pages;
+    };
+    auto fetch_v = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = vpiece + 256 * i, quad = piece % kQuads, vat = kStep * step + 8 * (piece / kQuads);
+            const size_t page = place_of(vpage[i]);
+            const int t = vat & within;
+            vpage_at[i] = vpage[i];
+            vreg[i] = *(const uint4 *)(c.values + page * plane + ((t >> 3) * kQuads + quad) * 16);
+            vstep[i] = *(const uint4 *)(c.value_steps + page * steps + (quad >> 3) * c.page_tokens + t);
+        }
+    };
+    uint8_t *const ksm = smem[ks][0], *const vsm = smem[ks][1];
+    auto stage_k = [&](int buffer) {
+        const int t = lane & 31, rho = 8 * ((t & 15) >> 2) + 4 * (t >> 4) + (t & 3);
+        if (W >= 128 || wave < 2) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                uint8_t *to = ksm + (((lane >> 5) * M + 2 * (kblock + 4 * i)) * 64 + rho) * 16;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *(half8 *)(to + 512 * j) = key_word(word_of(kreg[i], j), kstep[i]);
+            }
+        }
+        if (tid < 4) theres[ks][buffer][tid] = sthere;
+    };
+    // Element 4 q + e of 32 is row 8 e + q of its tile, so that the threads of a wavefront write side by side.
+    auto stage_v = [&](int step) {
+        if (W < 128 && wave < 2) return;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int piece = vpiece + 256 * i, quad = piece % kQuads, eighth = piece / kQuads;
+            const int vat = kStep * step + 8 * eighth;
+            const int limit = (unsigned)vpage_at[i] < (unsigned)c.pages ? until - vat + 1 : 0;
+            if (__builtin_amdgcn_ballot_w64(limit < 8)) vstep[i] = first_steps(vstep[i], limit);
+            half8 x[4];
+            value_words(vreg[i], vstep[i], x);
+            uint8_t *to = vsm + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 + 32 * (eighth >> 1 & 1) + (quad & 7)) * 16;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *(half8 *)(to + 128 * e) = x[e];
+        }
+    };
+    look_k(begin);
+    fetch_k(begin);
+    look_v(begin);
+    look_k(begin + KS);
+
+    half8 qh[M], ql[M];
+    float qscale;
+    {
+        const float *q = a.q + (rq.begin + token) * a.q_stride + (int64_t)head * W + 8 * h;
+        const bool aligned = ((uintptr_t)a.q & 15) == 0 && a.q_stride % 4 == 0;
+        float v[8 * M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            if (aligned) {
+                *(float4 *)(v + 8 * i) = *(const float4 *)(q + 16 * i);
+                *(float4 *)(v + 8 * i + 4) = *(const float4 *)(q + 16 * i + 4);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[8 * i + e] = q[16 * i + e];
+            }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8 * M; ++i) top = fmaxf(top, fabsf(v[i]));
+        const int e = 14 - __builtin_amdgcn_frexp_expf(halves_max(top));
+#pragma unroll
+        for (int i = 0; i < 8 * M; ++i) v[i] = ldexpf(a.scale < 0.f ? -v[i] : v[i], e);
+#pragma unroll
+        for (int i = 0; i < M; ++i) split_f16(v + 8 * i, qh[i], ql[i]);
+        // Above 0, so that it keeps minus infinity.
+        qscale = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504f, -e), 0x1p-126f);
+    }
+    f32x16 O[D], S[2];
+#pragma unroll
+    for (int d = 0; d < D; ++d) O[d] = (f32x16){};
+    half8 ph[2][2], pl[2][2];
+    float m = -INFINITY, l = 0.f;
+    bool far = false;
+    uint64_t saw = 0;   // lanes that had a score
+    auto outputs = [&]() {
+        const uint8_t *vs = vsm + 16 * lane;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                half8 v[D];
+#pragma unroll
+                for (int d = 0; d < D; ++d) v[d] = *(const half8 *)(vs + ((t * D + d) * 2 + u) * 1024);
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph[t][u], O[d], 0, 0, 0);
+#pragma unroll
+                for (int d = 0; d < D; ++d)
+                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[t][u], O[d], 0, 0, 0);
+            }
+    };
+    auto scores = [&]() {
+        const uint8_t *kp = ksm + 16 * lane;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) S[t] = (f32x16){};
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            const half8 k0 = *(const half8 *)(kp + j * 1024), k1 = *(const half8 *)(kp + (M + j) * 1024);
+            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[j], S[0], 0, 0, 0);
+            S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[j], S[1], 0, 0, 0);
+            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[j], S[0], 0, 0, 0);
+            S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[j], S[1], 0, 0, 0);
+        }
+    };
+    // Between the MFMAs: softmax of the scores, the last codes into LDS.
+    auto between = [&](int step, int buffer) {
+        stage_v(step);
+        stage_k(buffer ^ 1);
+        const int at = kStep * step;
+        const bool whole = all_from <= at && all_to >= at + kStep - 1;
+        bool there[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) there[t] = theres[ks][buffer][2 * t + h];
+        if (!whole || __builtin_amdgcn_ballot_w64(!there[0] || !there[1])) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int from = max(first - (at + 32 * t + 16 * h), 0), to = min(last - (at + 32 * t + 16 * h), 15);
+                const uint32_t seen = there[t] && from <= to ? (0xFFFFu >> (15 - to)) & (0xFFFFu << from) : 0;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) S[t][n] = seen >> n & 1 ? S[t][n] : -INFINITY;
+            }
+        }
+        float best = S[0][0];
+#pragma unroll
+        for (int n = 1; n < 32; ++n) best = fmaxf(best, S[n >> 4][n & 15]);
+        saw |= __builtin_amdgcn_ballot_w64(best > -INFINITY);
+        const float top = best * qscale;
+        if (__builtin_amdgcn_ballot_w64(top > m)) {
+            const float next = fmaxf(m, ceilf(halves_max(top)));
+            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            m = next;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < D; ++d) O[d] *= alpha;
+            far = __builtin_amdgcn_ballot_w64(is_far(m));
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float scale = qscale, add = 15.f - base;
+        if (far) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int n = 0; n < 32; ++n) S[n >> 4][n & 15] = S[n >> 4][n & 15] * qscale - base;
+            scale = 1.f;
+            add = 15.f;
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < 32; n += 8) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[n >> 4][(n & 15) + i], scale, add));
+                sum[i & 1] += w[i];
+            }
+            split_f16(w, ph[n >> 4][n >> 3 & 1], pl[n >> 4][n >> 3 & 1]);
+        }
+        l += sum[0] + sum[1];
+    };
+    // The next codes set out before the MFMAs and are there after them. A
+    // round past the group's last step is one of positions that are not there.
+    auto ahead = [&](int step) {
+        fetch_k(step + KS);
+        fetch_v(step);
+        look_v(step + KS);
+        look_k(step + 2 * KS);
+    };
+    if (rounds > 0) {
+        stage_k(0);
+        lds_barrier();
+        if (KS == 2 && ks) lds_barrier();   // half a step behind
+        ahead(begin);
+        __builtin_amdgcn_s_setprio(1);
+        scores();
+        __builtin_amdgcn_s_setprio(0);
+        lds_barrier();
+        between(begin, 0);
+        lds_barrier();
+        for (int i = 1; i < rounds; ++i) {
+            ahead(begin + KS * i);
+            __builtin_amdgcn_s_setprio(1);
+            outputs();
+            scores();
+            __builtin_amdgcn_s_setprio(0);
+            lds_barrier();   // this group's tiles are read
+            between(begin + KS * i, i & 1);
+            lds_barrier();   // the next ones are there
+        }
+        outputs();
+        if (KS == 2 && !ks) lds_barrier();
+        __syncthreads();
+    }
+    l = halves_sum(l);
+    if (m == -INFINITY && (saw >> col & 0x0000000100000001u)) m = -FLT_MAX;   // scores, none in fp32
+    if constexpr (KS == 2) {
+        // The second group's rows through LDS, as they lie in its registers.
+        float *po = (float *)&smem[0][0][0] + wave * (16 * D * 64) + lane;
+        static_assert(sizeof(smem) >= 4 * 16 * D * 64 * sizeof(float), "the second group's outputs fit");
+        if (ks) {
+#pragma unroll
+            for (int d = 0; d < D; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) po[(16 * d + i) * 64] = O[d][i];
+            if (h == 0) smem_ml[wave][col] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (ks) return;
+        const float2 other = smem_ml[wave][col];
+        const float top = fmaxf(m, other.x), base = top == -INFINITY ? 0.f : top;
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(other.x - base);
+        m = top;
+        l = l * f0 + other.y * f1;
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[d][i] = O[d][i] * f0 + po[(16 * d + i) * 64] * f1;
+    }
+    // Register 4 e + i of tile d is element 32 d + 16 h + 4 i + e.
+    if (row >= rq.rows) return;
+    if (g.active > 1) {
+        const Share to = split.share(c.kv_heads, x % tiles, kvh, row - kWideRows * tile, sp, W);
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(float4 *)(to.o + 32 * d + 16 * h + 4 * i) =
+                    make_float4(O[d][i], O[d][4 + i], O[d][8 + i], O[d][12 + i]);
+        if (h == 0) *to.ml = make_float2(m, l);
+        return;
+    }
+    float *out = a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W + 16 * h;
+    const float inverse = inverse_of(l, m);
+    const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 o = make_float4(O[d][i] * inverse, O[d][4 + i] * inverse, O[d][8 + i] * inverse,
+                                         O[d][12 + i] * inverse);
+            if (aligned) {
+                *(float4 *)(out + 32 * d + 4 * i) = o;
+            } else {
+                out[32 * d + 4 * i] = o.x;
+                out[32 * d + 4 * i + 1] = o.y;
+                out[32 * d + 4 * i + 2] = o.z;
+                out[32 * d + 4 * i + 3] = o.w;
+            }
+        }
+}
+
+// Both in one launch: `wide_blocks` workgroups of wide tiles, then those of few rows.
+template <int W>
+__global__ __launch_bounds__(256) void kv4_join(Kv4Attention a, Split few, Split wide, int most_rows, int wide_blocks)
+{
+    const int index = blockIdx.x;
+    if (index >= wide_blocks) join_row<W>(a, few, most_rows, index - wide_blocks);
+    else join_wide<W>(a, wide, most_rows, index);
+}
+
+template <int W>
+hipError_t launch_width(const Kv4Attention &a, const Plan &p, hipStream_t s)
+{
+    const unsigned requests = a.requests, kv_heads = a.cache.kv_heads;
+    if (p.any_few) {
+        const bool listed = p.few.listed;
+        const unsigned tiles = listed ? (unsigned)p.few.places : (unsigned)((p.few.tile + kRows - 1) / kRows);
+        const unsigned most = p.few.most, packed = p.few.packed ? tiles * requests * most : 0;
+        hipLaunchKernelGGL((kv4_rows<W>), packed ? dim3(packed * kv_heads) : dim3(tiles * kv_heads, listed ? 1 : requests, most),
+                           dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
+    }
+    int64_t wide_blocks = 0;
+    if constexpr (W <= 256) {
+        if (p.any_wide) {
+            constexpr int KS = W <= 128 ? 2 : 1;
+            const int64_t tiles = p.wide.places;
+            hipLaunchKernelGGL((kv4_wide<W, KS>), dim3((unsigned)(tiles * p.wide.most * kv_heads)), dim3(256 * KS), 0, s, a,
+                               p.wide, p.most_rows);
+            if (p.wide.most > 1) wide_blocks = tiles * kJoinParts * kv_heads;
+        }
+    }
+    const int64_t blocks = wide_blocks + (p.any_few && p.few.most > 1 ? (int64_t)p.few.tile * kv_heads * p.few.places : 0);
+    if (blocks)
+        hipLaunchKernelGGL((kv4_join<W>), dim3((unsigned)blocks), dim3(256), 0, s, a, p.few, p.wide, p.most_rows,
+                           (int)wide_blocks);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t kv4_attention_workspace(const Kv4Attention &)
+size_t kv4_attention_workspace(const Kv4Attention &a)
 {
-    return 0;
+    const Plan p = plan_of(a, nullptr, SIZE_MAX);
+    return (p.few.most > 1 ? p.few.most * share_bytes(a, p.few) : 0) +
+           (p.wide.most > 1 ? p.wide.most * share_bytes(a, p.wide) : 0);
 }
 
-hipError_t launch_kv4_attention(const Kv4Attention &a, void *, size_t, hipStream_t s)
+hipError_t launch_kv4_attention(const Kv4Attention &a, void *workspace, size_t workspace_bytes, hipStream_t s)
 {
-    const dim3 grid((unsigned)((int64_t)a.max_tokens * a.heads), a.requests);
+    const Plan p = plan_of(a, (float *)workspace, workspace ? workspace_bytes : 0);
     switch (a.cache.width) {
-    case 64: hipLaunchKernelGGL((kv4_simple<64>), grid, dim3(64), 0, s, a); break;
-    case 128: hipLaunchKernelGGL((kv4_simple<128>), grid, dim3(64), 0, s, a); break;
-    case 256: hipLaunchKernelGGL((kv4_simple<256>), grid, dim3(64), 0, s, a); break;
-    default: hipLaunchKernelGGL((kv4_simple<512>), grid, dim3(64), 0, s, a); break;
+    case 64: return launch_width<64>(a, p, s);
+    case 128: return launch_width<128>(a, p, s);
+    case 256: return launch_width<256>(a, p, s);
+    default: return launch_width<512>(a, p, s);
     }
-    return hipGetLastError();
 }
 
 }  // namespace fy
