@@ -15,8 +15,8 @@ extern "C" {
 #define NYA_HIP_LOGPROBS_TOP 64   /* the most alternatives */
 
 /* Of each of `count` rows of n fp32 logits x (logits + i stride floats), with
- * p_j = e^(scale x_j) / sum_k e^(scale x_k) (scale: 1 / temperature, finite and
- * above 0) over the entries j whose bit in `mask` is clear (uint32 words as
+ * p_j = e^(scale x_j) / sum_k e^(scale x_k) (scale: 1 / temperature, from
+ * 2^-20 to 2^20) over the entries j whose bit in `mask` is clear (uint32 words as
  * nya_hip_greedy's, 0: none masked):
  *   tokens      (or 0) int32 ids: logprobs[i] = ln p of tokens[i], and
  *               ranks[i] (ranks may be 0) how many tokens come before it;

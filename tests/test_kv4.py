@@ -99,7 +99,8 @@ def test_logprobs_refusals(kernels):
     refuse(kernels.lib.nya_hip_logprobs, good,
            [{"logits": 0}, {"logits": A + 2}, {"stride": 998}, {"stride": 1 << 31}, {"n": 0}, {"n": (1 << 24) + 1,
             "stride": 1 << 25}, {"count": 0}, {"count": (1 << 22) + 1}, {"mask": A + 1}, {"scale": 0.0},
-            {"scale": -1.0}, {"scale": math.nan}, {"scale": math.inf}, {"tokens": A + 3}, {"logprobs": 0},
+            {"scale": -1.0}, {"scale": math.nan}, {"scale": math.inf}, {"scale": 0.9 * 2.0 ** -20}, {"scale": 1.1 * 2.0 ** 20},
+            {"tokens": A + 3}, {"logprobs": 0},
             {"logprobs": A + 3 * far + 2}, {"ranks": A + 1}, {"entropies": A + 2}, {"top": 65}, {"top_ids": 0},
             {"top_logprobs": 0}, {"top_ids": A + 1}, {"top_logprobs": A + 3}, {"workspace": A + 8},
             {"tokens": 0, "entropies": 0, "top": 0},
