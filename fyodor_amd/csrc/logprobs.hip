@@ -9,13 +9,18 @@
 // token's ln p is -ln(1 + s), which 1 + s in fp32 would leave without its last
 // bits.
 //
-// The most likely tokens are a sorted list in LDS. A tile has at least `top`
-// logits not below the top-th largest of 64 maxima of its parts, and few more
-// (24 of 20 in random order): those, or the ones above the list's last, are put
-// in order by counting, each against all.
+// The pass keeps the maximum of every group of 32 logits as well. The top-th
+// largest of 256 maxima (of groups together) is not above the top-th logit,
+// and only the groups that reach it, about as many as are asked for, are read
+// again: a list of little more than `top` tokens is put in order by counting,
+// each against all. (Choosing in every tile as it passes cost nearly as much as the
+// pass: 64 rows of 128256 17 us with 20 alternatives, 10 without.)
 //
-// Bound by reading the logits for many rows; a few rows are split into shares,
-// which a second launch joins.
+// Bound by reading the logits for many rows (2047 of 50257 without alternatives
+// 77 us, 5.4 TB/s; with 20 of them 106). A few rows are split into shares,
+// which a second launch joins (64 of 128256: 11 us, 8 for the join; 1 of 32000: 3.9 and
+// 5.3): chains of waits, of which the join has five: the shares, the maxima again,
+// the logits, two turns in LDS.
 #include <float.h>
 #include <limits.h>
 #include <math.h>
@@ -38,7 +43,7 @@ struct Part {
     int rank;
     double count, s, t;
 };
-static_assert(sizeof(Part) % 16 == 0, "lists follow");
+static_assert(sizeof(Part) % 16 == 0, "maxima follow");
 
 // Order of tokens: the larger logit, of equal ones (zeros of both signs among
 // them) the lower id. 0 is no token.
@@ -52,31 +57,79 @@ __device__ __forceinline__ uint64_t key_of(float x, int id) { return (uint64_t)o
 __device__ __forceinline__ float logit_of(uint64_t key) { return of_order((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-// The first float above x, or below it (of 0 the one below both zeros); finite ones.
-__device__ __forceinline__ float above(float x) { return of_order(ordered(x) + 1); }
+// The first float below x (of 0 the one below both zeros); finite ones.
 __device__ __forceinline__ float below(float x)
 {
     const uint32_t o = ordered(x) - 1;
     return of_order(o == 0x7FFFFFFFu ? o - 1 : o);   // (0x7FFFFFFF is -0)
 }
 
-// A workgroup's list, in front of what may join it.
-template <int T> struct List {
-    static constexpr int kRoom = T + kMostTop > 1024 ? T + kMostTop : 1024;
-    uint64_t keys[kRoom], next[kMostTop];
-    float maxima[T];
-    unsigned n;
+// The sums by a maximum m, added to those by another that is not below it.
+__device__ __forceinline__ void add_to(Part &p, float m, double count, double s, double t, float c)
+{
+    const float d = m - p.m, f = m == p.m ? 1.f : __builtin_amdgcn_exp2f(d * c);
+    if (m == p.m) {
+        p.count += count;
+        p.s += s;
+        p.t += t;
+    } else {
+        p.s += (s + count) * f;
+        if (f != 0.f) p.t += (t + (s + count) * d) * f;
+    }
+}
+
+__device__ __forceinline__ bool is_masked(const Logprobs &a, int id) { return a.mask && (a.mask[id >> 5] >> (id & 31) & 1u); }
+
+// A token's place in the order; 0 where it has none.
+__device__ __forceinline__ uint64_t key_in(const Logprobs &a, int row, int id)
+{
+    const float x = a.logits[row * a.stride + id];
+    return x >= -FLT_MAX && !is_masked(a, id) ? key_of(x, id) : 0;
+}
+
+constexpr int kThreads = 256;
+constexpr int kV = 2;                    // 4 kV logits of a thread in a tile (four: 2047 rows of 50257 79 us, two 77)
+constexpr int kTile = 4 * kThreads * kV;
+constexpr int kRoom = 1024 + kMostTop;   // a list, and what may join it before it is put in order
+constexpr int kListed = 512;             // groups that are read again, by number
+
+struct List {
+    __align__(16) uint64_t keys[kRoom];
+    uint64_t next[kMostTop];
+    float maxima[kThreads];
+    int groups[kListed];
+    unsigned n, listed;
 };
 
-// Puts keys[0 .. n) in order and keeps the first `top`; how many there are.
-template <int T>
-__device__ int settle(List<T> &list, int top)
+// Puts keys[0 .. n) in order, each against all, and keeps the first `top`; how many there are.
+__device__ int settle(List &list, int top)
 {
-    const int n = min(list.n, (unsigned)List<T>::kRoom), held = min(n, top);
-    for (int i = threadIdx.x; i < n; i += T) {
+    const int n = list.n, held = min(n, top), lane = threadIdx.x & 63;
+    if (n <= 64) {
+        // One wavefront, the keys in its lanes.
+        if (threadIdx.x < 64) {
+            const uint64_t key = lane < n ? list.keys[lane] : 0;
+            int rank = 0;
+            for (int j = 0; j < n; j += 4)
+#pragma unroll
+                for (int i = j; i < j + 4; ++i) {   // (0 past the last)
+                    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)key, i),
+                                   hi = __builtin_amdgcn_readlane((int)(uint32_t)(key >> 32), i);
+                    rank += ((uint64_t)hi << 32 | lo) > key;
+                }
+            if (lane < n && rank < top) list.keys[rank] = key;
+            if (lane == 0) list.n = held;
+        }
+        __syncthreads();
+        return held;
+    }
+    for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t key = list.keys[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += list.keys[j] > key;
+        int rank = 0, j = 0;
+        for (; j + 8 <= n; j += 8)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) rank += list.keys[j + k] > key;
+        for (; j < n; ++j) rank += list.keys[j] > key;
         if (rank < top) list.next[rank] = key;
     }
     __syncthreads();
@@ -86,100 +139,132 @@ __device__ int settle(List<T> &list, int top)
     return held;
 }
 
-// N tokens of each thread into the list (held of them so far); `most`: the thread's largest
-// logit. In order: none of them comes before one in the list of the same logit.
-template <int T, int N, class X, class Id>
-__device__ __forceinline__ int join_list(List<T> &list, int held, int top, float most, const X &x, const Id &id)
+// A bound that at least `top` of the 256 maxima reach and not many more, by halving the range
+// between the least and the largest, in their order as whole numbers.
+__device__ __forceinline__ float bound_of(const List &list, int top)
 {
-    const int tid = threadIdx.x, lane = tid & 63;
-    float from;
-    if (held == top) {
-        from = above(logit_of(list.keys[top - 1]));
-        if (!__syncthreads_or(most >= from)) return held;
-    } else {
-        list.maxima[tid] = most;
-        __syncthreads();
-        float u = list.maxima[lane];
+    const int lane = threadIdx.x & 63;
+    uint32_t u[4];
+    float low, high;
 #pragma unroll
-        for (int w = 1; w < T / 64; ++w) u = fmaxf(u, list.maxima[64 * w + lane]);
-        // Distinct by the lane, in place of the last bits: rounded down, it still bounds them.
-        const uint32_t o = (ordered(u) & ~63u) | lane;
-        int rank = 0;
-#pragma unroll 16
-        for (int j = 0; j < 64; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)o, j) > o;
-        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == top - 1));
-        // Minus infinity is no token.
-        from = fmaxf(of_order((uint32_t)__builtin_amdgcn_readlane((int)o, at) & ~63u), -FLT_MAX);
+    for (int i = 0; i < 4; ++i) {
+        const float v = list.maxima[64 * i + lane];
+        u[i] = ordered(v);
+        low = i ? fminf(low, v) : v;
+        high = i ? fmaxf(high, v) : v;
     }
-    if (most >= from) {
-        int mine = 0;
+    // Minus infinity is no token.
+    uint32_t from = ordered(fmaxf(-wave_reduce<true>(-low), -FLT_MAX)), to = ordered(wave_reduce<true>(high));
+    for (int k = 0; k < 24 && to > from + 1; ++k) {
+        const uint32_t middle = from + (to - from) / 2;
+        int reach = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) mine += x(i) >= from;
-        unsigned at = atomicAdd(&list.n, (unsigned)mine);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (x(i) >= from) {
-                if (at < (unsigned)List<T>::kRoom) list.keys[at] = key_of(x(i), id(i));
-                ++at;
-            }
+        for (int i = 0; i < 4; ++i) reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(u[i] >= middle));
+        if (reach < top) {
+            to = middle;
+        } else {
+            from = middle;
+            if (reach <= top + 2) break;
+        }
     }
+    return of_order(__builtin_amdgcn_readfirstlane((int)from));
+}
+
+// How a row is read: `shares` of `sets` x `per_set` tiles. A set's group g of 64
+// has the 16 logits from 16 g on of each 1024.
+struct Reading {
+    int shares, sets, per_set;
+    __host__ __device__ int each() const { return sets * per_set; }
+};
+
+// The first `top` tokens of a row, in order, from its groups' maxima (`groups`, a multiple of 64,
+// in the order of shares and sets); how many there are.
+__device__ __forceinline__ int choose(const Logprobs &a, int row, int shift, const Reading &r, const float *maxima,
+    int groups, List &list)
+{
+    const int tid = threadIdx.x, top = a.top;
+    if (tid == 0) list.n = list.listed = 0;
+    float most = -INFINITY;
+#pragma unroll 4
+    for (int g = 4 * tid; g < groups; g += 4 * kThreads) {
+        const float4 q = *(const float4 *)(maxima + g);
+        most = fmaxf(fmaxf(most, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
+    }
+    list.maxima[tid] = most;
     __syncthreads();
-    if (list.n <= (unsigned)List<T>::kRoom) return settle(list, top);
-    // More than there is room for (many equal or ascending logits): a token of each thread at a time.
-    __syncthreads();
-    if (tid == 0) list.n = held;
-    __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {
-        float v = 0.f;
-        int k = 0;
+    const float from = bound_of(list, top);
+    if (most >= from)
+        for (int g = 4 * tid; g < groups; g += 4 * kThreads) {
+            const float4 q = *(const float4 *)(maxima + g);
+            const float four[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j == i) {
-                v = x(j);
-                k = id(j);
-            }
-        const uint64_t key = key_of(v, k);
-        if (v >= -FLT_MAX && (held < top || key > list.keys[top - 1])) list.keys[atomicAdd(&list.n, 1u)] = key;
+            for (int e = 0; e < 4; ++e)
+                if (four[e] >= from) {
+                    const unsigned at = atomicAdd(&list.listed, 1u);
+                    if (at < (unsigned)kListed) list.groups[at] = g + e;
+                }
+        }
+    __syncthreads();
+    // (More groups than are listed, of many equal logits: all of them are gone through.)
+    const bool all = list.listed > (unsigned)kListed;
+    const unsigned size = 16 * kV * r.per_set, n = (all ? groups : list.listed) * size;   // at most a row
+    int held = 0;
+    for (unsigned at = 0; at < n; at += 4 * kThreads) {
+        uint64_t key[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned e = at + i * kThreads + tid;
+            key[i] = 0;
+            if (e >= n) continue;
+            const unsigned k = e / size, j = e % size, g = all ? k : list.groups[k];
+            if (all && maxima[g] < from) continue;
+            const int id = (int)(((g / 64 * r.per_set) * kV + j / 16) * 1024 + 16 * (g % 64) + j % 16) - shift;
+            if (id >= 0 && id < a.n) key[i] = key_in(a, row, id);
+        }
+        const uint64_t bar = held == top ? list.keys[top - 1] + 1 : key_of(from, 0x7FFFFFFF);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (key[i] >= bar) list.keys[atomicAdd(&list.n, 1u)] = key[i];
         __syncthreads();
-        held = settle(list, top);
+        const unsigned now = list.n;
+        __syncthreads();   // read by all before the next ones join
+        if (at + 4 * kThreads >= n || now > (unsigned)(kRoom - 4 * kThreads)) held = settle(list, top);
     }
     return held;
 }
 
 // What the threads know, together, in all of them. c: scale in powers of two.
-template <int T>
-__device__ __forceinline__ Part together(const Part &p, float c)
+__device__ __forceinline__ Part together(float m, float count, float s, float t, int rank, float c)
 {
-    __shared__ double sums[4][T / 64];
-    __shared__ float tops[T / 64];
+    __shared__ float sums[3][kThreads / 64], tops[kThreads / 64];
+    __shared__ int ranks[kThreads / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float top = wave_reduce<true>(p.m);
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    Part all = {tops[0], 0, 0, 0, 0};
-#pragma unroll
-    for (int w = 1; w < T / 64; ++w) all.m = fmaxf(all.m, tops[w]);
-    const float d = p.m - all.m, f = p.m == all.m ? 1.f : __builtin_amdgcn_exp2f(d * c);
-    const bool most = p.m == all.m;
-    const double count = wave_sum(most ? p.count : 0.0), s = wave_sum(p.s * f + (most ? 0.0 : p.count * f)),
-                 t = wave_sum(f == 0.f ? 0.0 : most ? p.t : (p.t + (p.count + p.s) * d) * f), rank = wave_sum((double)p.rank);
+    // A wavefront's sums by its own maximum. (Whole numbers up to 2^24 are exact.)
+    const float top = wave_reduce<true>(m), d = m - top;
+    const bool most = m == top;
+    const float f = most ? 1.f : __builtin_amdgcn_exp2f(d * c);
+    t = f == 0.f ? 0.f : most ? t : (t + (count + s) * d) * f;
+    s = s * f + (most ? 0.f : count * f);
+    s = wave_sum(s);
+    t = wave_sum(t);
+    count = wave_sum(most ? count : 0.f);
+    rank = (int)wave_sum((float)rank);
     if (lane == 0) {
+        tops[wave] = top;
         sums[0][wave] = count;
         sums[1][wave] = s;
         sums[2][wave] = t;
-        sums[3][wave] = rank;
+        ranks[wave] = rank;
     }
     __syncthreads();
-    double ranks = 0;
+    Part all = {tops[0], 0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < T / 64; ++w) {
-        all.count += sums[0][w];
-        all.s += sums[1][w];
-        all.t += sums[2][w];
-        ranks += sums[3][w];
+    for (int w = 1; w < kThreads / 64; ++w) all.m = fmaxf(all.m, tops[w]);
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        add_to(all, tops[w], sums[0][w], sums[1][w], sums[2][w], c);
+        all.rank += ranks[w];
     }
-    all.rank = (int)ranks;
     return all;
 }
 
@@ -196,19 +281,27 @@ __device__ __forceinline__ Given given_of(const Logprobs &a, int row)
     g.there = (unsigned)g.id < (unsigned)a.n;
     const int id = g.there ? g.id : 0;
     const float x = a.logits[row * a.stride + id];
-    if (g.there && !(a.mask && (a.mask[id >> 5] >> (id & 31) & 1u))) g.x = x;
+    if (g.there && !is_masked(a, id)) g.x = x;
     return g;
 }
 
+// ln S. The exponentials were formed with scale log2 e rounded to fp32, scale (1 + off): to the first order in
+// `off` (at most 2^-23) ln S is larger by off times the mean of scale d.
+__device__ __forceinline__ double log_sum(const Logprobs &a, const Part &p)
+{
+    const float c = a.scale * 1.44269504f;
+    const double off = c / (a.scale * 1.4426950408889634) - 1;
+    return log1p((p.count - 1) + p.s) - off * a.scale * (p.t / (p.count + p.s));
+}
+
 // A row's results.
-template <int T>
-__device__ __forceinline__ void finish(const Logprobs &a, int row, const Given &g, const Part &p, const List<T> *list, int held)
+__device__ __forceinline__ void finish(const Logprobs &a, int row, const Given &g, const Part &p, const List *list, int held)
 {
     __shared__ double log_s;
     // NaN leaves a sum NaN; plus infinity is the maximum.
     const bool none = !(p.m > -INFINITY && p.m < INFINITY) || !(p.s >= 0);
     if (threadIdx.x == 0) {
-        log_s = log1p((p.count - 1) + p.s);
+        log_s = log_sum(a, p);
         if (a.tokens) {
             const bool ranked = g.there && !none && g.x > -INFINITY;
             a.logprobs[row] = !g.there ? 0.f : none ? NAN : (float)(((double)g.x - p.m) * a.scale - log_s);
@@ -218,7 +311,7 @@ __device__ __forceinline__ void finish(const Logprobs &a, int row, const Given &
     }
     if (!list) return;
     __syncthreads();
-    for (int k = threadIdx.x; k < a.top; k += T) {
+    for (int k = threadIdx.x; k < a.top; k += kThreads) {
         const uint64_t key = k < held ? list->keys[k] : 0;
         const size_t at = (size_t)row * a.top + k;
         a.top_ids[at] = none || !key ? -1 : id_of(key);
@@ -226,38 +319,42 @@ __device__ __forceinline__ void finish(const Logprobs &a, int row, const Given &
     }
 }
 
-// Workgroup (row, share of its tiles) of T threads, V times 4 logits each a tile.
-// Positions begin at the 16 bytes that the row begins in.
-template <int T, int V, bool kTop>
-__global__ __launch_bounds__(T) void logprobs_rows(Logprobs a, int shares, int tiles_each, Part *parts, uint64_t *lists)
+constexpr int kWholeGroups = 4096;   // the most of a row that is one share
+
+// Workgroup (row, share), 4 kV logits a thread and tile. Positions begin at the 16
+// bytes that the row begins in. kWhole: the row is one share.
+template <bool kTop, bool kWhole>
+__global__ __launch_bounds__(kThreads) void logprobs_rows(Logprobs a, Reading r, Part *parts, float *all_maxima)
 {
-    __shared__ List<kTop ? T : 64> list;
-    constexpr int kTile = 4 * T * V;
-    const int row = blockIdx.x / shares, share = blockIdx.x % shares, tid = threadIdx.x;
+    __shared__ __align__(16) float maxima[kTop && kWhole ? kWholeGroups : 4];
+    const int row = kWhole ? blockIdx.x : blockIdx.x / r.shares, share = kWhole ? 0 : blockIdx.x % r.shares, tid = threadIdx.x;
     const float *x0 = a.logits + row * a.stride;
     const int shift = (int)((uintptr_t)x0 >> 2 & 3), end = a.n + shift;
     x0 -= shift;
-    const int from = share * tiles_each * kTile, to = min(end, from + tiles_each * kTile);
+    float *to_maxima = kWhole ? maxima : all_maxima + (size_t)blockIdx.x * r.sets * 64;
     const Given g = given_of(a, row);
     const float c = a.scale * 1.44269504f;
-    Part p = {-INFINITY, 0, 0, 0, 0};
-    float s = 0.f, t = 0.f;
-    int count = 0, held = 0;
-    if (kTop) {
-        if (tid == 0) list.n = 0;
-        __syncthreads();
-    }
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    int count = 0, rank = 0;
+    float highest = -INFINITY;
+    int set = 0, in_set = 0;
+    // A set's maxima, of four threads each.
+    auto put = [&]() {
+        highest = fmaxf(highest, row_lane<0xB1>(highest));
+        highest = fmaxf(highest, row_lane<0x4E>(highest));
+        if (tid % 4 == 0) to_maxima[set * 64 + tid / 4] = highest;
+        highest = -INFINITY;
+        in_set = 0;
+        ++set;
+    };
+    const int from = share * r.each() * kTile, to = min(end, from + r.each() * kTile);
     for (int tile = from; tile < to; tile += kTile) {
-        float x[4 * V];
+        float x[4 * kV];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int at = tile + 4 * (T * v + tid);
+        for (int v = 0; v < kV; ++v) {
+            const int at = tile + 4 * (kThreads * v + tid);
             if (at >= shift && at + 3 < end) {
-                const float4 q = *(const float4 *)(x0 + at);
-                x[4 * v] = q.x;
-                x[4 * v + 1] = q.y;
-                x[4 * v + 2] = q.z;
-                x[4 * v + 3] = q.w;
+                *(float4 *)(x + 4 * v) = *(const float4 *)(x0 + at);
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[4 * v + e] = at + e >= shift && at + e < end ? x0[at + e] : -INFINITY;
@@ -265,8 +362,8 @@ __global__ __launch_bounds__(T) void logprobs_rows(Logprobs a, int shares, int t
         }
         if (a.mask) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int id = tile + 4 * (T * v + tid) - shift;
+            for (int v = 0; v < kV; ++v) {
+                const int id = tile + 4 * (kThreads * v + tid) - shift;
                 const int last = (a.n - 1) >> 5, first = max(id, 0) >> 5;
                 const uint64_t both = (uint64_t)a.mask[min(max(id + 3, 0) >> 5, last)] << 32 | a.mask[min(first, last)];
                 // (Of one word twice, the low one has the bits.)
@@ -279,115 +376,108 @@ __global__ __launch_bounds__(T) void logprobs_rows(Logprobs a, int shares, int t
         }
         float most = x[0];
 #pragma unroll
-        for (int i = 1; i < 4 * V; ++i) most = fmaxf(most, x[i]);
-        if (most > p.m) {
+        for (int i = 1; i < 4 * kV; ++i) most = fmaxf(most, x[i]);
+        highest = fmaxf(highest, most);
+        if (most > m) {
             // (The thread's first tile: there is nothing to rescale.)
-            const float d = p.m - most, f = __builtin_amdgcn_exp2f(d * c);
+            const float d = m - most, f = __builtin_amdgcn_exp2f(d * c);
             t = f == 0.f ? 0.f : (t + ((float)count + s) * d) * f;
             s = s * f + (float)count * f;
             count = 0;
-            p.m = most;
+            m = most;
         }
-        const float m = p.m == -INFINITY ? 0.f : p.m;
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < 4 * V; ++i) {
-            const float d = x[i] - m, e = __builtin_amdgcn_exp2f(d * c);
-            const bool at_most = x[i] == m;
+        for (int i = 0; i < 4 * kV; ++i) {
+            // (NaN stays NaN in e, minus infinity is 0 there.)
+            const float d = x[i] - base, low = fmaxf(d, -FLT_MAX);
+            const float e = __builtin_amdgcn_exp2f(d * c);
+            const bool at_most = x[i] == base;
             count += at_most;
             s += at_most ? 0.f : e;
-            t = __builtin_fmaf(fmaxf(d, -FLT_MAX), e, t);
+            t = __builtin_fmaf(low, e, t);
         }
         // Which logits come before the given one goes by the id where they are equal.
         if (g.there) {
             const int id = tile - shift;
             if (g.id >= id && g.id < id + kTile) {
 #pragma unroll
-                for (int i = 0; i < 4 * V; ++i) {
-                    const int mine = id + 4 * (T * (i / 4) + tid) + i % 4;
-                    p.rank += x[i] > g.x || (x[i] == g.x && mine < g.id);
+                for (int i = 0; i < 4 * kV; ++i) {
+                    const int mine = id + 4 * (kThreads * (i / 4) + tid) + i % 4;
+                    rank += x[i] > g.x || (x[i] == g.x && mine < g.id);
                 }
             } else {
                 const float bar = g.id < id || !(g.x > -INFINITY) ? g.x : below(g.x);
 #pragma unroll
-                for (int i = 0; i < 4 * V; ++i) p.rank += x[i] > bar;
+                for (int i = 0; i < 4 * kV; ++i) rank += x[i] > bar;
             }
         }
         if constexpr (kTop)
-            held = join_list<T, 4 * V>(list, held, a.top, most, [&](int i) { return x[i]; },
-                                       [&](int i) { return tile - shift + 4 * (T * (i / 4) + tid) + i % 4; });
+            if (++in_set == r.per_set) put();
     }
-    p.count = count;
-    p.s = s;
-    p.t = t;
-    p = together<T>(p, c);
-    if (shares == 1) {
-        if constexpr (kTop) finish<T>(a, row, g, p, &list, held);
-        else finish<T>(a, row, g, p, nullptr, 0);
-        return;
-    }
-    if (tid == 0) parts[blockIdx.x] = p;
     if constexpr (kTop)
-        for (int k = tid; k < a.top; k += T) lists[(size_t)blockIdx.x * a.top + k] = k < held ? list.keys[k] : 0;
+        while (set < r.sets) put();
+    const Part p = together(m, (float)count, s, t, rank, c);
+    if constexpr (!kWhole) {
+        if (tid == 0) parts[blockIdx.x] = p;
+    } else if constexpr (kTop) {
+        __shared__ List list;
+        const int held = choose(a, row, shift, r, maxima, r.sets * 64, list);
+        finish(a, row, g, p, &list, held);
+    } else {
+        finish(a, row, g, p, nullptr, 0);
+    }
 }
 
 // Workgroup: a row, from its shares.
 template <bool kTop>
-__global__ __launch_bounds__(256) void logprobs_join(Logprobs a, int shares, const Part *parts, const uint64_t *lists)
+__global__ __launch_bounds__(kThreads) void logprobs_join(Logprobs a, Reading r, const Part *parts, const float *all_maxima)
 {
-    __shared__ List<kTop ? 256 : 64> list;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const Given g = given_of(a, row);
+    __shared__ Part all;
+    const int row = blockIdx.x, tid = threadIdx.x, groups = r.shares * r.sets * 64;
     Part p = {-INFINITY, 0, 0, 0, 0};
-    if (tid < shares) p = parts[(size_t)row * shares + tid];
-    int held = 0;
-    if constexpr (kTop) {
-        if (tid == 0) list.n = 0;
-        __syncthreads();
-        constexpr int kEach = 4;
-        const int n = shares * a.top;
-        lists += (size_t)row * n;
-        // Share after share, so that of equal logits the lower ids come first.
-        for (int at = 0; at < n; at += 256 * kEach) {
-            uint64_t key[kEach];
-            float most = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int k = at + 256 * i + tid;
-                key[i] = k < n ? lists[k] : 0;
-                if (!key[i]) key[i] = key_of(-INFINITY, 0);
-                most = fmaxf(most, logit_of(key[i]));
-            }
-            held = join_list<256, kEach>(list, held, a.top, most, [&](int i) { return logit_of(key[i]); },
-                                         [&](int i) { return id_of(key[i]); });
-        }
+    if (tid < r.shares) p = parts[(size_t)row * r.shares + tid];
+    const Given g = given_of(a, row);
+    const float c = a.scale * 1.44269504f;
+    // The shares' sums, in the first wavefront.
+    if (tid < 64) {
+        Part q = {wave_reduce<true>(p.m), 0, 0, 0, 0};
+        add_to(q, p.m, p.count, p.s, p.t, c);
+        q.count = wave_sum(q.count);
+        q.s = wave_sum(q.s);
+        q.t = wave_sum(q.t);
+        q.rank = (int)wave_sum((float)p.rank);
+        if (tid == 0) all = q;
     }
-    p = together<256>(p, a.scale * 1.44269504f);
-    if constexpr (kTop) finish<256>(a, row, g, p, &list, held);
-    else finish<256>(a, row, g, p, nullptr, 0);
+    __syncthreads();
+    if constexpr (kTop) {
+        __shared__ List list;
+        const int shift = (int)((uintptr_t)(a.logits + row * a.stride) >> 2 & 3);
+        const int held = choose(a, row, shift, r, all_maxima + (size_t)row * groups, groups, list);
+        finish(a, row, g, all, &list, held);
+    } else {
+        finish(a, row, g, all, nullptr, 0);
+    }
 }
 
-// How a call's rows are read: `threads` per workgroup, a row's tiles in `shares` of `each`.
-struct Reading {
-    int threads, shares, each;
-};
-
-constexpr int kFew = 1024, kFewTile = 4 * kFew * 8, kManyTile = 4 * 256 * 4;
+size_t share_bytes(const Reading &r, int top) { return sizeof(Part) + (top ? (size_t)r.sets * 64 * sizeof(float) : 0); }
 
 Reading reading_of(int n, int count, int top, size_t bytes)
 {
-    const int span = n + 3;   // a row may begin 3 floats into its 16 bytes
-    const auto tiles = [&](int tile) { return (span + tile - 1) / tile; };
-    // Rows of two large tiles: what a second launch costs is more.
-    if (count <= 256 && tiles(kFewTile) <= 2) return {kFew, 1, tiles(kFewTile)};
-    const int all = tiles(kManyTile);
-    int shares = count >= 1024 ? 1 : (2048 + count - 1) / count;
+    const int all = (n + 3 + kTile - 1) / kTile;   // a row may begin 3 floats into its 16 bytes
+    // Four workgroups for each CU: 64 rows of 128256, 8, 16 and 32 shares 13.0, 10.6 and 11.5 us, the join 8;
+    // from 1024 rows on, whole ones (2047 of 50257 77 us, in 4 shares 85 and 5 for the join).
+    int shares = count >= 1024 ? 1 : (1024 + count - 1) / count;
     shares = shares < kMostShares ? shares : kMostShares;
-    const size_t each = (sizeof(Part) + sizeof(uint64_t) * top) * count;
-    if (bytes / each < (size_t)shares) shares = (int)(bytes / each);
-    if (shares > all) shares = all;
-    if (shares < 2) return {256, 1, all};
-    const int tiles_each = (all + shares - 1) / shares;
-    return {256, (all + tiles_each - 1) / tiles_each, tiles_each};
+    for (;; --shares) {
+        if (shares > all) shares = all;
+        if (shares < 1) shares = 1;
+        // Tiles of a share, in sets so that a row has at most 64 of them, and one for each share.
+        const int each = (all + shares - 1) / shares, per_set = (each * shares + 63) / 64;
+        Reading r = {shares, (each + per_set - 1) / per_set, per_set};
+        r.shares = (all + r.each() - 1) / r.each();
+        if (r.shares == 1 || share_bytes(r, top) * r.shares * count <= bytes) return r;
+    }
 }
 
 }  // namespace
@@ -395,25 +485,26 @@ Reading reading_of(int n, int count, int top, size_t bytes)
 size_t logprobs_workspace(int n, int count, int top)
 {
     const Reading r = reading_of(n, count, top, SIZE_MAX);
-    return r.shares == 1 ? 0 : (sizeof(Part) + sizeof(uint64_t) * top) * count * r.shares;
+    return r.shares == 1 ? 0 : share_bytes(r, top) * r.shares * count;
 }
 
 hipError_t launch_logprobs(const Logprobs &a, void *workspace, size_t workspace_bytes, hipStream_t s)
 {
     const Reading r = reading_of(a.n, a.count, a.top, workspace ? workspace_bytes : 0);
     Part *parts = (Part *)workspace;
-    uint64_t *lists = (uint64_t *)(parts + (size_t)a.count * r.shares);
-    const dim3 grid((unsigned)((int64_t)a.count * r.shares));
-    if (r.threads == kFew) {
-        if (a.top) hipLaunchKernelGGL((logprobs_rows<kFew, 8, true>), grid, dim3(kFew), 0, s, a, 1, r.each, parts, lists);
-        else hipLaunchKernelGGL((logprobs_rows<kFew, 8, false>), grid, dim3(kFew), 0, s, a, 1, r.each, parts, lists);
+    float *maxima = (float *)(parts + (size_t)a.count * r.shares);
+    const dim3 grid((unsigned)((int64_t)a.count * r.shares)), threads(kThreads);
+    if (r.shares == 1) {
+        if (a.top) hipLaunchKernelGGL((logprobs_rows<true, true>), grid, threads, 0, s, a, r, parts, maxima);
+        else hipLaunchKernelGGL((logprobs_rows<false, true>), grid, threads, 0, s, a, r, parts, maxima);
         return hipGetLastError();
     }
-    if (a.top) hipLaunchKernelGGL((logprobs_rows<256, 4, true>), grid, dim3(256), 0, s, a, r.shares, r.each, parts, lists);
-    else hipLaunchKernelGGL((logprobs_rows<256, 4, false>), grid, dim3(256), 0, s, a, r.shares, r.each, parts, lists);
-    if (r.shares > 1) {
-        if (a.top) hipLaunchKernelGGL((logprobs_join<true>), dim3(a.count), dim3(256), 0, s, a, r.shares, parts, lists);
-        else hipLaunchKernelGGL((logprobs_join<false>), dim3(a.count), dim3(256), 0, s, a, r.shares, parts, lists);
+    if (a.top) {
+        hipLaunchKernelGGL((logprobs_rows<true, false>), grid, threads, 0, s, a, r, parts, maxima);
+        hipLaunchKernelGGL((logprobs_join<true>), dim3(a.count), threads, 0, s, a, r, parts, maxima);
+    } else {
+        hipLaunchKernelGGL((logprobs_rows<false, false>), grid, threads, 0, s, a, r, parts, maxima);
+        hipLaunchKernelGGL((logprobs_join<false>), dim3(a.count), threads, 0, s, a, r, parts, maxima);
     }
     return hipGetLastError();
 }
