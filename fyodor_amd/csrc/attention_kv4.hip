@@ -29,46 +29,70 @@ namespace {
 
 constexpr int kBlock = 32;   // elements that share a step
 
-// The four nibbles i of a word's halves' bytes as codes from -8 to 7: under the exponent of
-// 1024 the low nibbles of a half, under that of 64 the high ones, are that plus n.
-__device__ __forceinline__ half2 low_codes(uint32_t w)
-{
-    const half2 bias = {(_Float16)1032.f, (_Float16)1032.f};
-    return __builtin_bit_cast(half2, (w & 0x000F000Fu) | 0x64006400u) - bias;
-}
-__device__ __forceinline__ half2 high_codes(uint32_t w)
-{
-    const half2 bias = {(_Float16)72.f, (_Float16)72.f};
-    return __builtin_bit_cast(half2, (w & 0x00F000F0u) | 0x54005400u) - bias;
-}
+// Nibbles of a word's halves as codes from -8 to 7: under the exponent of 1024 the
+// low nibble of a half, under that of 64 the high one, is that plus n. (The
+// constants are opaque: as literals they would make two instructions of one.)
+struct Codes {
+    uint32_t low = 0x000F000Fu, high = 0x00F000F0u, low_one = 0x64006400u, high_one = 0x54005400u;
+    __device__ __forceinline__ Codes() { asm("" : "+s"(low), "+s"(high), "+v"(low_one), "+v"(high_one)); }
+    __device__ __forceinline__ half2 lows(uint32_t w) const
+    {
+        return __builtin_bit_cast(half2, (w & low) | low_one) - (half2){(_Float16)1032.f, (_Float16)1032.f};
+    }
+    __device__ __forceinline__ half2 highs(uint32_t w) const
+    {
+        return __builtin_bit_cast(half2, (w & high) | high_one) - (half2){(_Float16)72.f, (_Float16)72.f};
+    }
+};
 
 // 8 elements of a key.
-__device__ __forceinline__ half8 key_word(uint32_t w, _Float16 step)
+__device__ __forceinline__ half8 key_word(const Codes &c, uint32_t w, _Float16 step)
 {
     const half2 s = {step, step};
     union { half8 v; half2 p[4]; } u;
-    u.p[0] = low_codes(w) * s;
-    u.p[1] = high_codes(w) * s;
-    u.p[2] = low_codes(w >> 8) * s;
-    u.p[3] = high_codes(w >> 8) * s;
+    u.p[0] = c.lows(w) * s;
+    u.p[1] = c.highs(w) * s;
+    u.p[2] = c.lows(w >> 8) * s;
+    u.p[3] = c.highs(w >> 8) * s;
     return u.v;
 }
 
 // 8 positions of 4 elements of the values: a word of codes, and of steps, has two positions.
-__device__ __forceinline__ void value_words(const uint4 &w, const uint4 &steps, half8 *x)
+__device__ __forceinline__ void value_words(const Codes &c, const uint4 &w, const uint4 &steps, half8 *x)
 {
     union { half8 v; half2 p[4]; } u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t n = word_of(w, i);
         const half2 s = __builtin_bit_cast(half2, word_of(steps, i));
-        u[0].p[i] = low_codes(n) * s;
-        u[1].p[i] = high_codes(n) * s;
-        u[2].p[i] = low_codes(n >> 8) * s;
-        u[3].p[i] = high_codes(n >> 8) * s;
+        u[0].p[i] = c.lows(n) * s;
+        u[1].p[i] = c.highs(n) * s;
+        u[2].p[i] = c.lows(n >> 8) * s;
+        u[3].p[i] = c.highs(n >> 8) * s;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = u[e].v;
+}
+
+// One of x's two pieces: hi (second 0), or lo (-1).
+__device__ __forceinline__ half8 piece_f16(const float *x, float second)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    union { half8 v; half2 p[4]; } u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x2 v = {x[2 * i], x[2 * i + 1]};
+        const half2 h = __builtin_convertvector(v, half2);
+        const f32x2 r = {__builtin_fmaf((float)h.x, second, v.x), __builtin_fmaf((float)h.y, second, v.y)};
+        u.p[i] = __builtin_convertvector(r, half2);
+    }
+    return u.v;
+}
+
+// The value of the lane eight on (of eight back) in a row of 16, part of the addition that uses it.
+__device__ __forceinline__ float eight_on(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true));
 }
 
 // Steps of the first `limit` of 8 positions, 0 for the others: what memory holds there
@@ -86,26 +110,25 @@ __device__ __forceinline__ uint4 first_steps(const uint4 &s, int limit)
 // fourth step of its share of the positions and meet in LDS at the end. Keys
 // and values go from memory straight into the operands' lanes: K and V of a
 // step are requested as soon as the last step's are used up, pages a step
-// before that.
-template <int W>
-__device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, int sp, int tile, const Split &split,
-    int place, int most_rows, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
+// before that. Steps [from, until) of the tile's; a `shared` tile's rows go to
+// `to`, `stride` places apart.
+template <int W, bool kPair>
+__device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Request &rq, const Range &g, int kvh, int tile,
+    int from, int until, bool shared, const Share &to, int stride, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
 {
     // A lane has, of 16 positions of a step, 4 elements x U of the values, and of 4 positions B blocks of
     // the keys (half a block of heads of 64) in J words.
     constexpr int U = W / 64, D = W / 16, B = W < 128 ? 1 : W / 128, J = W / 32, kBlocks = W / kBlock;
     constexpr bool kAhead = W <= 256;   // room for a step's K and V in registers
     const Kv4 &c = a.cache;
+    const Codes codes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, part = lane >> 4;
+    const float second = kPair && col & 8 ? -1.f : 0.f;
     const int group = a.heads / c.kv_heads;
-    const Request rq = request_of(a, r);
-    if (kRows * tile >= rq.rows || rq.rows > most_rows) return;
-    const Range g = range_of(a, rq, tile, kRows, split.most, split.least);
-    if (sp >= g.active) return;
 
     // Rows past the request's last repeat it and are not written.
-    const int row = min(kRows * tile + col, rq.rows - 1), token = row / group, head = kvh * group + row % group;
+    const int row = min(kRows * tile + (kPair ? col & 7 : col), rq.rows - 1), token = row / group, head = kvh * group + row % group;
     const int64_t p = rq.first + token;
     const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
@@ -116,21 +139,22 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
 
     const int *table = a.table + (size_t)r * a.table_stride;
     const int shift = 31 - __builtin_clz(c.page_tokens), within = c.page_tokens - 1;
-    const int begin = g.from(sp) + wave, stop = g.until(sp);
+    const int begin = from + wave, stop = until;
     // Lane l reads keys of the granule of 16 positions (l % 16) / 4 of a step and
     // holds scores and values of granule l / 16. Everything is read
-    // unconditionally (positions past the last one lead to page 0).
+    // unconditionally (positions past these steps' lead to page 0).
+    const int most = min(g.highest, kStep * stop - 1);
     auto entry_of = [&](int at) {
         const int entry = table[min(at >> shift, a.table_stride - 1)];
-        return at <= g.highest ? entry : -1;
+        return at <= most ? entry : -1;
     };
-    auto place_of = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + kvh; };
-    const size_t plane = (size_t)c.page_tokens * (W / 2), steps = (size_t)c.page_tokens * kBlocks;
-    int kpage, vpage;
-    auto look = [&](int step) {
-        kpage = entry_of(kStep * step + 16 * (col >> 2));
-        vpage = entry_of(kStep * step + 16 * part);
-    };
+    // A page's codes and steps of this head: whole pages of 32 bits of bytes from the first one's.
+    const unsigned plane = c.page_tokens * (W / 2), steps = c.page_tokens * kBlocks;
+    const unsigned page_codes = c.kv_heads * plane, page_steps = 2 * c.kv_heads * steps;
+    const uint8_t *keys = c.keys + (size_t)kvh * plane, *values = c.values + (size_t)kvh * plane;
+    const uint8_t *key_steps = (const uint8_t *)(c.key_steps + (size_t)kvh * steps),
+                  *value_step = (const uint8_t *)(c.value_steps + (size_t)kvh * steps);
+    auto page_of = [&](int page) { return (unsigned)page < (unsigned)c.pages ? (unsigned)page : 0u; };
     // (Half a block each of two lanes in heads of 64.)
     const int block = W == 64 ? part >> 1 : part;
     typedef uint32_t words __attribute__((ext_vector_type(W == 64 ? 2 : 4)));
@@ -138,13 +162,21 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
     words kr[4][B];
     half4 ks[B];
     uint4 vr[2][U], vs[2][U];
+    int kpage, vpage;
     bool there;
+    const uint8_t *vb;
+    const uint16_t *wb;
+    auto look = [&](int step) {
+        kpage = entry_of(kStep * step + 16 * (col >> 2));
+        vpage = entry_of(kStep * step + 16 * part);
+    };
     auto fetch_k = [&](int step) {
         const int at = kStep * step + 16 * (col >> 2);
-        const size_t page = place_of(kpage);
-        const uint8_t *kb = c.keys + page * plane + (block * c.page_tokens + (at & within) + (col & 3)) * 16 +
+        const unsigned page = page_of(kpage);
+        const uint8_t *kb = keys + (uint64_t)page * page_codes + (block * c.page_tokens + (at & within) + (col & 3)) * 16 +
                             (W == 64 ? 8 * (part & 1) : 0);
-        const uint16_t *sb = c.key_steps + page * steps + (((at & within) >> 4) * kBlocks + block) * 16 + 4 * (col & 3);
+        const uint16_t *sb = (const uint16_t *)(key_steps + (uint64_t)page * page_steps) +
+                             (((at & within) >> 4) * kBlocks + block) * 16 + 4 * (col & 3);
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             ks[b] = *(const half4 *)(sb + 64 * b);
@@ -152,15 +184,13 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
             for (int t = 0; t < 4; ++t) kr[t][b] = *(const words *)(kb + (size_t)64 * c.page_tokens * b + 64 * t);
         }
     };
-    const uint8_t *vb;
-    const uint16_t *wb;
     auto value_codes = [&](int n, int u) { return *(const uint4 *)(vb + ((W / 4) * n + 16 * u) * 16); };
     auto value_steps = [&](int n, int u) { return *(const uint4 *)(wb + 2 * u * c.page_tokens + 8 * n); };
     auto fetch_v = [&](int step) {
         const int at = kStep * step + 16 * part;
-        const size_t page = place_of(vpage);
-        vb = c.values + page * plane + (((at & within) >> 3) * (W / 4) + col) * 16;
-        wb = c.value_steps + page * steps + (col >> 3) * c.page_tokens + (at & within);
+        const unsigned page = page_of(vpage);
+        vb = values + (uint64_t)page * page_codes + (((at & within) >> 3) * (W / 4) + col) * 16;
+        wb = (const uint16_t *)(value_step + (uint64_t)page * page_steps) + (col >> 3) * c.page_tokens + (at & within);
         there = (unsigned)vpage < (unsigned)c.pages;
         if constexpr (kAhead) {
 #pragma unroll
@@ -176,7 +206,7 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
 
     // The row's q in two pieces, scaled by a power of two; the scale's sign goes with it. Word j's
     // elements are 8 j.. of a lane's block (of its half block).
-    half8 qh[J], ql[J];
+    half8 qh[J], ql[kPair ? 1 : J];
     float qscale;
     {
         const float *q = a.q + (rq.begin + token) * a.q_stride + (int64_t)head * W + (W == 64 ? 16 : kBlock) * part;
@@ -203,7 +233,10 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
 #pragma unroll
         for (int i = 0; i < 8 * J; ++i) v[i] = ldexpf(a.scale < 0.f ? -v[i] : v[i], e);
 #pragma unroll
-        for (int j = 0; j < J; ++j) split_f16(v + 8 * j, qh[j], ql[j]);
+        for (int j = 0; j < J; ++j) {
+            if constexpr (kPair) qh[j] = piece_f16(v + 8 * j, second);
+            else split_f16(v + 8 * j, qh[j], ql[j]);
+        }
         // exp(s) = exp2(s log2 e), q back to its size; above 0, so that it keeps minus infinity.
         qscale = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504f, -e), 0x1p-126f);
     }
@@ -227,11 +260,18 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
         for (int j = 0; j < J; ++j) {
             half8 k[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) k[t] = key_word(kr[t][j / 4][j % 4], ks[j / 4][t]);
+            for (int t = 0; t < 4; ++t) k[t] = key_word(codes, kr[t][j / 4][j % 4], ks[j / 4][t]);
 #pragma unroll
             for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], qh[j], S[t], 0, 0, 0);
+            if constexpr (!kPair) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[j], S[t], 0, 0, 0);
+                for (int t = 0; t < 4; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t], ql[j], S[t], 0, 0, 0);
+            }
+        }
+        if constexpr (kPair) {
+            // The other piece's score is eight columns on.
+#pragma unroll
+            for (int i = 0; i < 16; ++i) S[i >> 2][i & 3] += eight_on(S[i >> 2][i & 3]);
         }
         if constexpr (kAhead) fetch_k(step + kWaves);
         const int at = kStep * step, pos = at + 16 * part;
@@ -271,7 +311,7 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
             scale = 1.f;
             add = 15.f;
         }
-        half8 ph[2], pl[2];
+        half8 ph[2], pl[kPair ? 1 : 2];
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -281,22 +321,25 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
                 w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[2 * n + (i >> 2)][i & 3], scale, add));
                 sum[i & 1] += w[i];
             }
-            split_f16(w, ph[n], pl[n]);
+            if constexpr (kPair) ph[n] = piece_f16(w, second);
+            else split_f16(w, ph[n], pl[n]);
         }
         l += sum[0] + sum[1];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                half8 x[4];
-                if constexpr (kAhead) value_words(vr[n][u], vs[n][u], x);
-                else value_words(value_codes(n, u), first_steps(value_steps(n, u), limit - 8 * n), x);
+                half8 v[4];
+                if constexpr (kAhead) value_words(codes, vr[n][u], vs[n][u], v);
+                else value_words(codes, value_codes(n, u), first_steps(value_steps(n, u), limit - 8 * n), v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[e], ph[n], O[4 * u + e], 0, 0, 0);
+                    O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[e], ph[n], O[4 * u + e], 0, 0, 0);
+                if constexpr (!kPair) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[e], pl[n], O[4 * u + e], 0, 0, 0);
+                    for (int e = 0; e < 4; ++e)
+                        O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[e], pl[n], O[4 * u + e], 0, 0, 0);
+                }
             }
         if constexpr (kAhead) {
             fetch_v(step + kWaves);
@@ -306,14 +349,17 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
     l = column_sum(l);
     if (m == -INFINITY && (saw >> col & 0x0001000100010001u)) m = -FLT_MAX;   // scores, none in fp32
 
-    // The wavefronts' partial softmaxes meet in LDS, 64 columns at a time.
-    if (part == 0) {
-        ml[0][wave][col] = m;
-        ml[1][wave][col] = l;
+    // The wavefronts' partial softmaxes meet in LDS, 64 columns at a time. (The thread's number is opaque: what
+    // follows from it would be formed before the loops and live through them.)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int my_wave = tid >> 6, my_col = tid & 15, my_part = tid >> 4 & 3;
+    if (my_part == 0) {
+        ml[0][my_wave][my_col] = m;
+        ml[1][my_wave][my_col] = l;
     }
-    const int mrow = threadIdx.x >> 4, mcol = 4 * (threadIdx.x & 15);   // this thread's output: 4 columns of a row
+    const int mrow = tid >> 4, mcol = 4 * my_col;   // this thread's output: 4 columns of a row
     const int out_row = kRows * tile + mrow;
-    const Share to = split.share(c.kv_heads, place, kvh, split.listed ? mrow : out_row, sp, W);
     const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -321,7 +367,7 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
         // Row 4 part + k of tile 4 i + e is element 64 i + 16 part + 4 k + e.
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            *(f32x4 *)&po[wave][col][16 * part + 4 * k] =
+            *(f32x4 *)&po[my_wave][my_col][16 * my_part + 4 * k] =
                 (f32x4){O[4 * i][k], O[4 * i + 1][k], O[4 * i + 2][k], O[4 * i + 3][k]};
         __syncthreads();
         float top = -INFINITY, total = 0.f;
@@ -334,11 +380,12 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
             const float f = __builtin_amdgcn_exp2f(ml[0][w][mrow] - base);
             total += ml[1][w][mrow] * f;
             o += *(const f32x4 *)&po[w][mrow][mcol] * f;
+            if constexpr (kPair) o += *(const f32x4 *)&po[w][mrow ^ 8][mcol] * f;
         }
-        if (out_row < rq.rows) {
-            if (g.active > 1) {
-                *(f32x4 *)(to.o + 64 * i + mcol) = o;
-                if (i == 0 && mcol == 0) *to.ml = make_float2(top, total);
+        if (out_row < rq.rows && (!kPair || mrow < 8)) {
+            if (shared) {
+                *(f32x4 *)(to.o + (size_t)mrow * stride * W + 64 * i + mcol) = o;
+                if (i == 0 && mcol == 0) to.ml[mrow * stride] = make_float2(top, total);
             } else {
                 float *out = a.out + (rq.begin + out_row / group) * a.out_stride +
                              (int64_t)(kvh * group + out_row % group) * W + 64 * i + mcol;
@@ -355,19 +402,23 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, int kvh, 
     }
 }
 
-template <int W>
-__global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv4_rows(Kv4Attention a, Split split, int most_rows)
+// Wavefronts of few rows on a SIMD, and so their workgroups on a CU: what their registers leave.
+constexpr int waves_of(int width, bool pair) { return width == 64 ? (pair ? 4 : 3) : width == 128 ? (pair ? 3 : 2) : 1; }
+
+template <int W, bool kPair>
+__global__ __launch_bounds__(64 * kWaves, waves_of(W, kPair)) void kv4_rows(Kv4Attention a, Split split, int most_rows)
 {
     __shared__ float ml[2][kWaves][kRows];
     __shared__ __align__(16) float po[kWaves][kRows][64 + 4];
-    TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / a.cache.kv_heads)};
-    int place = at.request, share = split.most - 1 - (int)blockIdx.z;
+    const int kv_heads = a.cache.kv_heads, kvh = blockIdx.x % kv_heads;
+    TileOf at = {(int)blockIdx.y, (int)(blockIdx.x / kv_heads)};
+    int place = at.request, sp = split.most - 1 - (int)blockIdx.z;
     if (split.packed) {
         const ItemOf it = item_of(a, split, most_rows, at.tile);
         if (it.request < 0) return;
         at = {it.request, it.item.tile};
         place = it.request;
-        share = it.item.share;
+        sp = it.item.share;
     }
     if constexpr (W > 256) {   // every request runs here, prompts too
         if (split.listed) {
@@ -376,7 +427,12 @@ __global__ __launch_bounds__(64 * kWaves, W <= 128 ? 2 : 1) void kv4_rows(Kv4Att
             if (at.request < 0) return;
         }
     }
-    few_rows<W>(a, at.request, blockIdx.x % a.cache.kv_heads, share, at.tile, split, place, most_rows, ml, po);
+    const Request rq = request_of(a, at.request);
+    if (kRows * at.tile >= rq.rows || rq.rows > most_rows) return;
+    const Range g = range_of(a, rq, at.tile, kRows, split.most, split.least);
+    if (sp >= g.active) return;
+    const Share to = split.share(kv_heads, place, kvh, split.listed ? 0 : kRows * at.tile, sp, W);
+    few_rows<W, kPair>(a, at.request, rq, g, kvh, at.tile, g.from(sp), g.until(sp), g.active > 1, to, split.most, ml, po);
 }
 
 // Many rows of one request: 32 per wavefront, 128 per group of four
@@ -399,6 +455,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     __shared__ int theres[KS][2][4];                        // whether 16 positions have a page
     __shared__ float2 smem_ml[4][32];
     const Kv4 &c = a.cache;
+    const Codes codes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
     const int ks = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), tid = threadIdx.x & 255;
     const int col = lane & 31, h = lane >> 5;
@@ -493,7 +550,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
             for (int i = 0; i < N; ++i) {
                 uint8_t *to = ksm + (((lane >> 5) * M + 2 * (kblock + 4 * i)) * 64 + rho) * 16;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) *(half8 *)(to + 512 * j) = key_word(word_of(kreg[i], j), kstep[i]);
+                for (int j = 0; j < 4; ++j) *(half8 *)(to + 512 * j) = key_word(codes, word_of(kreg[i], j), kstep[i]);
             }
         }
         if (tid < 4) theres[ks][buffer][tid] = sthere;
@@ -508,7 +565,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
             const int limit = (unsigned)vpage_at[i] < (unsigned)c.pages ? until - vat + 1 : 0;
             if (__builtin_amdgcn_ballot_w64(limit < 8)) vstep[i] = first_steps(vstep[i], limit);
             half8 x[4];
-            value_words(vreg[i], vstep[i], x);
+            value_words(codes, vreg[i], vstep[i], x);
             uint8_t *to = vsm + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 + 32 * (eighth >> 1 & 1) + (quad & 7)) * 16;
 #pragma unroll
             for (int e = 0; e < 4; ++e) *(half8 *)(to + 128 * e) = x[e];
@@ -745,8 +802,10 @@ hipError_t launch_width(const Kv4Attention &a, const Plan &p, hipStream_t s)
         const bool listed = p.few.listed;
         const unsigned tiles = listed ? (unsigned)p.few.places : (unsigned)((p.few.tile + kRows - 1) / kRows);
         const unsigned most = p.few.most, packed = p.few.packed ? tiles * requests * most : 0;
-        hipLaunchKernelGGL((kv4_rows<W>), packed ? dim3(packed * kv_heads) : dim3(tiles * kv_heads, listed ? 1 : requests, most),
-                           dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
+        const dim3 grid = packed ? dim3(packed * kv_heads) : dim3(tiles * kv_heads, listed ? 1 : requests, most);
+        // No request of few rows has more than eight: a column for each piece.
+        if (p.few.tile <= 8) hipLaunchKernelGGL((kv4_rows<W, true>), grid, dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
+        else hipLaunchKernelGGL((kv4_rows<W, false>), grid, dim3(64 * kWaves), 0, s, a, p.few, p.most_rows);
     }
     int64_t wide_blocks = 0;
     if constexpr (W <= 256) {
