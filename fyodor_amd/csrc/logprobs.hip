@@ -98,12 +98,73 @@ struct List {
     uint64_t next[kMostTop];
     float maxima[kThreads];
     int groups[kListed];
+    uint32_t reach[2][kThreads / 64];
     unsigned n, listed;
 };
+
+// Leaves, of more keys than are worth comparing with each other, the ones above a bound that at
+// least `top` of them reach and few more do (all, if they are of one logit): as bound_of, with
+// every thread's keys in registers.
+__device__ void narrow(List &list, int top)
+{
+    constexpr int kEach = (kRoom + kThreads - 1) / kThreads;
+    const int n = list.n, tid = threadIdx.x, wave = tid >> 6;
+    uint64_t key[kEach];
+    uint32_t from = ~0u, to = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int k = tid + i * kThreads;
+        key[i] = k < n ? list.keys[k] : 0;
+        const uint32_t o = (uint32_t)(key[i] >> 32);
+        if (key[i]) from = min(from, o);
+        to = max(to, o);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        from = min(from, (uint32_t)__shfl_xor((int)from, d, 64));
+        to = max(to, (uint32_t)__shfl_xor((int)to, d, 64));
+    }
+    if ((tid & 63) == 0) {
+        list.reach[0][wave] = from;
+        list.reach[1][wave] = to;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        from = min(from, list.reach[0][w]);
+        to = max(to, list.reach[1][w]);
+    }
+    __syncthreads();
+    for (int turn = 0; to > from + 1 && turn < 32; ++turn) {
+        const uint32_t middle = from + (to - from) / 2;
+        int mine = 0, reach = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64((uint32_t)(key[i] >> 32) >= middle));
+        if ((tid & 63) == 0) list.reach[turn & 1][wave] = mine;
+        __syncthreads();   // (the other half is written next: one wait a turn)
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) reach += (int)list.reach[turn & 1][w];
+        if (reach < top) {
+            to = middle;
+        } else {
+            from = middle;
+            if (reach <= top + 8) break;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) list.n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (key[i] && (uint32_t)(key[i] >> 32) >= from) list.keys[atomicAdd(&list.n, 1u)] = key[i];
+    __syncthreads();
+}
 
 // Puts keys[0 .. n) in order, each against all, and keeps the first `top`; how many there are.
 __device__ int settle(List &list, int top)
 {
+    if (list.n > 256 && (int)list.n > top) narrow(list, top);
     const int n = list.n, held = min(n, top), lane = threadIdx.x & 63;
     if (n <= 64) {
         // One wavefront, the keys in its lanes.
@@ -185,25 +246,27 @@ __device__ __forceinline__ int choose(const Logprobs &a, int row, int shift, con
     const int tid = threadIdx.x, top = a.top;
     if (tid == 0) list.n = list.listed = 0;
     float most = -INFINITY;
+    // Four maxima at a time while 256 threads have some each.
+    const int each = groups >= 4 * kThreads ? 4 : 1;
+    if (each == 4) {
 #pragma unroll 4
-    for (int g = 4 * tid; g < groups; g += 4 * kThreads) {
-        const float4 q = *(const float4 *)(maxima + g);
-        most = fmaxf(fmaxf(most, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
+        for (int g = 4 * tid; g < groups; g += 4 * kThreads) {
+            const float4 q = *(const float4 *)(maxima + g);
+            most = fmaxf(fmaxf(most, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
+        }
+    } else {
+        for (int g = tid; g < groups; g += kThreads) most = fmaxf(most, maxima[g]);
     }
     list.maxima[tid] = most;
     __syncthreads();
     const float from = bound_of(list, top);
     if (most >= from)
-        for (int g = 4 * tid; g < groups; g += 4 * kThreads) {
-            const float4 q = *(const float4 *)(maxima + g);
-            const float four[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (four[e] >= from) {
+        for (int g = each * tid; g < groups; g += each * kThreads)
+            for (int e = 0; e < each; ++e)
+                if (maxima[g + e] >= from) {
                     const unsigned at = atomicAdd(&list.listed, 1u);
                     if (at < (unsigned)kListed) list.groups[at] = g + e;
                 }
-        }
     __syncthreads();
     // (More groups than are listed, of many equal logits: all of them are gone through.)
     const bool all = list.listed > (unsigned)kListed;
