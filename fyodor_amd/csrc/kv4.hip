@@ -187,21 +187,21 @@ __global__ __launch_bounds__(256) void kv4_store(Store4 s)
 }
 
 // Workgroup: 256 threads of (row, quad) from number blockIdx.x * 256 on.
+template <int W>
 __global__ __launch_bounds__(256) void kv4_load(Kv4 c, const int *__restrict__ slots, int count, float *__restrict__ k,
     int64_t k_stride, float *__restrict__ v, int64_t v_stride, bool quads)
 {
-    const unsigned per_row = c.kv_heads * c.width / 4;
-    const uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const unsigned per_row = c.kv_heads * W / 4, at = blockIdx.x * 256 + threadIdx.x;
     const int row = (int)(at / per_row);
     if (row >= count) return;
     const int slot = slots[row];
     if ((unsigned)slot >= (unsigned)(c.pages * c.page_tokens)) return;
-    const int t = slot & (c.page_tokens - 1), i = (int)(at % per_row), head = i / (c.width / 4),
-              quad = i % (c.width / 4), b = quad / 8, blocks = c.width / kBlock;
+    const int t = slot & (c.page_tokens - 1), i = (int)(at % per_row), head = i / (W / 4),
+              quad = i % (W / 4), b = quad / 8, blocks = W / kBlock;
     const size_t place = (size_t)(slot / c.page_tokens) * c.kv_heads + head;
-    const size_t codes = place * (c.page_tokens * (c.width / 2)), steps = place * (c.page_tokens * blocks);
+    const size_t codes = place * (c.page_tokens * (W / 2)), steps = place * (c.page_tokens * blocks);
     const uint32_t kw = *(const uint32_t *)(c.keys + codes + (b * c.page_tokens + t) * 16 + (quad % 8 & ~1) * 2) >> (quad & 1 ? 8 : 0);
-    const uint32_t vw = *(const uint16_t *)(c.values + codes + ((t / 8 * (c.width / 4) + quad) * 8 + t % 8) * 2);
+    const uint32_t vw = *(const uint16_t *)(c.values + codes + ((t / 8 * (W / 4) + quad) * 8 + t % 8) * 2);
     const float ks = f16_to_f32(c.key_steps[steps + (t / 16 * blocks + b) * 16 + t % 4 * 4 + t % 16 / 4]);
     const float vs = ks != ks ? ks : f16_to_f32(c.value_steps[steps + b * c.page_tokens + t]);
     float x[4], y[4];
@@ -212,8 +212,9 @@ __global__ __launch_bounds__(256) void kv4_load(Kv4 c, const int *__restrict__ s
     }
     float *to_k = k + row * k_stride + 4 * i, *to_v = v + row * v_stride + 4 * i;
     if (quads) {
-        *(float4 *)to_k = make_float4(x[0], x[1], x[2], x[3]);
-        *(float4 *)to_v = make_float4(y[0], y[1], y[2], y[3]);
+        typedef float f32x4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store((f32x4){x[0], x[1], x[2], x[3]}, (f32x4 *)to_k);
+        __builtin_nontemporal_store((f32x4){y[0], y[1], y[2], y[3]}, (f32x4 *)to_v);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -254,9 +255,22 @@ hipError_t launch_kv4_load(const Kv4 &cache, const int *slots, int count, float 
     int64_t v_stride, hipStream_t s)
 {
     const bool quads = (((uintptr_t)k | (uintptr_t)v) & 15) == 0 && k_stride % 4 == 0 && v_stride % 4 == 0;
-    const int64_t threads = (int64_t)count * cache.kv_heads * (cache.width / 4);
-    hipLaunchKernelGGL(kv4_load, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, cache, slots, count, k,
-                       k_stride, v, v_stride, quads);
+    // Threads are numbered in 32 bits: as many rows in a launch as that allows, nearly always all.
+    const int per_row = cache.kv_heads * (cache.width / 4), most = (1 << 30) / per_row;
+    for (int first = 0; first < count; first += most) {
+        const int rows = count - first < most ? count - first : most;
+        const dim3 grid((unsigned)(((int64_t)rows * per_row + 255) / 256));
+        const auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, cache, slots + first, rows, k + first * k_stride, k_stride,
+                               v + first * v_stride, v_stride, quads);
+        };
+        switch (cache.width) {
+        case 64: launch(kv4_load<64>); break;
+        case 128: launch(kv4_load<128>); break;
+        case 256: launch(kv4_load<256>); break;
+        default: launch(kv4_load<512>); break;
+        }
+    }
     return hipGetLastError();
 }
 
