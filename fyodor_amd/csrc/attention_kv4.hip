@@ -95,14 +95,15 @@ __device__ __forceinline__ float eight_on(float v)
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true));
 }
 
-// Steps of the first `limit` of 8 positions, 0 for the others: what memory holds there
-// may be NaN, and a weight of 0 would not hide it.
-__device__ __forceinline__ uint4 first_steps(const uint4 &s, int limit)
+// Steps of positions from .. limit - 1 of 8, 0 for the others (no row's, past the last or before
+// every window): what memory holds there may be NaN, and a weight of 0 would not hide it.
+__device__ __forceinline__ uint4 some_steps(const uint4 &s, int from, int limit)
 {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        w[i] = limit > 2 * i + 1 ? word_of(s, i) : limit > 2 * i ? word_of(s, i) & 0xFFFFu : 0u;
+        w[i] = word_of(s, i) & ((from <= 2 * i && limit > 2 * i ? 0xFFFFu : 0u) |
+                                (from <= 2 * i + 1 && limit > 2 * i + 1 ? 0xFFFF0000u : 0u));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -275,17 +276,18 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Req
         }
         if constexpr (kAhead) fetch_k(step + kWaves);
         const int at = kStep * step, pos = at + 16 * part;
-        int limit = 16;
+        int low = 0, limit = 16;   // the tile's positions of these 16
         if (all_from > at || all_to < at + kStep - 1 || __builtin_amdgcn_ballot_w64(!there)) {
             const int from = there ? max(first - pos, 0) : 16, to = min(last - pos, 15);
 #pragma unroll
             for (int i = 0; i < 16; ++i) S[i >> 2][i & 3] = i >= from && i <= to ? S[i >> 2][i & 3] : -INFINITY;
+            low = g.lowest - pos;
             limit = there ? min(g.highest - pos + 1, 16) : 0;
             if constexpr (kAhead) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int u = 0; u < U; ++u) vs[n][u] = first_steps(vs[n][u], limit - 8 * n);
+                    for (int u = 0; u < U; ++u) vs[n][u] = some_steps(vs[n][u], low - 8 * n, limit - 8 * n);
             }
         }
         float best = S[0][0];
@@ -331,7 +333,7 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Req
             for (int n = 0; n < 2; ++n) {
                 half8 v[4];
                 if constexpr (kAhead) value_words(codes, vr[n][u], vs[n][u], v);
-                else value_words(codes, value_codes(n, u), first_steps(value_steps(n, u), limit - 8 * n), v);
+                else value_words(codes, value_codes(n, u), some_steps(value_steps(n, u), low - 8 * n, limit - 8 * n), v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     O[4 * u + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[e], ph[n], O[4 * u + e], 0, 0, 0);
@@ -563,7 +565,8 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
             const int piece = vpiece + 256 * i, quad = piece % kQuads, eighth = piece / kQuads;
             const int vat = kStep * step + 8 * eighth;
             const int limit = (unsigned)vpage_at[i] < (unsigned)c.pages ? until - vat + 1 : 0;
-            if (__builtin_amdgcn_ballot_w64(limit < 8)) vstep[i] = first_steps(vstep[i], limit);
+            const int low = g.lowest - vat;
+            if (__builtin_amdgcn_ballot_w64(limit < 8 || low > 0)) vstep[i] = some_steps(vstep[i], low, limit);
             half8 x[4];
             value_words(codes, vreg[i], vstep[i], x);
             uint8_t *to = vsm + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 + 32 * (eighth >> 1 & 1) + (quad & 7)) * 16;

@@ -329,6 +329,25 @@ def test_attention_holes(env, dev, page_tokens, heads, kv_heads, width, lengths,
     assert np.all(got[starts[2]:starts[3]] == 0)
 
 
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 64), (8, 2, 128), (4, 2, 256), (4, 2, 512), (16, 1, 128)])
+@pytest.mark.parametrize("page_tokens", [16, 128])
+@pytest.mark.parametrize("tokens", [1, 3, 90])
+def test_attention_window_unstored(env, dev, heads, kv_heads, width, page_tokens, tokens):
+    """Positions before every row's window were never stored (a program that goes on from a window's worth of
+    positions): what memory holds there, NaN and infinity among it, does not matter."""
+    lengths, counts, window = [300, 171], [tokens, 1], 75
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, page_tokens, 8)
+    for r in range(2):
+        for p in range(lengths[r] - counts[r] - window + 1):
+            at = (table[r, p // page_tokens], slice(None), p % page_tokens)
+            cache.k.steps[at] = np.float16(np.nan)
+            cache.v.steps[at] = np.float16(np.nan if p % 2 else np.inf)
+    cache.put()
+    got = run_attention(env, dev, cache, q, starts, lengths, table, window=window)
+    check_attention(cache, q, got, starts, lengths, table, window=window)
+    assert np.all(np.isfinite(got))
+
+
 @pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 64), (8, 2, 128), (4, 2, 256), (4, 2, 512)])
 @pytest.mark.parametrize("tokens", [1, 4, 80])
 def test_attention_values(env, dev, heads, kv_heads, width, tokens):
