@@ -80,23 +80,17 @@ __device__ __forceinline__ void add_to(Part &p, float m, double count, double s,
 
 __device__ __forceinline__ bool is_masked(const Logprobs &a, int id) { return a.mask && (a.mask[id >> 5] >> (id & 31) & 1u); }
 
-// A token's place in the order; 0 where it has none.
-__device__ __forceinline__ uint64_t key_in(const Logprobs &a, int row, int id)
-{
-    const float x = a.logits[row * a.stride + id];
-    return x >= -FLT_MAX && !is_masked(a, id) ? key_of(x, id) : 0;
-}
-
 constexpr int kThreads = 256;
 constexpr int kV = 2;                    // 4 kV logits of a thread in a tile (four: 2047 rows of 50257 79 us, two 77)
 constexpr int kTile = 4 * kThreads * kV;
 constexpr int kRoom = 1024 + kMostTop;   // a list, and what may join it before it is put in order
 constexpr int kListed = 512;             // groups that are read again, by number
+constexpr int kMostGroups = 64 * 64;     // of a row
 
 struct List {
     __align__(16) uint64_t keys[kRoom];
     uint64_t next[kMostTop];
-    float maxima[kThreads];
+    float maxima[kThreads], bound;
     int groups[kListed];
     uint32_t reach[2][kThreads / 64];
     unsigned n, listed;
@@ -225,7 +219,7 @@ __device__ __forceinline__ float bound_of(const List &list, int top)
             to = middle;
         } else {
             from = middle;
-            if (reach <= top + 2) break;
+            if (reach <= top + 2 + k) break;   // (equal maxima: a few groups more, not every turn)
         }
     }
     return of_order(__builtin_amdgcn_readfirstlane((int)from));
@@ -238,62 +232,140 @@ struct Reading {
     __host__ __device__ int each() const { return sets * per_set; }
 };
 
-// The first `top` tokens of a row, in order, from its groups' maxima (`groups`, a multiple of 64,
-// in the order of shares and sets); how many there are.
-__device__ __forceinline__ int choose(const Logprobs &a, int row, int shift, const Reading &r, const float *maxima,
-    int groups, List &list)
+// A thread's maxima of a row's groups (a multiple of 64 of them, in the order of shares and sets).
+struct Maxima {
+    static constexpr int kChunks = 4;
+    float4 v[kChunks];
+
+    // Four side by side while 256 threads have some each.
+    static __device__ __forceinline__ bool wide(int groups) { return groups >= 4 * kThreads; }
+    static __device__ __forceinline__ int number(bool wide, int i, int e)
+    {
+        return wide ? 4 * (i * kThreads + (int)threadIdx.x) + e : e * kThreads + (int)threadIdx.x;
+    }
+    __device__ __forceinline__ void load(const float *maxima, int groups)
+    {
+        const bool is_wide = wide(groups);
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+            v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (i * 4 * kThreads >= groups) continue;
+            const int g = number(is_wide, i, 0);
+            if (is_wide) {
+                if (g < groups) v[i] = *(const float4 *)(maxima + g);
+            } else {
+                if (g < groups) v[i].x = maxima[g];
+                if (g + kThreads < groups) v[i].y = maxima[g + kThreads];
+                if (g + 2 * kThreads < groups) v[i].z = maxima[g + 2 * kThreads];
+                if (g + 3 * kThreads < groups) v[i].w = maxima[g + 3 * kThreads];
+            }
+        }
+    }
+    __device__ __forceinline__ float most() const
+    {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) m = fmaxf(fmaxf(fmaxf(m, v[i].x), fmaxf(v[i].y, v[i].z)), v[i].w);
+        return m;
+    }
+};
+static_assert(4 * kThreads * Maxima::kChunks >= kMostGroups, "every group of a row");
+
+// The first `top` tokens of a row, in order, from its groups' maxima (a thread's are `mine`); how many
+// there are. `beside` is done by the second wavefront, while the first looks for the bound.
+template <class F>
+__device__ __forceinline__ int choose(const Logprobs &a, int row, int shift, const Reading &r, const Maxima &mine,
+    const float *maxima, int groups, List &list, const F &beside)
 {
     const int tid = threadIdx.x, top = a.top;
     if (tid == 0) list.n = list.listed = 0;
-    float most = -INFINITY;
-    // Four maxima at a time while 256 threads have some each.
-    const int each = groups >= 4 * kThreads ? 4 : 1;
-    if (each == 4) {
-#pragma unroll 4
-        for (int g = 4 * tid; g < groups; g += 4 * kThreads) {
-            const float4 q = *(const float4 *)(maxima + g);
-            most = fmaxf(fmaxf(most, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
-        }
-    } else {
-        for (int g = tid; g < groups; g += kThreads) most = fmaxf(most, maxima[g]);
-    }
+    const float most = mine.most();
     list.maxima[tid] = most;
     __syncthreads();
-    const float from = bound_of(list, top);
-    if (most >= from)
-        for (int g = each * tid; g < groups; g += each * kThreads)
-            for (int e = 0; e < each; ++e)
-                if (maxima[g + e] >= from) {
-                    const unsigned at = atomicAdd(&list.listed, 1u);
-                    if (at < (unsigned)kListed) list.groups[at] = g + e;
+    if (tid < 64) {
+        const float bound = bound_of(list, top);
+        if (tid == 0) list.bound = bound;
+    } else if (tid < 128) {
+        beside();
+    }
+    __syncthreads();
+    const float from = list.bound;
+    if (most >= from) {
+        const bool wide = Maxima::wide(groups);
+        unsigned n = 0;
+#pragma unroll
+        for (int i = 0; i < Maxima::kChunks; ++i)
+            n += (mine.v[i].x >= from) + (mine.v[i].y >= from) + (mine.v[i].z >= from) + (mine.v[i].w >= from);
+        unsigned at = atomicAdd(&list.listed, n);
+#pragma unroll
+        for (int i = 0; i < Maxima::kChunks; ++i) {
+            const float4 q = mine.v[i];
+            const float v[4] = {q.x, q.y, q.z, q.w};
+            if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) < from) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v[e] >= from) {
+                    if (at < (unsigned)kListed) list.groups[at] = Maxima::number(wide, i, e);
+                    ++at;
                 }
+        }
+    }
     __syncthreads();
     // (More groups than are listed, of many equal logits: all of them are gone through.)
     const bool all = list.listed > (unsigned)kListed;
-    const unsigned size = 16 * kV * r.per_set, n = (all ? groups : list.listed) * size;   // at most a row
+    const int n = all ? groups : (int)list.listed;
+    const float *x = a.logits + row * a.stride;
+    // 32 threads a group of 32 logits of each of its tiles, 32 groups at a time.
+    constexpr int kAtOnce = 4 * kThreads / 32;
+    static_assert(kV == 2, "32 logits");
     int held = 0;
-    for (unsigned at = 0; at < n; at += 4 * kThreads) {
-        uint64_t key[4];
+    for (int base = 0, tile = 0;;) {
+        // All of a thread's loads set out together (of what is no candidate, the row's first).
+        int id[4];
+        bool is[4];
+        float logit[4];
+        uint32_t word[4] = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned e = at + i * kThreads + tid;
-            key[i] = 0;
-            if (e >= n) continue;
-            const unsigned k = e / size, j = e % size, g = all ? k : list.groups[k];
-            if (all && maxima[g] < from) continue;
-            const int id = (int)(((g / 64 * r.per_set) * kV + j / 16) * 1024 + 16 * (g % 64) + j % 16) - shift;
-            if (id >= 0 && id < a.n) key[i] = key_in(a, row, id);
+            const int k = base + i * (kThreads / 32) + tid / 32;
+            is[i] = k < n;
+            const int g = !is[i] ? 0 : all ? k : list.groups[k];
+            if (all && is[i]) is[i] = maxima[g] >= from;
+            id[i] = ((g / 64 * r.per_set + tile) * kV + (tid >> 4 & 1)) * 1024 + 16 * (g % 64) + tid % 16 - shift;
+            is[i] = is[i] && id[i] >= 0 && id[i] < a.n;
+            id[i] = is[i] ? id[i] : 0;
+            logit[i] = x[id[i]];
+        }
+        if (a.mask) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) word[i] = a.mask[id[i] >> 5];
         }
         const uint64_t bar = held == top ? list.keys[top - 1] + 1 : key_of(from, 0x7FFFFFFF);
+        uint64_t key[4];
+        unsigned joins = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (key[i] >= bar) list.keys[atomicAdd(&list.n, 1u)] = key[i];
+        for (int i = 0; i < 4; ++i) {
+            key[i] = key_of(logit[i], id[i]);
+            is[i] = is[i] && logit[i] >= -FLT_MAX && !(word[i] >> (id[i] & 31) & 1u) && key[i] >= bar;
+            joins += is[i];
+        }
+        if (joins) {
+            unsigned to = atomicAdd(&list.n, joins);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (is[i]) list.keys[to++] = key[i];
+        }
         __syncthreads();
         const unsigned now = list.n;
         __syncthreads();   // read by all before the next ones join
-        if (at + 4 * kThreads >= n || now > (unsigned)(kRoom - 4 * kThreads)) held = settle(list, top);
+        if (++tile == r.per_set) {
+            tile = 0;
+            base += kAtOnce;
+        }
+        const bool last = base >= n;
+        if (last || now > (unsigned)(kRoom - 4 * kThreads)) held = settle(list, top);
+        if (last) return held;
     }
-    return held;
 }
 
 // What the threads know, together, in all of them. c: scale in powers of two.
@@ -357,39 +429,40 @@ __device__ __forceinline__ double log_sum(const Logprobs &a, const Part &p)
     return log1p((p.count - 1) + p.s) - off * a.scale * (p.t / (p.count + p.s));
 }
 
-// A row's results.
-__device__ __forceinline__ void finish(const Logprobs &a, int row, const Given &g, const Part &p, const List *list, int held)
+// NaN leaves a sum NaN; plus infinity is the maximum.
+__device__ __forceinline__ bool has_none(const Part &p) { return !(p.m > -INFINITY && p.m < INFINITY) || !(p.s >= 0); }
+
+// A row's results beside its first tokens, by one thread; ln S.
+__device__ __forceinline__ double finish(const Logprobs &a, int row, const Given &g, const Part &p)
 {
-    __shared__ double log_s;
-    // NaN leaves a sum NaN; plus infinity is the maximum.
-    const bool none = !(p.m > -INFINITY && p.m < INFINITY) || !(p.s >= 0);
-    if (threadIdx.x == 0) {
-        log_s = log_sum(a, p);
-        if (a.tokens) {
-            const bool ranked = g.there && !none && g.x > -INFINITY;
-            a.logprobs[row] = !g.there ? 0.f : none ? NAN : (float)(((double)g.x - p.m) * a.scale - log_s);
-            if (a.ranks) a.ranks[row] = ranked ? p.rank : -1;
-        }
-        if (a.entropies) a.entropies[row] = none ? NAN : (float)(log_s - p.t / (p.count + p.s) * a.scale);
+    const bool none = has_none(p);
+    const double log_s = log_sum(a, p);
+    if (a.tokens) {
+        const bool ranked = g.there && !none && g.x > -INFINITY;
+        a.logprobs[row] = !g.there ? 0.f : none ? NAN : (float)(((double)g.x - p.m) * a.scale - log_s);
+        if (a.ranks) a.ranks[row] = ranked ? p.rank : -1;
     }
-    if (!list) return;
-    __syncthreads();
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
-        const uint64_t key = k < held ? list->keys[k] : 0;
-        const size_t at = (size_t)row * a.top + k;
-        a.top_ids[at] = none || !key ? -1 : id_of(key);
-        a.top_logprobs[at] = none ? NAN : !key ? -INFINITY : (float)(((double)logit_of(key) - p.m) * a.scale - log_s);
-    }
+    if (a.entropies) a.entropies[row] = none ? NAN : (float)(log_s - p.t / (p.count + p.s) * a.scale);
+    return log_s;
 }
 
-constexpr int kWholeGroups = 4096;   // the most of a row that is one share
+__device__ __forceinline__ void put_top(const Logprobs &a, int row, const Part &p, double log_s, const List &list, int held)
+{
+    const int k = threadIdx.x;
+    if (k >= a.top) return;
+    const bool none = has_none(p);
+    const uint64_t key = k < held ? list.keys[k] : 0;
+    const size_t at = (size_t)row * a.top + k;
+    a.top_ids[at] = none || !key ? -1 : id_of(key);
+    a.top_logprobs[at] = none ? NAN : !key ? -INFINITY : (float)(((double)logit_of(key) - p.m) * a.scale - log_s);
+}
 
 // Workgroup (row, share), 4 kV logits a thread and tile. Positions begin at the 16
 // bytes that the row begins in. kWhole: the row is one share.
 template <bool kTop, bool kWhole>
 __global__ __launch_bounds__(kThreads) void logprobs_rows(Logprobs a, Reading r, Part *parts, float *all_maxima)
 {
-    __shared__ __align__(16) float maxima[kTop && kWhole ? kWholeGroups : 4];
+    __shared__ __align__(16) float maxima[kTop && kWhole ? kMostGroups : 4];
     const int row = kWhole ? blockIdx.x : blockIdx.x / r.shares, share = kWhole ? 0 : blockIdx.x % r.shares, tid = threadIdx.x;
     const float *x0 = a.logits + row * a.stride;
     const int shift = (int)((uintptr_t)x0 >> 2 & 3), end = a.n + shift;
@@ -485,10 +558,15 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(Logprobs a, Reading r,
         if (tid == 0) parts[blockIdx.x] = p;
     } else if constexpr (kTop) {
         __shared__ List list;
-        const int held = choose(a, row, shift, r, maxima, r.sets * 64, list);
-        finish(a, row, g, p, &list, held);
-    } else {
-        finish(a, row, g, p, nullptr, 0);
+        __shared__ double log_s;
+        Maxima mine;
+        mine.load(maxima, r.sets * 64);
+        const int held = choose(a, row, shift, r, mine, maxima, r.sets * 64, list, [&]() {
+            if (tid == 64) log_s = finish(a, row, g, p);
+        });
+        put_top(a, row, p, log_s, list, held);
+    } else if (tid == 0) {
+        finish(a, row, g, p);
     }
 }
 
@@ -496,30 +574,39 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(Logprobs a, Reading r,
 template <bool kTop>
 __global__ __launch_bounds__(kThreads) void logprobs_join(Logprobs a, Reading r, const Part *parts, const float *all_maxima)
 {
-    __shared__ Part all;
-    const int row = blockIdx.x, tid = threadIdx.x, groups = r.shares * r.sets * 64;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, groups = r.shares * r.sets * 64;
     Part p = {-INFINITY, 0, 0, 0, 0};
-    if (tid < r.shares) p = parts[(size_t)row * r.shares + tid];
+    if (lane < r.shares) p = parts[(size_t)row * r.shares + lane];
     const Given g = given_of(a, row);
     const float c = a.scale * 1.44269504f;
-    // The shares' sums, in the first wavefront.
-    if (tid < 64) {
+    // The shares' sums, in a wavefront.
+    auto sums = [&]() {
         Part q = {wave_reduce<true>(p.m), 0, 0, 0, 0};
         add_to(q, p.m, p.count, p.s, p.t, c);
         q.count = wave_sum(q.count);
         q.s = wave_sum(q.s);
         q.t = wave_sum(q.t);
         q.rank = (int)wave_sum((float)p.rank);
-        if (tid == 0) all = q;
-    }
-    __syncthreads();
+        return q;
+    };
     if constexpr (kTop) {
         __shared__ List list;
+        __shared__ double log_s;
+        __shared__ Part all;
+        const float *maxima = all_maxima + (size_t)row * groups;
+        Maxima mine;
+        mine.load(maxima, groups);
         const int shift = (int)((uintptr_t)(a.logits + row * a.stride) >> 2 & 3);
-        const int held = choose(a, row, shift, r, all_maxima + (size_t)row * groups, groups, list);
-        finish(a, row, g, all, &list, held);
-    } else {
-        finish(a, row, g, all, nullptr, 0);
+        const int held = choose(a, row, shift, r, mine, maxima, groups, list, [&]() {
+            const Part q = sums();
+            if (lane != 0) return;
+            all = q;
+            log_s = finish(a, row, g, q);
+        });
+        put_top(a, row, all, log_s, list, held);
+    } else if (tid < 64) {
+        const Part q = sums();
+        if (lane == 0) finish(a, row, g, q);
     }
 }
 
@@ -535,8 +622,8 @@ Reading reading_of(int n, int count, int top, size_t bytes)
     for (;; --shares) {
         if (shares > all) shares = all;
         if (shares < 1) shares = 1;
-        // Tiles of a share, in sets so that a row has at most 64 of them, and one for each share.
-        const int each = (all + shares - 1) / shares, per_set = (each * shares + 63) / 64;
+        // Tiles of a share, in sets so that a row has at most 64 of them.
+        const int each = (all + shares - 1) / shares, most = kMostGroups / 64 / shares, per_set = (each + most - 1) / most;
         Reading r = {shares, (each + per_set - 1) / per_set, per_set};
         r.shares = (all + r.each() - 1) / r.each();
         if (r.shares == 1 || share_bytes(r, top) * r.shares * count <= bytes) return r;
