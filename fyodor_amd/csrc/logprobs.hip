@@ -501,13 +501,17 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(Logprobs a, Reading r,
             for (int v = 0; v < kV; ++v) {
                 const int id = tile + 4 * (kThreads * v + tid) - shift;
                 const int last = (a.n - 1) >> 5, first = max(id, 0) >> 5;
-                const uint64_t both = (uint64_t)a.mask[min(max(id + 3, 0) >> 5, last)] << 32 | a.mask[min(first, last)];
-                // (Of one word twice, the low one has the bits.)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int bit = id + e - 32 * first;
-                    if (bit >= 0 && (both >> (bit & 63) & 1u)) x[4 * v + e] = -INFINITY;
+                uint32_t off = a.mask[min(first, last)];
+                if (shift) {
+                    // The four may lie in two words, or before the row's first.
+                    const uint64_t both = (uint64_t)a.mask[min(max(id + 3, 0) >> 5, last)] << 32 | off;
+                    off = id < 0 ? off << -id : (uint32_t)(both >> (id & 31));
+                } else {
+                    off >>= id & 31;
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (off >> e & 1u) x[4 * v + e] = -INFINITY;
             }
         }
         float most = x[0];
