@@ -21,7 +21,16 @@
 // workgroup of 16 rows that converts straight into the operands' lanes (kv4_rows),
 // and one of 128 rows that convert each code once, in LDS (kv4_wide). What is
 // too few tiles for the chip is split over the positions and joined by a second
-// launch (kv4_join).
+// launch (kv4_join), by the rules of the 8-bit cache: the count of shares was
+// measured again here (64 requests of 500 to 8192 positions, shares for 1536,
+// 2048, 3072 and 4096 workgroups: 51 to 56 us).
+//
+// Measured, 32 heads over 8 of 128 unless said: one token of 65536 positions 19.9 us
+// and 3.9 for the join (75 MB, 3.8 TB/s), 64 requests as above 50.8 and 6.0 (186 MB,
+// 3.7 TB/s; the loads alone take 45, the arithmetic alone 48), eight requests of 5
+// tokens, 32 heads over 4 of 64, 9.6 and 4.8; a prompt of 1024 tokens at the end of
+// 8192 positions 239 us, 1078 TFLOP/s as issued where a large library product
+// reaches 1154; prompts of 16 heads over 8 of 256 110 (kv4_wide).
 #include "paged_attention.h"
 
 namespace fy {
@@ -111,8 +120,13 @@ __device__ __forceinline__ uint4 some_steps(const uint4 &s, int from, int limit)
 // fourth step of its share of the positions and meet in LDS at the end. Keys
 // and values go from memory straight into the operands' lanes: K and V of a
 // step are requested as soon as the last step's are used up, pages a step
-// before that. Steps [from, until) of the tile's; a `shared` tile's rows go to
-// `to`, `stride` places apart.
+// before that (two steps ahead: 62 us for the 64 requests' 51). Steps [from, until) of the
+// tile's; a `shared` tile's rows go to `to`, `stride` places apart.
+//
+// kPair, where a tile has at most eight rows: the two pieces of q and of the
+// weights are columns of their own, eight apart, so a product is one matrix
+// instruction, and half the registers of q let a third wavefront onto a SIMD
+// (with conversions free of literals the 64 requests went from 68 to 51 us).
 template <int W, bool kPair>
 __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Request &rq, const Range &g, int kvh, int tile,
     int from, int until, bool shared, const Share &to, int stride, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
@@ -405,7 +419,10 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Req
 }
 
 // Wavefronts of few rows on a SIMD, and so their workgroups on a CU: what their registers leave.
-constexpr int waves_of(int width, bool pair) { return width == 64 ? (pair ? 4 : 3) : width == 128 ? (pair ? 3 : 2) : 1; }
+constexpr int waves_of(int width, bool pair)
+{
+    return width == 64 ? (pair ? 4 : 3) : width == 128 ? (pair ? 3 : 2) : 1;
+}
 
 template <int W, bool kPair>
 __global__ __launch_bounds__(64 * kWaves, waves_of(W, kPair)) void kv4_rows(Kv4Attention a, Split split, int most_rows)
@@ -443,7 +460,10 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(W, kPair)) void kv4_rows(Kv4A
 // end. Two groups run half a step apart: while one is in its MFMAs (last
 // step's outputs, this step's scores) the other does its softmax and stages
 // its next codes, so that the matrix cores of a SIMD always have one of its two
-// wavefronts. Heads of 256 fill the registers with one group.
+// wavefronts. Heads of 256 fill the registers with one group, whose softmax and
+// conversions nothing covers: matrix cores busy 24 % (16 rows per wavefront and
+// two groups: 136 us for 110, twice the reads of LDS; the last step's outputs
+// under the softmax: 109).
 template <int W, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
 void kv4_wide(Kv4Attention a, Split split, int most_rows)
@@ -569,7 +589,8 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
             if (__builtin_amdgcn_ballot_w64(limit < 8 || low > 0)) vstep[i] = some_steps(vstep[i], low, limit);
             half8 x[4];
             value_words(codes, vreg[i], vstep[i], x);
-            uint8_t *to = vsm + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 + 32 * (eighth >> 1 & 1) + (quad & 7)) * 16;
+            uint8_t *to = vsm + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 +
+                                 32 * (eighth >> 1 & 1) + (quad & 7)) * 16;
 #pragma unroll
             for (int e = 0; e < 4; ++e) *(half8 *)(to + 128 * e) = x[e];
         }

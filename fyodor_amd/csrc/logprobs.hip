@@ -17,10 +17,13 @@
 // pass: 64 rows of 128256 17 us with 20 alternatives, 10 without.)
 //
 // Bound by reading the logits for many rows (2047 of 50257 without alternatives
-// 77 us, 5.4 TB/s; with 20 of them 106). A few rows are split into shares,
-// which a second launch joins (64 of 128256: 11 us, 8 for the join; 1 of 32000: 3.9 and
-// 5.3): chains of waits, of which the join has five: the shares, the maxima again,
-// the logits, two turns in LDS.
+// 77 us, 5.4 TB/s; with 20 of them 99: the choice at a row's end is waits, and its LDS
+// leaves five workgroups on a CU for eight). A few rows are split into shares,
+// which a second launch joins (64 of 128256 with 20: 11.0 us and 7.2, masked 12.2 and
+// 7.4; 1 of 32000 with 5: 3.8 and 5.0): chains of waits, of which the join has four:
+// the shares with the maxima, the bound with the sums beside it, the logits, their
+// order. (The maxima read twice, the logits one after another, the sums first:
+// 11.8 for 7.4.)
 #include <float.h>
 #include <limits.h>
 #include <math.h>
@@ -96,7 +99,8 @@ struct List {
     unsigned n, listed;
 };
 
-// Leaves, of more keys than are worth comparing with each other, the ones above a bound that at
+// Leaves, of more keys than are worth comparing with each other (634 rows of 984, 33 of them: 34 us without
+// this, 13 with it), the ones above a bound that at
 // least `top` of them reach and few more do (all, if they are of one logit): as bound_of, with
 // every thread's keys in registers.
 __device__ void narrow(List &list, int top)
@@ -619,7 +623,7 @@ size_t share_bytes(const Reading &r, int top) { return sizeof(Part) + (top ? (si
 Reading reading_of(int n, int count, int top, size_t bytes)
 {
     const int all = (n + 3 + kTile - 1) / kTile;   // a row may begin 3 floats into its 16 bytes
-    // Four workgroups for each CU: 64 rows of 128256, 8, 16 and 32 shares 13.0, 10.6 and 11.5 us, the join 8;
+    // Four workgroups for each CU: 64 rows of 128256, 8, 16 and 32 shares 13.0, 10.6 and 11.5 us, the join 7;
     // from 1024 rows on, whole ones (2047 of 50257 77 us, in 4 shares 85 and 5 for the join).
     int shares = count >= 1024 ? 1 : (1024 + count - 1) / count;
     shares = shares < kMostShares ? shares : kMostShares;

@@ -67,8 +67,9 @@ __device__ __forceinline__ float column_sum(float v)
 constexpr float kFar = 0x1p22f;
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -INFINITY; }
 
-// What a row's sum of weights makes of its outputs (times A::kLess, by which sums are held smaller). Without weights the row saw
-// nothing (no maximum) and gives zeros, or its scores were beyond fp32.
+// What a row's sum of weights makes of its outputs (times A::kLess, by which sums are
+// held smaller). Without weights the row saw nothing (no maximum) and gives zeros,
+// or its scores were beyond fp32.
 __device__ __forceinline__ float inverse_of(float total, float top)
 {
     return total == 0.f ? (top == -INFINITY ? 0.f : NAN) : 1.f / total;

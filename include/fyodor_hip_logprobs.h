@@ -29,9 +29,9 @@ extern "C" {
  * is minus infinity, is in no order: ln p is minus infinity, its rank -1, and
  * if fewer than `top` others are left the rest of top_ids is -1 with minus
  * infinity. An id outside [0, n) is no token (a padded batch, a prompt's
- * first position): 0 and rank -1, whatever the row holds. A row with a NaN or plus infinity among the
- * entries that are not masked, or with no entry above minus infinity, has no
- * probabilities: NaN, ranks and ids -1.
+ * first position): 0 and rank -1, whatever the row holds. A row with a NaN or
+ * plus infinity among the entries that are not masked, or with no entry above
+ * minus infinity, has no probabilities: NaN, ranks and ids -1.
  *
  * Logits enter as they are; exponentials and their sums are fp32, the
  * logarithm's argument and what follows 64 bits, rounded once. The same
