@@ -289,6 +289,15 @@ def test_attention_runs(env, dev, heads, kv_heads, width, window):
         assert np.all(got[starts[5]:starts[5] + 4] == 0)
 
 
+@pytest.mark.parametrize("heads,kv_heads,width", [(80, 1, 64), (129, 1, 128), (144, 2, 128), (72, 1, 256), (96, 1, 512)])
+@pytest.mark.parametrize("lengths,counts", [([300, 41, 90], [1, 1, 1]), ([300, 41, 90], [2, 0, 7]), ([150], [3])])
+def test_attention_wide_groups(env, dev, heads, kv_heads, width, lengths, counts):
+    """Groups of more heads than a call of few rows takes."""
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 32, 9)
+    got = run_attention(env, dev, cache, q, starts, lengths, table)
+    check_attention(cache, q, got, starts, lengths, table)
+
+
 @pytest.mark.parametrize("heads,kv_heads,width,page_tokens,length,tokens,window", [
     (8, 2, 128, 64, 9000, 1, 0), (8, 2, 128, 16, 9001, 3, 0), (4, 4, 64, 128, 5000, 1, 1000),
     (16, 1, 64, 32, 6000, 9, 0), (8, 8, 128, 64, 2500, 300, 0), (4, 2, 256, 32, 1500, 130, 500),
