@@ -22,8 +22,8 @@
 // and one of 128 rows that convert each code once, in LDS (kv4_wide). What is
 // too few tiles for the chip is split over the positions and joined by a second
 // launch (kv4_join), by the rules of the 8-bit cache: the count of shares was
-// measured again here (64 requests of 500 to 8192 positions, shares for 1536,
-// 2048, 3072 and 4096 workgroups: 51 to 56 us).
+// measured again here (64 requests of 500 to 8192 positions, shares for 1536 to
+// 4096 workgroups: 51 to 56 us, least with the 2048 of there).
 //
 // Measured, 32 heads over 8 of 128 unless said: one token of 65536 positions 19.9 us
 // and 3.9 for the join (75 MB, 3.8 TB/s), 64 requests as above 50.8 and 6.0 (186 MB,
@@ -126,7 +126,8 @@ __device__ __forceinline__ uint4 some_steps(const uint4 &s, int from, int limit)
 // kPair, where a tile has at most eight rows: the two pieces of q and of the
 // weights are columns of their own, eight apart, so a product is one matrix
 // instruction, and half the registers of q let a third wavefront onto a SIMD
-// (with conversions free of literals the 64 requests went from 68 to 51 us).
+// (with conversions free of literals the 64 requests went from 68 to 51 us; four
+// wavefronts, which leave no registers for a step ahead, 70).
 template <int W, bool kPair>
 __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Request &rq, const Range &g, int kvh, int tile,
     int from, int until, bool shared, const Share &to, int stride, float (*ml)[kWaves][kRows], float (*po)[kRows][64 + 4])
