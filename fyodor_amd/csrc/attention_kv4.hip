@@ -30,7 +30,7 @@
 // 3.7 TB/s; the loads alone take 45, the arithmetic alone 48), eight requests of 5
 // tokens, 32 heads over 4 of 64, 9.6 and 4.8; a prompt of 1024 tokens at the end of
 // 8192 positions 239 us, 1078 TFLOP/s as issued where a large library product
-// reaches 1154; prompts of 16 heads over 8 of 256 110 (kv4_wide).
+// reaches 1154; prompts of 16 heads over 8 of 256 94 (kv4_wide).
 #include "paged_attention.h"
 
 namespace fy {
@@ -54,11 +54,17 @@ struct Codes {
     }
 };
 
+// 8 positions of an element, or 8 elements of a position, by pairs.
+union Pairs {
+    half8 v;
+    half2 p[4];
+};
+
 // 8 elements of a key.
 __device__ __forceinline__ half8 key_word(const Codes &c, uint32_t w, _Float16 step)
 {
     const half2 s = {step, step};
-    union { half8 v; half2 p[4]; } u;
+    Pairs u;
     u.p[0] = c.lows(w) * s;
     u.p[1] = c.highs(w) * s;
     u.p[2] = c.lows(w >> 8) * s;
@@ -69,7 +75,7 @@ __device__ __forceinline__ half8 key_word(const Codes &c, uint32_t w, _Float16 s
 // 8 positions of 4 elements of the values: a word of codes, and of steps, has two positions.
 __device__ __forceinline__ void value_words(const Codes &c, const uint4 &w, const uint4 &steps, half8 *x)
 {
-    union { half8 v; half2 p[4]; } u[4];
+    Pairs u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t n = word_of(w, i);
@@ -148,7 +154,7 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Req
     const int64_t p = rq.first + token;
     const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
-    // Positions that all rows see: up to the first row's last, from the last row's first.
+    // Pairs that all rows see: up to the first row's last, from the last row's first.
     const int64_t p0 = rq.first + kRows * tile / group, p1 = rq.first + min(kRows * tile + kRows - 1, rq.rows - 1) / group;
     const int all_to = (int)(p0 < g.highest ? p0 : g.highest);
     const int all_from = (int)(a.window && p1 >= a.window ? (p1 - a.window < g.highest ? p1 - a.window + 1 : g.highest + 1) : 0);
@@ -461,10 +467,12 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(W, kPair)) void kv4_rows(Kv4A
 // end. Two groups run half a step apart: while one is in its MFMAs (last
 // step's outputs, this step's scores) the other does its softmax and stages
 // its next codes, so that the matrix cores of a SIMD always have one of its two
-// wavefronts. Heads of 256 fill the registers with one group, whose softmax and
-// conversions nothing covers: matrix cores busy 24 % (16 rows per wavefront and
-// two groups: 136 us for 110, twice the reads of LDS; the last step's outputs
-// under the softmax: 109).
+// wavefronts. Heads of 256 fill the registers with one group (q and the outputs are
+// 256 of them; 16 rows per wavefront and two groups read LDS twice as often, 136 us
+// for 110), which runs its conversions and weights under its own MFMAs: prompts of up
+// to 700 tokens, 16 heads over 8, 94 us (110 with everything in turn; operands
+// requested a tile ahead 104, the codes under the scores 100). A step is 7000 cycles
+// where its MFMAs take 4100, and q, in 32 MB at once, and the outputs are 25 us at both ends.
 template <int W, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
 void kv4_wide(Kv4Attention a, Split split, int most_rows)
@@ -474,7 +482,8 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     constexpr int N = W < 128 ? 1 : W / 128;   // 16-byte pieces of K, and of V, per thread and step
     constexpr int kBlocks = W / kBlock, kBytes = 2 * kStep * W;
     constexpr int kQuads = W / 4;   // pieces of V per 8 positions
-    __shared__ __align__(16) uint8_t smem[KS][2][kBytes];   // [group][K, V]
+    constexpr int kBuffers = KS == 1 ? 2 : 1;
+    __shared__ __align__(16) uint8_t smem[KS][2 * kBuffers][kBytes];   // [group][K's, V's]
     __shared__ int theres[KS][2][4];                        // whether 16 positions have a page
     __shared__ float2 smem_ml[4][32];
     const Kv4 &c = a.cache;
@@ -500,7 +509,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     // (Rows past the request's last repeat it and are not written.)
     const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
-    // Positions that all of the wavefront's rows see.
+    // Pairs that all of the wavefront's rows see.
     int all_from = first, all_to = last;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -519,12 +528,16 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     // everything unconditionally (positions past the last one lead to page 0):
     // loads under a condition would be waited for where it ends.
     const int until = min(g.highest, kStep * stop - 1);   // this workgroup's last position
-    auto entry_of = [&](int at) {
-        const int entry = table[min(at >> shift, a.table_stride - 1)];
-        return at <= until ? entry : -1;
-    };
-    auto place_of = [&](int page) { return (size_t)((unsigned)page < (unsigned)c.pages ? page : 0) * c.kv_heads + kvh; };
-    const size_t plane = (size_t)c.page_tokens * (W / 2), steps = (size_t)c.page_tokens * kBlocks;
+    // (What is past `until` is told where an entry is used: where it is read, the select would wait for it.)
+    auto entry_of = [&](int at) { return table[min(at >> shift, a.table_stride - 1)]; };
+    auto page_at = [&](int at, int entry) { return at <= until ? entry : -1; };
+    // A page's codes and steps of this head: whole pages of 32 bits of bytes from the first one's.
+    auto page_of = [&](int page) { return (unsigned)page < (unsigned)c.pages ? (unsigned)page : 0u; };
+    const unsigned plane = c.page_tokens * (W / 2), steps = c.page_tokens * kBlocks;
+    const unsigned page_codes = c.kv_heads * plane, page_steps = 2 * c.kv_heads * steps;
+    const uint8_t *keys = c.keys + (size_t)kvh * plane, *values = c.values + (size_t)kvh * plane;
+    const uint8_t *key_steps = (const uint8_t *)(c.key_steps + (size_t)kvh * steps),
+                  *value_steps = (const uint8_t *)(c.value_steps + (size_t)kvh * steps);
     int kpage, vpage[N], spage;
     // This thread's piece i of K is block wave + 4 i of position `lane` of the
     // step, of V the elements 4 quad.. of 8 positions. Heads of 64 have half as many:
@@ -544,56 +557,67 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     bool sthere;
     auto fetch_k = [&](int step) {
         const int t = (kStep * step + lane) & within;
-        const size_t page = place_of(kpage);
-        const uint8_t *kb = c.keys + page * plane + (kblock * c.page_tokens + t) * 16;
-        const uint16_t *sb = c.key_steps + page * steps + ((t >> 4) * kBlocks + kblock) * 16 + (t & 3) * 4 + (t >> 2 & 3);
+        const unsigned page = page_of(page_at(kStep * step + (lane & 48), kpage));
+        const uint8_t *kb = keys + (uint64_t)page * page_codes + (kblock * c.page_tokens + t) * 16;
+        const uint16_t *sb = (const uint16_t *)(key_steps + (uint64_t)page * page_steps) +
+                             (((t >> 4) * kBlocks + kblock) * 16 + (t & 3) * 4 + (t >> 2 & 3));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             kreg[i] = *(const uint4 *)(kb + (size_t)64 * c.page_tokens * i);
             kstep[i] = __builtin_bit_cast(_Float16, sb[64 * i]);
         }
-        sthere = (unsigned)spage < (unsigned)c.pages;
+        sthere = (unsigned)page_at(kStep * step + 16 * (tid & 3), spage) < (unsigned)c.pages;
     };
     auto fetch_v = [&](int step) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int piece = vpiece + 256 * i, quad = piece % kQuads, vat = kStep * step + 8 * (piece / kQuads);
-            const size_t page = place_of(vpage[i]);
+            vpage_at[i] = page_at(vat, vpage[i]);
+            const unsigned page = page_of(vpage_at[i]);
             const int t = vat & within;
-            vpage_at[i] = vpage[i];
-            vreg[i] = *(const uint4 *)(c.values + page * plane + ((t >> 3) * kQuads + quad) * 16);
-            vstep[i] = *(const uint4 *)(c.value_steps + page * steps + (quad >> 3) * c.page_tokens + t);
+            vreg[i] = *(const uint4 *)(values + (uint64_t)page * page_codes + ((t >> 3) * kQuads + quad) * 16);
+            vstep[i] = *(const uint4 *)(value_steps + (uint64_t)page * page_steps + 2 * ((quad >> 3) * c.page_tokens + t));
         }
     };
-    uint8_t *const ksm = smem[ks][0], *const vsm = smem[ks][1];
-    auto stage_k = [&](int buffer) {
+    auto ktile = [&](int buffer) { return smem[ks][buffer & (kBuffers - 1)]; };
+    auto vtile = [&](int buffer) { return smem[ks][kBuffers + (buffer & (kBuffers - 1))]; };
+    auto k_place = [&](int buffer, int i) {
         const int t = lane & 31, rho = 8 * ((t & 15) >> 2) + 4 * (t >> 4) + (t & 3);
-        if (W >= 128 || wave < 2) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                uint8_t *to = ksm + (((lane >> 5) * M + 2 * (kblock + 4 * i)) * 64 + rho) * 16;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) *(half8 *)(to + 512 * j) = key_word(codes, word_of(kreg[i], j), kstep[i]);
-            }
-        }
-        if (tid < 4) theres[ks][buffer][tid] = sthere;
+        return ktile(buffer) + (((lane >> 5) * M + 2 * (kblock + 4 * i)) * 64 + rho) * 16;
     };
+    auto stage_k = [&](int buffer) {
+        if (W < 128 && wave >= 2) return;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(half8 *)(k_place(buffer, i) + 512 * j) = key_word(codes, word_of(kreg[i], j), kstep[i]);
+    };
+    auto stage_there = [&](int buffer) {
+        if (tid < 4) theres[ks][buffer & 1][tid] = sthere;
+    };
+    // The steps of V's piece i, of what this workgroup's rows see.
+    auto v_limit = [&](int step, int i) {
+        const int vat = kStep * step + 8 * ((vpiece + 256 * i) / kQuads);
+        return (unsigned)vpage_at[i] < (unsigned)c.pages ? until - vat + 1 : 0;
+    };
+    auto v_low = [&](int step, int i) { return g.lowest - (kStep * step + 8 * ((vpiece + 256 * i) / kQuads)); };
     // Element 4 q + e of 32 is row 8 e + q of its tile, so that the threads of a wavefront write side by side.
-    auto stage_v = [&](int step) {
+    auto v_place = [&](int buffer, int i) {
+        const int piece = vpiece + 256 * i, quad = piece % kQuads, eighth = piece / kQuads;
+        return vtile(buffer) + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 + 32 * (eighth >> 1 & 1) +
+                                (quad & 7)) * 16;
+    };
+    auto stage_v = [&](int step, int buffer) {
         if (W < 128 && wave < 2) return;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int piece = vpiece + 256 * i, quad = piece % kQuads, eighth = piece / kQuads;
-            const int vat = kStep * step + 8 * eighth;
-            const int limit = (unsigned)vpage_at[i] < (unsigned)c.pages ? until - vat + 1 : 0;
-            const int low = g.lowest - vat;
+            const int low = v_low(step, i), limit = v_limit(step, i);
             if (__builtin_amdgcn_ballot_w64(limit < 8 || low > 0)) vstep[i] = some_steps(vstep[i], low, limit);
             half8 x[4];
             value_words(codes, vreg[i], vstep[i], x);
-            uint8_t *to = vsm + ((((eighth >> 2) * D + (quad >> 3)) * 2 + (eighth & 1)) * 64 +
-                                 32 * (eighth >> 1 & 1) + (quad & 7)) * 16;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) *(half8 *)(to + 128 * e) = x[e];
+            for (int e = 0; e < 4; ++e) *(half8 *)(v_place(buffer, i) + 128 * e) = x[e];
         }
     };
     look_k(begin);
@@ -625,6 +649,11 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
         for (int i = 0; i < 8 * M; ++i) v[i] = ldexpf(a.scale < 0.f ? -v[i] : v[i], e);
 #pragma unroll
         for (int i = 0; i < M; ++i) split_f16(v + 8 * i, qh[i], ql[i]);
+        if constexpr (KS == 1) {
+            // q in the accumulation registers, where MFMAs read it: left to the compiler it was copied from there.
+#pragma unroll
+            for (int i = 0; i < M; ++i) asm("" : "+a"(qh[i]), "+a"(ql[i]));
+        }
         // Above 0, so that it keeps minus infinity.
         qscale = fmaxf(ldexpf(fabsf(a.scale) * 1.44269504f, -e), 0x1p-126f);
     }
@@ -635,40 +664,72 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     float m = -INFINITY, l = 0.f;
     bool far = false;
     uint64_t saw = 0;   // lanes that had a score
-    auto outputs = [&]() {
-        const uint8_t *vs = vsm + 16 * lane;
+    // Each tile's operands are requested a tile ahead (the groups keep the compiler from moving the
+    // reads to where they are used): a wavefront would wait for every one of them.
+    constexpr int kMfma = 0x008, kRead = 0x100;
+    auto outputs = [&](int buffer, auto beside) {
+        const uint8_t *vs = vtile(buffer) + 16 * lane;
+        auto tile = [&](int n, int d) { return *(const half8 *)(vs + ((n >> 1) * (2 * D) + 2 * d + (n & 1)) * 1024); };
+        constexpr int kAhead = 4;   // (pairs of tiles are two apart)
+        half8 v[kAhead];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int d = 0; d < kAhead; ++d) v[d] = tile(d / D, d % D);
+        if constexpr (KS == 2) __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                half8 v[D];
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int d = 0; d < D; ++d) v[d] = *(const half8 *)(vs + ((t * D + d) * 2 + u) * 1024);
+            for (int d = 0; d < D; d += 2) {
 #pragma unroll
-                for (int d = 0; d < D; ++d)
-                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph[t][u], O[d], 0, 0, 0);
+                for (int part = 0; part < 4; ++part) {
+                    const int e = d + (part & 1);
+                    if constexpr (KS == 1) __builtin_amdgcn_sched_barrier(0);
+                    O[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[(n * D + e) % kAhead],
+                                                                  part < 2 ? ph[n >> 1][n & 1] : pl[n >> 1][n & 1], O[e], 0, 0, 0);
+                    if constexpr (KS == 1) __builtin_amdgcn_sched_barrier(0);
+                    beside(n, d, part);
+                }
+                if constexpr (KS == 1) __builtin_amdgcn_sched_barrier(0);
+                else __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
+                if (n * D + d + kAhead >= 4 * D) continue;
 #pragma unroll
-                for (int d = 0; d < D; ++d)
-                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[t][u], O[d], 0, 0, 0);
+                for (int e = d; e < d + 2; ++e) v[(n * D + e) % kAhead] = tile((n * D + e + kAhead) / D, (n * D + e + kAhead) % D);
+                if constexpr (KS == 2) __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
             }
     };
-    auto scores = [&]() {
-        const uint8_t *kp = ksm + 16 * lane;
+    auto scores = [&](int buffer, auto beside) {
+        const uint8_t *kp = ktile(buffer) + 16 * lane;
 #pragma unroll
         for (int t = 0; t < 2; ++t) S[t] = (f32x16){};
+        constexpr int kAhead = KS == 1 ? 2 : 1;
+        half8 k[kAhead + 1][2];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) k[j][t] = *(const half8 *)(kp + (t * M + j) * 1024);
+        if constexpr (KS == 2) __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
 #pragma unroll
         for (int j = 0; j < M; ++j) {
-            const half8 k0 = *(const half8 *)(kp + j * 1024), k1 = *(const half8 *)(kp + (M + j) * 1024);
-            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[j], S[0], 0, 0, 0);
-            S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[j], S[1], 0, 0, 0);
-            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[j], S[0], 0, 0, 0);
-            S[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[j], S[1], 0, 0, 0);
+            if (j + kAhead < M) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) k[(j + kAhead) % (kAhead + 1)][t] = *(const half8 *)(kp + (t * M + j + kAhead) * 1024);
+                if constexpr (KS == 2) __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+            }
+#pragma unroll
+            for (int part = 0; part < 4; ++part) {
+                const int t = part & 1;
+                if constexpr (KS == 1) __builtin_amdgcn_sched_barrier(0);
+                S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j % (kAhead + 1)][t], part < 2 ? qh[j] : ql[j], S[t], 0, 0, 0);
+                if constexpr (KS == 1) __builtin_amdgcn_sched_barrier(0);
+                beside(j, part);
+            }
+            if constexpr (KS == 1) __builtin_amdgcn_sched_barrier(0);
+            else __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
         }
     };
-    // Between the MFMAs: softmax of the scores, the last codes into LDS.
-    auto between = [&](int step, int buffer) {
-        stage_v(step);
-        stage_k(buffer ^ 1);
+    // A step's softmax: its maximum (`grew`: alpha is what the sums so far are worth less) ...
+    float alpha = 1.f, scale = 0.f, add = 0.f;
+    bool grew = false;
+    auto peak = [&](int step, int buffer) {
         const int at = kStep * step;
         const bool whole = all_from <= at && all_to >= at + kStep - 1;
         bool there[2];
@@ -688,17 +749,17 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
         for (int n = 1; n < 32; ++n) best = fmaxf(best, S[n >> 4][n & 15]);
         saw |= __builtin_amdgcn_ballot_w64(best > -INFINITY);
         const float top = best * qscale;
-        if (__builtin_amdgcn_ballot_w64(top > m)) {
+        grew = __builtin_amdgcn_ballot_w64(top > m);
+        if (grew) {
             const float next = fmaxf(m, ceilf(halves_max(top)));
-            const float alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
+            alpha = __builtin_amdgcn_exp2f(m - (next == -INFINITY ? 0.f : next));
             m = next;
             l *= alpha;
-#pragma unroll
-            for (int d = 0; d < D; ++d) O[d] *= alpha;
             far = __builtin_amdgcn_ballot_w64(is_far(m));
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float scale = qscale, add = 15.f - base;
+        scale = qscale;
+        add = 15.f - base;
         if (far) {
 #pragma clang fp contract(off)
 #pragma unroll
@@ -706,51 +767,169 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
             scale = 1.f;
             add = 15.f;
         }
-        float sum[2] = {0.f, 0.f};
+    };
+    // ... what it makes of the outputs ...
+    auto rescale = [&]() {
+        if (!grew) return;
 #pragma unroll
-        for (int n = 0; n < 32; n += 8) {
-            float w[8];
+        for (int d = 0; d < D; ++d) O[d] *= alpha;
+    };
+    // ... and its weights.
+    float sum[2];
+    auto weight = [&](int n) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[n >> 4][n & 15], scale, add));
+        sum[n & 1] += w;
+        return w;
+    };
+    // A round past the group's last step is one of positions that are not there.
+    if (KS == 2 && rounds > 0) {
+        // The next codes set out before the MFMAs and are there after them, and go into
+        // LDS between the MFMAs with the softmax.
+        auto ahead = [&](int step) {
+            fetch_k(step + KS);
+            fetch_v(step);
+            look_v(step + KS);
+            look_k(step + 2 * KS);
+        };
+        auto between = [&](int i) {
+            stage_v(begin + KS * i, 0);
+            stage_k(0);
+            stage_there(i + 1);
+            peak(begin + KS * i, i & 1);
+            rescale();
+            sum[0] = sum[1] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[n >> 4][(n & 15) + i], scale, add));
-                sum[i & 1] += w[i];
+            for (int n = 0; n < 4; ++n) {
+                float w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = weight(8 * n + k);
+                split_f16(w, ph[n >> 1][n & 1], pl[n >> 1][n & 1]);
             }
-            split_f16(w, ph[n >> 4][n >> 3 & 1], pl[n >> 4][n >> 3 & 1]);
-        }
-        l += sum[0] + sum[1];
-    };
-    // The next codes set out before the MFMAs and are there after them. A
-    // round past the group's last step is one of positions that are not there.
-    auto ahead = [&](int step) {
-        fetch_k(step + KS);
-        fetch_v(step);
-        look_v(step + KS);
-        look_k(step + 2 * KS);
-    };
-    if (rounds > 0) {
+            l += sum[0] + sum[1];
+        };
+        auto none = [](auto...) {};
         stage_k(0);
+        stage_there(0);
         lds_barrier();
-        if (KS == 2 && ks) lds_barrier();   // half a step behind
+        if (ks) lds_barrier();   // half a step behind
         ahead(begin);
         __builtin_amdgcn_s_setprio(1);
-        scores();
+        scores(0, none);
         __builtin_amdgcn_s_setprio(0);
         lds_barrier();
-        between(begin, 0);
+        between(0);
         lds_barrier();
         for (int i = 1; i < rounds; ++i) {
             ahead(begin + KS * i);
             __builtin_amdgcn_s_setprio(1);
-            outputs();
-            scores();
+            outputs(0, none);
+            scores(0, none);
             __builtin_amdgcn_s_setprio(0);
             lds_barrier();   // this group's tiles are read
-            between(begin + KS * i, i & 1);
+            between(i);
             lds_barrier();   // the next ones are there
         }
-        outputs();
-        if (KS == 2 && !ks) lds_barrier();
+        outputs(0, none);
+        if (!ks) lds_barrier();
         __syncthreads();
+    }
+    if constexpr (KS == 1) {
+        // One wavefront per SIMD, so what is not an MFMA goes under those of the same wavefront, a few
+        // instructions behind each: the next codes under the scores, into tiles of their own (a step
+        // has one wait), the weights under the last step's outputs.
+        static_assert(KS == 2 || (8 * N == M && D == 8), "as much as the MFMAs cover");
+        Pairs u[4], key, high[4], low[4];
+        // Behind MFMA `part` of four of part j of the scores: two elements of K's word j, or of V's word j - 4 N.
+        auto stage = [&](int i, int j, int part) {
+            const int piece = j / 4 % N, w = j % 4;
+            const uint32_t n = (j < 4 * N ? word_of(kreg[piece], w) : word_of(vreg[piece], w)) >> (part & 2 ? 8 : 0);
+            const half2 code = part & 1 ? codes.highs(n) : codes.lows(n);
+            if (j < 4 * N) {
+                key.p[part] = code * (half2){kstep[piece], kstep[piece]};
+                if (part == 3) *(half8 *)(k_place(i + 1, piece) + 512 * w) = key.v;
+            } else {
+                u[part].p[w] = code * __builtin_bit_cast(half2, word_of(vstep[piece], w));
+                if (w == 3) *(half8 *)(v_place(i, piece) + 128 * part) = u[part].v;
+            }
+        };
+        // Behind MFMA `part` of four of the outputs' tiles d and d + 1: weights d and d + 1 of eight n, and their pieces.
+        float minus = -1.f, w[2];
+        asm("" : "+s"(minus));   // as in split_f16
+        auto weigh = [&](int n, int d, int part) {
+            if (part < 2) {
+                w[part] = weight(8 * n + d + part);
+            } else if (part == 2) {
+                typedef float f32x2 __attribute__((ext_vector_type(2)));
+                half2 hi = __builtin_convertvector((f32x2){w[0], w[1]}, half2);
+                const f32x2 r = {__builtin_fmaf((float)hi.x, minus, w[0]), __builtin_fmaf((float)hi.y, minus, w[1])};
+                half2 lo = __builtin_convertvector(r, half2);
+                asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sum[0]), "+v"(sum[1]));   // here, not where they are used
+                high[n].p[d / 2] = hi;
+                low[n].p[d / 2] = lo;
+            }
+        };
+        // Codes wait for their turn in accumulation registers, as q does: loads reach them.
+        auto wait_there = [](uint4 &x) {
+            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+            u32x4 v = __builtin_bit_cast(u32x4, x);
+            asm volatile("" : "+a"(v));
+            x = __builtin_bit_cast(uint4, v);
+        };
+        auto scored = [&](int i) {
+            const int step = begin + i;
+#pragma unroll
+            for (int p = 0; p < N; ++p) {
+                wait_there(kreg[p]);
+                wait_there(vreg[p]);
+                wait_there(vstep[p]);
+            }
+#pragma unroll
+            for (int p = 0; p < N; ++p) {
+                const int below = v_low(step, p), limit = v_limit(step, p);
+                if (__builtin_amdgcn_ballot_w64(limit < 8 || below > 0)) vstep[p] = some_steps(vstep[p], below, limit);
+            }
+            scores(i, [&](int j, int part) { stage(i, j, part); });
+            stage_there(i + 1);
+            fetch_k(step + 2);
+            fetch_v(step + 1);
+            look_v(step + 2);
+            look_k(step + 3);
+            peak(step, i & 1);
+            sum[0] = sum[1] = 0.f;
+        };
+        auto weighed = [&]() {
+            l += sum[0] + sum[1];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                ph[n >> 1][n & 1] = high[n].v;
+                pl[n >> 1][n & 1] = low[n].v;
+            }
+            lds_barrier();   // this step's tiles are read, the next ones are there
+        };
+        stage_k(0);
+        stage_there(0);
+        fetch_k(begin + 1);
+        fetch_v(begin);
+        look_v(begin + 1);
+        look_k(begin + 2);
+        lds_barrier();
+        if (rounds > 0) {
+            scored(0);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int d = 0; d < D; d += 2)
+#pragma unroll
+                    for (int part = 0; part < 3; ++part) weigh(n, d, part);
+            weighed();
+        }
+        for (int i = 1; i < rounds; ++i) {
+            scored(i);
+            outputs(i - 1, weigh);
+            rescale();
+            weighed();
+        }
+        if (rounds > 0) outputs(rounds - 1, [](auto...) {});
     }
     l = halves_sum(l);
     if (m == -INFINITY && (saw >> col & 0x0000000100000001u)) m = -FLT_MAX;   // scores, none in fp32
