@@ -29,7 +29,7 @@
 // and 3.9 for the join (75 MB, 3.8 TB/s), 64 requests as above 50.8 and 6.0 (186 MB,
 // 3.7 TB/s; the loads alone take 45, the arithmetic alone 48), eight requests of 5
 // tokens, 32 heads over 4 of 64, 9.6 and 4.8; a prompt of 1024 tokens at the end of
-// 8192 positions 239 us, 1078 TFLOP/s as issued where a large library product
+// 8192 positions 234 us, 1103 TFLOP/s as issued where a large library product
 // reaches 1154; prompts of 16 heads over 8 of 256 94 (kv4_wide).
 #include "paged_attention.h"
 
