@@ -30,7 +30,7 @@
 // 3.7 TB/s; the loads alone take 45, the arithmetic alone 48), eight requests of 5
 // tokens, 32 heads over 4 of 64, 9.6 and 4.8; a prompt of 1024 tokens at the end of
 // 8192 positions 234 us, 1103 TFLOP/s as issued where a large library product
-// reaches 1154; prompts of 16 heads over 8 of 256 94 (kv4_wide).
+// reaches 1154; prompts of 16 heads over 8 of 256 85 (kv4_wide).
 #include "paged_attention.h"
 
 namespace fy {
@@ -470,9 +470,10 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(W, kPair)) void kv4_rows(Kv4A
 // wavefronts. Heads of 256 fill the registers with one group (q and the outputs are
 // 256 of them; 16 rows per wavefront and two groups read LDS twice as often, 136 us
 // for 110), which runs its conversions and weights under its own MFMAs: prompts of up
-// to 700 tokens, 16 heads over 8, 94 us (110 with everything in turn; operands
-// requested a tile ahead 104, the codes under the scores 100). A step is 7000 cycles
-// where its MFMAs take 4100, and q, in 32 MB at once, and the outputs are 25 us at both ends.
+// to 700 tokens, 16 heads over 8, 85 us (110 with everything in turn; operands
+// requested a tile ahead 104, the codes under the scores 100, the weights under the
+// outputs 94, rows out whole 85). A step is 7000 cycles where its MFMAs take 4100;
+// q is 32 MB that all CUs read at once, 6 us.
 template <int W, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
 void kv4_wide(Kv4Attention a, Split split, int most_rows)
@@ -956,37 +957,41 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
 #pragma unroll
             for (int i = 0; i < 16; ++i) O[d][i] = O[d][i] * f0 + po[(16 * d + i) * 64] * f1;
     }
-    // Register 4 e + i of tile d is element 32 d + 16 h + 4 i + e.
-    if (row >= rq.rows) return;
-    if (g.active > 1) {
-        const Share to = split.share(c.kv_heads, x % tiles, kvh, row - kWideRows * tile, sp, W);
-#pragma unroll
-        for (int d = 0; d < D; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *(float4 *)(to.o + 32 * d + 16 * h + 4 * i) =
-                    make_float4(O[d][i], O[d][4 + i], O[d][8 + i], O[d][12 + i]);
-        if (h == 0) *to.ml = make_float2(m, l);
-        return;
-    }
-    float *out = a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W + 16 * h;
-    const float inverse = inverse_of(l, m);
-    const bool aligned = ((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0;
+    // Rows go out whole, through LDS: as they lie in registers a store would touch 32 rows (16 heads over 8 of
+    // 256: 13 us at the kernel's end). Register 4 e + i of tile d is element 32 d + 16 h + 4 i + e. A row's
+    // pieces of 16 bytes are turned by its number, so that neither side meets in a bank.
+    if (KS == 1) __syncthreads();   // the last tiles are read
+    constexpr int kPieces = W / 4, kTurn = (kPieces < 32 ? kPieces : 32) - 1, kAtOnce = 64 / (kPieces < 64 ? kPieces : 64);
+    uint8_t *const rows = &smem[0][0][0] + wave * (32 * 4 * W);
+    static_assert(sizeof(smem) >= 4 * 32 * 4 * W, "the rows fit");
+    const bool shared = g.active > 1, aligned = shared || (((uintptr_t)a.out & 15) == 0 && a.out_stride % 4 == 0);
+    const Share to = split.share(c.kv_heads, x % tiles, kvh, row - kWideRows * tile, sp, W);
+    float *const mine = shared ? to.o : a.out + (rq.begin + token) * a.out_stride + (int64_t)head * W;
+    if (shared && h == 0 && row < rq.rows) *to.ml = make_float2(m, l);
+    const float inverse = shared ? 1.f : inverse_of(l, m);
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 o = make_float4(O[d][i] * inverse, O[d][4 + i] * inverse, O[d][8 + i] * inverse,
-                                         O[d][12 + i] * inverse);
-            if (aligned) {
-                *(float4 *)(out + 32 * d + 4 * i) = o;
-            } else {
-                out[32 * d + 4 * i] = o.x;
-                out[32 * d + 4 * i + 1] = o.y;
-                out[32 * d + 4 * i + 2] = o.z;
-                out[32 * d + 4 * i + 3] = o.w;
-            }
+        for (int i = 0; i < 4; ++i)
+            *(float4 *)(rows + (col * kPieces + ((8 * d + 4 * h + i) ^ (col & kTurn))) * 16) =
+                make_float4(O[d][i] * inverse, O[d][4 + i] * inverse, O[d][8 + i] * inverse, O[d][12 + i] * inverse);
+#pragma unroll 8
+    for (int p = 0; p < 32; p += kAtOnce) {
+        const int r = p + lane / kPieces, piece = lane % kPieces;
+        const float4 o = *(const float4 *)(rows + (r * kPieces + (piece ^ (r & kTurn))) * 16);
+        const uintptr_t at = (uintptr_t)mine;
+        float *const out = (float *)((uint64_t)(uint32_t)__shfl((int)(at >> 32), r, 64) << 32 | (uint32_t)__shfl((int)at, r, 64)) +
+                           4 * piece;
+        if (kWideRows * tile + 32 * wave + r >= rq.rows) continue;
+        if (aligned) {
+            *(float4 *)out = o;
+        } else {
+            out[0] = o.x;
+            out[1] = o.y;
+            out[2] = o.z;
+            out[3] = o.w;
         }
+    }
 }
 
 // Both in one launch: `wide_blocks` workgroups of wide tiles, then those of few rows.
