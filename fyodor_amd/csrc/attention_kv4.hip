@@ -29,8 +29,8 @@
 // and 3.9 for the join (75 MB, 3.8 TB/s), 64 requests as above 50.8 and 6.0 (186 MB,
 // 3.7 TB/s; the loads alone take 45, the arithmetic alone 48), eight requests of 5
 // tokens, 32 heads over 4 of 64, 9.6 and 4.8; a prompt of 1024 tokens at the end of
-// 8192 positions 234 us, 1103 TFLOP/s as issued where a large library product
-// reaches 1154; prompts of 16 heads over 8 of 256 85 (kv4_wide).
+// 8192 positions 231 us, 1116 TFLOP/s as issued where a large library product
+// reaches 1154 (the card holds 1.47 GHz under it, 2.1 in short calls); prompts of 16 heads over 8 of 256 85 (kv4_wide).
 #include "paged_attention.h"
 
 namespace fy {
