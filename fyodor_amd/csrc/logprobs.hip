@@ -17,7 +17,7 @@
 // pass: 64 rows of 128256 17 us with 20 alternatives, 10 without.)
 //
 // Bound by reading the logits for many rows (2047 of 50257 without alternatives
-// 77 us, 5.4 TB/s; with 20 of them 99: the choice at a row's end is waits, and its LDS
+// 77 us, 5.4 TB/s; with 20 of them 94: the choice at a row's end is waits, and its LDS
 // leaves five workgroups on a CU for eight). A few rows are split into shares,
 // which a second launch joins (64 of 128256 with 20: 11.0 us and 7.2, masked 12.2 and
 // 7.4; 1 of 32000 with 5: 3.8 and 5.0): chains of waits, of which the join has four:
