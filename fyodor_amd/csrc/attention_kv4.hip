@@ -154,7 +154,7 @@ __device__ __forceinline__ void few_rows(const Kv4Attention &a, int r, const Req
     const int64_t p = rq.first + token;
     const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
-    // Pairs that all rows see: up to the first row's last, from the last row's first.
+    // Positions that all rows see: up to the first row's last, from the last row's first.
     const int64_t p0 = rq.first + kRows * tile / group, p1 = rq.first + min(kRows * tile + kRows - 1, rq.rows - 1) / group;
     const int all_to = (int)(p0 < g.highest ? p0 : g.highest);
     const int all_from = (int)(a.window && p1 >= a.window ? (p1 - a.window < g.highest ? p1 - a.window + 1 : g.highest + 1) : 0);
@@ -510,7 +510,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
     // (Rows past the request's last repeat it and are not written.)
     const int last = (int)(p < g.highest ? p : g.highest);
     const int first = (int)(a.window && p >= a.window ? (p - a.window < g.highest ? p - a.window + 1 : g.highest + 1) : 0);
-    // Pairs that all of the wavefront's rows see.
+    // Positions that all of the wavefront's rows see.
     int all_from = first, all_to = last;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {

@@ -443,6 +443,18 @@ def test_attention_strides(env, dev, counts, q_pad, out_pad, shift, heads, kv_he
     check_attention(cache, q, got, starts, lengths, table)
 
 
+@pytest.mark.parametrize("counts,window", [([150, 1, 37], 0), ([150, 1, 37], 90)])
+@pytest.mark.parametrize("q_pad,out_pad,shift", [(4, 8, 0), (1, 3, 0), (0, 0, 4), (5, 0, 12)])
+@pytest.mark.parametrize("heads,kv_heads,width", [(6, 2, 256), (3, 1, 256), (12, 4, 64), (10, 2, 128)])
+def test_attention_prompt_strides(env, dev, counts, window, q_pad, out_pad, shift, heads, kv_heads, width):
+    """Prompts whose rows end inside a tile, at any stride and alignment, holes among their pages."""
+    lengths = [250, 70, 133]
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 16, 10)
+    table[0, 3], table[2, 5] = -1, 2**30
+    got = run_attention(env, dev, cache, q, starts, lengths, table, window=window, q_pad=q_pad, out_pad=out_pad, shift=shift)
+    check_attention(cache, q, got, starts, lengths, table, window=window)
+
+
 def test_attention_rows_cut_off(env, dev):
     """starts past `count`, negative and out of order: no row outside is read or written."""
     lengths = [50, 60, 70, 80]
