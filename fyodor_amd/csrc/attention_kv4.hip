@@ -956,6 +956,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
         for (int d = 0; d < D; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) O[d][i] = O[d][i] * f0 + po[(16 * d + i) * 64] * f1;
+        lds_wave();   // rows go where other lanes read
     }
     // Rows go out whole, through LDS: as they lie in registers a store would touch 32 rows (16 heads over 8 of
     // 256: 13 us at the kernel's end). Register 4 e + i of tile d is element 32 d + 16 h + 4 i + e. A row's
@@ -975,6 +976,7 @@ void kv4_wide(Kv4Attention a, Split split, int most_rows)
         for (int i = 0; i < 4; ++i)
             *(float4 *)(rows + (col * kPieces + ((8 * d + 4 * h + i) ^ (col & kTurn))) * 16) =
                 make_float4(O[d][i] * inverse, O[d][4 + i] * inverse, O[d][8 + i] * inverse, O[d][12 + i] * inverse);
+    lds_wave();   // a row is read by other lanes than wrote it
 #pragma unroll 8
     for (int p = 0; p < 32; p += kAtOnce) {
         const int r = p + lane / kPieces, piece = lane % kPieces;

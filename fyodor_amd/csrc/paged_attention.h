@@ -146,6 +146,16 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// The same among a wavefront's lanes, where others are not waited for: what lanes wrote may be read by the
+// wavefront's others after it, and what they read overwritten. (Its LDS operations are in order, so this
+// costs nothing; it keeps the compiler from moving one before the other.)
+__device__ __forceinline__ void lds_wave()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M) over a row's shares.
 // Requests of a few rows: workgroup (place, row of a KV head).
 template <int W, class A>

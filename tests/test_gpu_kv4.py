@@ -455,6 +455,20 @@ def test_attention_prompt_strides(env, dev, counts, window, q_pad, out_pad, shif
     check_attention(cache, q, got, starts, lengths, table, window=window)
 
 
+@pytest.mark.parametrize("workspace", [None, 0])
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 64), (8, 2, 128), (4, 2, 256)])
+def test_attention_prompt_rows(env, dev, heads, kv_heads, width, workspace):
+    """Prompts in wide tiles, whole and in shares: a wavefront's lanes hand their rows to each other, so every row and
+    element of many runs of the same call has the same bits, at a stride that stores whole pieces and at one that does not."""
+    lengths, counts = [900, 165], [101, 165]
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 32, 21)
+    first = run_attention(env, dev, cache, q, starts, lengths, table, workspace=workspace)
+    check_attention(cache, q, first, starts, lengths, table)
+    for i in range(12):
+        got = run_attention(env, dev, cache, q, starts, lengths, table, workspace=workspace, out_pad=i % 2)
+        assert np.array_equal(first, got), i
+
+
 def test_attention_rows_cut_off(env, dev):
     """starts past `count`, negative and out of order: no row outside is read or written."""
     lengths = [50, 60, 70, 80]
