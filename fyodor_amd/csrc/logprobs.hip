@@ -36,6 +36,7 @@ namespace fy {
 namespace {
 
 constexpr int kMostShares = 64;
+constexpr int kSplitRows = 1024;   // from so many rows on they are whole; shares are for so many workgroups
 constexpr int kMostTop = NYA_HIP_LOGPROBS_TOP;
 static_assert(kMostTop <= 64, "a tile's 64 maxima bound its most likely");
 
@@ -625,7 +626,7 @@ Reading reading_of(int n, int count, int top, size_t bytes)
     const int all = (n + 3 + kTile - 1) / kTile;   // a row may begin 3 floats into its 16 bytes
     // Four workgroups for each CU: 64 rows of 128256, 8, 16 and 32 shares 13.0, 10.6 and 11.5 us, the join 7;
     // from 1024 rows on, whole ones (2047 of 50257 77 us, in 4 shares 85 and 5 for the join).
-    int shares = count >= 1024 ? 1 : (1024 + count - 1) / count;
+    int shares = count >= kSplitRows ? 1 : (kSplitRows + count - 1) / count;
     shares = shares < kMostShares ? shares : kMostShares;
     for (;; --shares) {
         if (shares > all) shares = all;
@@ -642,8 +643,15 @@ Reading reading_of(int n, int count, int top, size_t bytes)
 
 size_t logprobs_workspace(int n, int count, int top)
 {
-    const Reading r = reading_of(n, count, top, SIZE_MAX);
-    return r.shares == 1 ? 0 : share_bytes(r, top) * r.shares * count;
+    // Fewer rows are split into more shares, and may want more: of the counts with the same shares the largest.
+    size_t most = 0;
+    for (int shares = 1; shares <= kMostShares; ++shares) {
+        const int rows = shares == 1 || count < (kSplitRows - 1) / (shares - 1) ? count : (kSplitRows - 1) / (shares - 1);
+        const Reading r = reading_of(n, rows, top, SIZE_MAX);
+        const size_t bytes = r.shares == 1 ? 0 : share_bytes(r, top) * r.shares * rows;
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 hipError_t launch_logprobs(const Logprobs &a, void *workspace, size_t workspace_bytes, hipStream_t s)

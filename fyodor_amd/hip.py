@@ -358,7 +358,7 @@ class Kernels:
     # ---- answers (include/fyodor_hip_logprobs.h) -----------------------------
 
     def logprobs_bytes(self, n: int, count: int, top: int) -> int:
-        """The workspace with which logprobs splits the rows as it wants to."""
+        """The workspace with which logprobs splits the rows as it wants to: up to `count` of them, up to `top`."""
         b = _sz()
         if self.lib.nya_hip_logprobs_bytes(n, count, top, ctypes.byref(b)):
             raise ValueError("request unsupported")

@@ -40,8 +40,11 @@ extern "C" {
  * n <= 2^24, count <= 2^22. Outputs overlap neither each other nor an input.
  * `workspace` (16-byte aligned) is scratch for rows that are split over several
  * workgroups (nothing in it is kept, nor has to be cleared): with less than
- * nya_hip_logprobs_bytes says, or none, the call runs with fewer of them, and
- * slower. Calls that may overlap in time need workspaces of their own. */
+ * nya_hip_logprobs_bytes says, or none, the call may run with fewer of them, and
+ * slower. What it says is enough for every call of up to `count` rows of n with up
+ * to `top` alternatives (few rows are split and many are not, so it is not what a
+ * call of `count` rows takes). Calls that may overlap in time need workspaces of
+ * their own. */
 NYA_HIP_EXPORT int nya_hip_logprobs_bytes(size_t n, size_t count, size_t top, size_t *bytes);
 NYA_HIP_EXPORT int nya_hip_logprobs(uintptr_t logits, size_t stride, size_t n, size_t count, uintptr_t mask, float scale,
     uintptr_t tokens, uintptr_t logprobs, uintptr_t ranks, uintptr_t entropies, size_t top, uintptr_t top_ids,

@@ -115,6 +115,19 @@ def test_logprobs_refusals(kernels):
     assert kernels.lib.nya_hip_logprobs_bytes(9, 7, 5, None) == 1
 
 
+@pytest.mark.parametrize("n", [1, 984, 2046, 2047, 32000, 50257, 128256, 131070, 262147, 1 << 24])
+def test_logprobs_scratch_of_the_largest_batch(kernels, n):
+    """Scratch for the largest batch and the most alternatives is what every smaller one wants."""
+    said = {(rows, top): kernels.logprobs_bytes(n, rows, top) for rows in range(1, 1100) for top in (0, 1, 64)}
+    for top in (0, 1, 64):
+        sizes = [said[rows, top] for rows in range(1, 1100)]
+        assert sizes == sorted(sizes)
+        assert kernels.logprobs_bytes(n, 1 << 22, top) == sizes[-1] <= 20 << 20
+    assert all(said[rows, 0] <= said[rows, 1] == said[rows, 64] for rows in range(1, 1100))
+    # Rows longer than a tile of 2048 are split while there are few.
+    assert (said[1, 0] > 0) == (n > 2045)
+
+
 def test_steps():
     """Steps by hand: 8 bits, ties to even, the negative one of two extremes, the ends."""
     def block(*x):
