@@ -20,11 +20,14 @@ extern "C" {
  * of the largest magnitude (of -m and m: -m), d = m / -8, rounded to 8 bits
  * (ties to even), its magnitude at most 8160, then to fp16;
  * n = round(x / d) + 8 (ties to even) within 0 .. 15, and 8 where d is 0. So
- * an element is off by half a step, by one where it is next to 8 |d| on m's
- * other side; magnitudes from 65280 on are held as that, and blocks below
- * 2^-22 as zeros. With 8 bits in the step (n - 8) d is an fp16 number: what
- * attention multiplies is exactly what is held. No position changes when
- * another one is stored, so rows may come in any order.
+ * an element is off by up to half a step, a sixteenth of |m|, and on m's other
+ * side, where 7 |d| is the most there is, by up to 33/32 of one, an eighth of |m|.
+ * Magnitudes from 65280 on are held as that on m's side, as 57120 on the other.
+ * In blocks below 2^-14 the step is an fp16 number of fewer bits, which adds up to
+ * 2^-22 to both; those whose m is no more than 2^-22 (in 8 bits) are zeros.
+ * With 8 bits in the step (n - 8) d is an fp16 number: what attention multiplies
+ * is exactly what is held. No position changes when another one is stored, so rows
+ * may come in any order.
  *
  * Heads of 64, 128, 256 or 512. The codes of a page and head, page_tokens *
  * width / 2 bytes at (page * kv_heads + head) times that, are laid out for the

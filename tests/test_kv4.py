@@ -156,6 +156,33 @@ def test_quantised(size):
     assert np.mean((off <= np.abs(d) * (0.5 + 8 * 2.0 ** -8) + 8 * 2.0 ** -25)[inside]) > 0.95
 
 
+@pytest.mark.parametrize("exponent", [*range(-26, -9), -3, 0, 5, 14, 15, 16, 20, 60])
+def test_off_by_as_declared(exponent):
+    """How far what is held may be off, as the header says it, and that it is held the same when stored again. With m
+    the largest magnitude, d0 = m / -8 and |d - d0| <= 2^-8 |d0|, in fp16's subnormals 2^-25 more: codes -8 .. 7 leave
+    half a step or, past -8 steps, |m| - 8 |d| <= |d| / 32 (1 + 2^-7) + 2^-22; past 7 steps |m| - 7 |d|, one step more
+    than that. (A 32nd of a step rounds to (1 + 2^-7) of it; zeros are off by |m| <= 2^-22 (1 + 2^-8).)"""
+    rng = np.random.default_rng(exponent + 100)
+    x = rng.standard_normal((2000, BLOCK))
+    x[::3, 3] = -x[::3, 7] * (1 - rng.random(667) / 16)   # near -m, in some of them
+    x[::3, 7] = np.abs(x[::3]).max(1) * np.sign(x[::3, 7])
+    x = (x / np.abs(x).max(1, keepdims=True) * 2.0 ** (exponent + rng.random((2000, 1)))).astype(np.float32)
+    codes, steps = quantised(x)
+    d, y = steps.astype(np.float64), x.astype(np.float64)
+    got = (codes.astype(np.float64) - 8) * d
+    other = y * d > 0                                     # (m's own side has d's other sign)
+    y = np.where(other, np.clip(y, -57120, 57120), np.clip(y, -65280, 65280))
+    m = np.abs(x).max(1, keepdims=True)
+    more = np.where(m < 2.0 ** -14, 2.0 ** -22 * (1 + 2.0 ** -8), 0)
+    bound = np.abs(d) * np.where(other, 1 + (1 + 2.0 ** -7) / 32, 0.5) + more
+    assert np.all(np.abs(got - y) <= bound)
+    assert np.all(bound[(m >= 2.0 ** -14).ravel()] <= (m / np.where(other, 7.5, 15.8))[(m >= 2.0 ** -14).ravel()])
+    assert not got[(m <= 2.0 ** -22).ravel()].any()
+    again = quantised(got.astype(np.float32))
+    whole = (m >= 2.0 ** -14).ravel()
+    assert np.array_equal(again[0][whole], codes[whole]) and np.array_equal(again[1][whole], steps[whole])
+
+
 @pytest.mark.parametrize("page_tokens,width", [(16, 64), (32, 128), (128, 256), (64, 512)])
 def test_layout(page_tokens, width):
     """Every nibble and every step has its own place, and the statement stores and reads back."""
