@@ -684,6 +684,22 @@ def test_logprobs_rows(env, dev, rows, n):
                 check_logprobs(got, x[part], m, 1.0, tokens[part], top)
 
 
+@pytest.mark.parametrize("rows,n,top", [(6, 3001, 20), (3, 40000, 64), (1100, 2500, 5)])
+@pytest.mark.parametrize("exponent", [-20, -11, 7, 20])
+@pytest.mark.parametrize("spread", [0.01, 1.0, 40.0])
+def test_logprobs_scales(env, dev, rows, n, top, exponent, spread):
+    """The scales that the header allows, to both ends, on logits that they bring to nearly equal ones, to ordinary ones
+    and to a few likely ones; logits of the ends of fp32 and ordinary ones under the same scale."""
+    scale = 2.0 ** exponent * (1 if abs(exponent) == 20 else 1.1)
+    x, mask, tokens = logits_of(rows, n, exponent + 40)
+    x *= np.float32(spread / scale)
+    x[rows // 2] = 2.5 * np.random.default_rng(1).standard_normal(n)
+    x[rows - 1] = np.where(np.arange(n) % 3, np.float32(3e38), np.float32(-3e38))
+    for m in (None, mask):
+        got = run_logprobs(env, dev, x, m, scale, tokens, top)
+        check_logprobs(got, x, m, scale, tokens, top)
+
+
 def test_logprobs_parts(env, dev):
     """Some of the results only; rank 0 is the greedy choice."""
     rt, kern, stream = env
