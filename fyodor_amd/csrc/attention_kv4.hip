@@ -28,9 +28,11 @@
 // Measured, 32 heads over 8 of 128 unless said: one token of 65536 positions 19.9 us
 // and 3.9 for the join (75 MB, 3.8 TB/s), 64 requests as above 50.8 and 6.0 (186 MB,
 // 3.7 TB/s; the loads alone take 45, the arithmetic alone 48), eight requests of 5
-// tokens, 32 heads over 4 of 64, 9.6 and 4.8; a prompt of 1024 tokens at the end of
-// 8192 positions 231 us, 1116 TFLOP/s as issued where a large library product
-// reaches 1154 (the card holds 1.47 GHz under it, 2.1 in short calls); prompts of 16 heads over 8 of 256 85 (kv4_wide).
+// tokens, 32 heads over 4 of 64, 9.6 and 4.8; prompts of 16 heads over 8 of 256 85
+// (kv4_wide). A prompt of 1024 tokens at the end of 8192 positions goes by the clock
+// that the card's power leaves it, 1.6 to 1.9 GHz: 231 us in a few passes among
+// others', 241 to 251 in 200 in a row, 269 to 284 in 20; 905 to 1116 TFLOP/s as issued,
+// a library product of 8192^3 in such runs 1080 to 1320.
 #include "paged_attention.h"
 
 namespace fy {
@@ -472,8 +474,11 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(W, kPair)) void kv4_rows(Kv4A
 // for 110), which runs its conversions and weights under its own MFMAs: prompts of up
 // to 700 tokens, 16 heads over 8, 85 us (110 with everything in turn; operands
 // requested a tile ahead 104, the codes under the scores 100, the weights under the
-// outputs 94, rows out whole 85). A step is 7000 cycles where its MFMAs take 4100;
-// q is 32 MB that all CUs read at once, 6 us.
+// outputs 94, rows out whole 85). Of the 85 tables take 3, q 5 (32 MB that all CUs
+// read at once), 18 steps 68, their last outputs and the rows 6. A step is 7900
+// cycles: the scores 2930 and the outputs 2190, whose MFMAs are 2050 each, codes that
+// are waited for and masked 630, the next ones' addresses 580, the maximum 730,
+// rescaling 510, sums and the barrier 310.
 template <int W, int KS>
 __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(KS, KS)))
 void kv4_wide(Kv4Attention a, Split split, int most_rows)
