@@ -101,45 +101,46 @@ struct List {
 };
 
 // Leaves, of more keys than are worth comparing with each other (634 rows of 984, 33 of them: 34 us without
-// this, 13 with it), the ones above a bound that at
-// least `top` of them reach and few more do (all, if they are of one logit): as bound_of, with
-// every thread's keys in registers.
+// this, 13 with it), the ones above a bound that at least `top` of them reach and few more do: as bound_of, with
+// every thread's keys in registers, and their ids where logits are equal.
 __device__ void narrow(List &list, int top)
 {
     constexpr int kEach = (kRoom + kThreads - 1) / kThreads;
     const int n = list.n, tid = threadIdx.x, wave = tid >> 6;
     uint64_t key[kEach];
-    uint32_t from = ~0u, to = 0;
+    uint32_t least = ~0u, most = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         const int k = tid + i * kThreads;
         key[i] = k < n ? list.keys[k] : 0;
         const uint32_t o = (uint32_t)(key[i] >> 32);
-        if (key[i]) from = min(from, o);
-        to = max(to, o);
+        if (key[i]) least = min(least, o);
+        most = max(most, o);
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
-        from = min(from, (uint32_t)__shfl_xor((int)from, d, 64));
-        to = max(to, (uint32_t)__shfl_xor((int)to, d, 64));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+        most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
     }
     if ((tid & 63) == 0) {
-        list.reach[0][wave] = from;
-        list.reach[1][wave] = to;
+        list.reach[0][wave] = least;
+        list.reach[1][wave] = most;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kThreads / 64; ++w) {
-        from = min(from, list.reach[0][w]);
-        to = max(to, list.reach[1][w]);
+        least = min(least, list.reach[0][w]);
+        most = max(most, list.reach[1][w]);
     }
     __syncthreads();
-    for (int turn = 0; to > from + 1 && turn < 32; ++turn) {
-        const uint32_t middle = from + (to - from) / 2;
+    // (Ids are below 2^31, so keys above that of the last one.)
+    uint64_t from = (uint64_t)least << 32 | 0x80000000u, to = (uint64_t)most << 32 | 0xFFFFFFFFu;
+    for (int turn = 0; to > from + 1 && turn < 64; ++turn) {
+        const uint64_t middle = from + (to - from) / 2;
         int mine = 0, reach = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64((uint32_t)(key[i] >> 32) >= middle));
+            mine += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[i] >= middle));
         if ((tid & 63) == 0) list.reach[turn & 1][wave] = mine;
         __syncthreads();   // (the other half is written next: one wait a turn)
 #pragma unroll
@@ -156,7 +157,7 @@ __device__ void narrow(List &list, int top)
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-        if (key[i] && (uint32_t)(key[i] >> 32) >= from) list.keys[atomicAdd(&list.n, 1u)] = key[i];
+        if (key[i] >= from) list.keys[atomicAdd(&list.n, 1u)] = key[i];
     __syncthreads();
 }
 
@@ -200,7 +201,8 @@ __device__ int settle(List &list, int top)
 }
 
 // A bound that at least `top` of the 256 maxima reach and not many more, by halving the range
-// between the least and the largest, in their order as whole numbers.
+// between the least and the largest, in their order as whole numbers; one of the maxima, where too
+// many are equal.
 __device__ __forceinline__ float bound_of(const List &list, int top)
 {
     const int lane = threadIdx.x & 63;
@@ -214,8 +216,8 @@ __device__ __forceinline__ float bound_of(const List &list, int top)
         high = i ? fmaxf(high, v) : v;
     }
     // Minus infinity is no token.
-    uint32_t from = ordered(fmaxf(-wave_reduce<true>(-low), -FLT_MAX)), to = ordered(wave_reduce<true>(high));
-    for (int k = 0; k < 24 && to > from + 1; ++k) {
+    uint32_t from = ordered(fmaxf(-wave_reduce<true>(-low), -FLT_MAX)), to = ordered(wave_reduce<true>(high)) + 1;
+    for (int k = 0; k < 32 && to > from + 1; ++k) {
         const uint32_t middle = from + (to - from) / 2;
         int reach = 0;
 #pragma unroll
@@ -276,6 +278,49 @@ struct Maxima {
 };
 static_assert(4 * kThreads * Maxima::kChunks >= kMostGroups, "every group of a row");
 
+// Lists the groups of a row anew where too many reach the bound, as they do in a row of equal logits (a batch's
+// padding: with all of its groups gone through, 64 rows of 128256 with 20 alternatives, half of them zeros,
+// took 306 us, so 33): those above it, and of those with just it the first sets' until there are `top`. A set's ids
+// are below the next one's, so no other group has a token that comes as early.
+__device__ void list_first(List &list, int top, float from, bool wide, const Maxima &mine)
+{
+    static_assert(kMostGroups / 64 <= 64, "a lane each");
+    unsigned *equal = (unsigned *)list.next;   // groups of a set whose maximum is the bound
+    const int tid = threadIdx.x, lane = tid & 63;
+    __syncthreads();   // the count is read
+    if (tid < 64) equal[tid] = 0;
+    if (tid == 0) list.listed = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Maxima::kChunks; ++i) {
+        const float v[4] = {mine.v[i].x, mine.v[i].y, mine.v[i].z, mine.v[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (v[e] == from) atomicAdd(&equal[Maxima::number(wide, i, e) / 64], 1u);
+    }
+    __syncthreads();
+    int sum = (int)equal[lane];
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int v = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += v;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sum >= top);
+    const int end = past ? 64 * (__builtin_ctzll(past) + 1) : kMostGroups;
+#pragma unroll
+    for (int i = 0; i < Maxima::kChunks; ++i) {
+        const float v[4] = {mine.v[i].x, mine.v[i].y, mine.v[i].z, mine.v[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int g = Maxima::number(wide, i, e);
+            if (!(v[e] > from || (v[e] == from && g < end))) continue;
+            const unsigned at = atomicAdd(&list.listed, 1u);
+            if (at < (unsigned)kListed) list.groups[at] = g;
+        }
+    }
+    __syncthreads();
+}
+
 // The first `top` tokens of a row, in order, from its groups' maxima (a thread's are `mine`); how many
 // there are. `beside` is done by the second wavefront, while the first looks for the bound.
 template <class F>
@@ -295,8 +340,8 @@ __device__ __forceinline__ int choose(const Logprobs &a, int row, int shift, con
     }
     __syncthreads();
     const float from = list.bound;
+    const bool wide = Maxima::wide(groups);
     if (most >= from) {
-        const bool wide = Maxima::wide(groups);
         unsigned n = 0;
 #pragma unroll
         for (int i = 0; i < Maxima::kChunks; ++i)
@@ -316,7 +361,8 @@ __device__ __forceinline__ int choose(const Logprobs &a, int row, int shift, con
         }
     }
     __syncthreads();
-    // (More groups than are listed, of many equal logits: all of them are gone through.)
+    if (list.listed > (unsigned)kListed) list_first(list, top, from, wide, mine);
+    // (More groups than are listed all the same: all of them are gone through.)
     const bool all = list.listed > (unsigned)kListed;
     const int n = all ? groups : (int)list.listed;
     const float *x = a.logits + row * a.stride;

@@ -3,6 +3,7 @@ against their statements in kv4_check.py, at the sizes and data where they can g
 are exact; rotated rows are one rounding from 64 bits; attention stays in the bound that attention_bound derives, log
 probabilities in the one that logprobs derives."""
 import ctypes
+import time
 
 import numpy as np
 import pytest
@@ -698,6 +699,57 @@ def test_logprobs_scales(env, dev, rows, n, top, exponent, spread):
     for m in (None, mask):
         got = run_logprobs(env, dev, x, m, scale, tokens, top)
         check_logprobs(got, x, m, scale, tokens, top)
+
+
+@pytest.mark.parametrize("n,shift", [(32000, 0), (128257, 8), (262147, 4)])
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_logprobs_equal(env, dev, n, shift, top):
+    """Rows in which more groups of logits reach the bound than are listed: zeros (a batch's padding), few values,
+    equal ones above or below the others, in the last tokens only, after larger ones that are few or many."""
+    rng = np.random.default_rng(n)
+    x, mask, tokens = logits_of(9, n, 7)
+    x[0] = 0
+    x[1] = np.where(np.arange(n) % 2, np.float32(-1), np.float32(0))
+    x[2] = rng.integers(0, 3, n)
+    x[3] = np.minimum(x[3], 0)
+    x[4] = np.where(np.arange(n) < n - 30, np.float32(1), np.float32(2))
+    x[5] = 0
+    x[5, rng.permutation(n)[:7]] = 3
+    x[6] = 0
+    x[6, rng.permutation(n)[:700]] = rng.permutation(700) + 1
+    x[7] = np.where(np.arange(n) < n // 2, -np.inf, np.float32(-3e38))
+    x[8] = np.where(np.arange(n) // 16 % 64 < 9, np.float32(5), x[8] - 40)   # in the same groups of every set
+    tokens[:4] = n - 1, 1, n // 2, 0
+    for m in (None, mask):
+        for workspace in (None, 0):
+            got = run_logprobs(env, dev, x, m, 1.0, tokens, top, shift=shift, workspace=workspace)
+            check_logprobs(got, x, m, 1.0, tokens, top)
+
+
+def test_logprobs_padding_costs_little(env, dev):
+    """Rows of zeros that pad a batch are no slower than rows of logits, but for the choice among equal ones (12 times
+    as slow with every group gone through)."""
+    rt, kern, stream = env
+    rows, n, top = 64, 128256, 20
+    x = logits_of(rows, n, 3)[0]
+    size = kern.logprobs_bytes(n, rows, top)
+    scratch, ids, lp = dev.put(np.zeros(size, np.uint8)), dev.put(np.zeros(rows * top, np.int32)), dev.put(
+        np.zeros(rows * top, np.float32))
+
+    def best(x):
+        at, least = dev.put(x), np.inf
+        for _ in range(6):
+            rt.sync(stream)
+            begin = time.perf_counter()
+            for _ in range(50):
+                kern.logprobs(at, n, n, rows, 0, 1.0, 0, 0, 0, 0, top, ids, lp, scratch, size, stream)
+            rt.sync(stream)
+            least = min(least, time.perf_counter() - begin)
+        return least
+
+    whole = best(x)
+    x[rows // 2:] = 0
+    assert best(x) < 5 * whole
 
 
 def test_logprobs_parts(env, dev):
