@@ -726,6 +726,34 @@ def test_logprobs_equal(env, dev, n, shift, top):
             check_logprobs(got, x, m, 1.0, tokens, top)
 
 
+@pytest.mark.parametrize("shift,workspace", [(0, None), (4, None), (0, 0)])
+def test_logprobs_longest_row(env, dev, shift, workspace):
+    """2^24 logits: whole numbers in a known order (ranks to the last one, exact counts), and all equal."""
+    n, top = 1 << 24, 64
+    order = (np.arange(n) * 0x9E3779B1 + 12345) % n            # the rank of each id (an odd factor: each once)
+    first = np.empty(n, np.int64)
+    first[order] = np.arange(n)
+    x = np.stack([(-order).astype(np.float32), np.full(n, 2.5, np.float32)])
+    for token in (int(first[-1]), int(first[0]), n - 1):
+        tokens = [token, token]
+        lp, ranks, entropy, ids, top_lp = run_logprobs(env, dev, x, None, 2.0 ** -20, tokens, top, shift=shift,
+                                                       workspace=workspace)
+        assert ranks.tolist() == [order[token], token]
+        assert np.array_equal(ids[0], first[:top]) and np.array_equal(ids[1], np.arange(top))
+        w = np.arange(n) * 2.0 ** -20
+        p = np.exp(-w)
+        lse, p = np.log(p.sum()), p / p.sum()
+        # As in kv4_check.logprobs.
+        chain = n / 256 + 64 + 16
+        each = (p * (3 * w + 4 + chain)).sum() * F32_HALF + n * 2.0 ** -126
+        assert abs(lp[0] - (-w[order[token]] - lse)) <= each + abs(lp[0]) * F32_HALF * (1 + 1e-6)
+        assert abs(entropy[0] - (lse + (p * w).sum())) <= each + (p * w * (3 * w + 8 + chain)).sum() * F32_HALF + (
+            p * w).sum() * each + abs(entropy[0]) * F32_HALF * (1 + 1e-6)
+        # Nothing but the maximum, which is counted: the logarithm, rounded once.
+        assert lp[1] == np.float32(-24 * np.log(2)) and entropy[1] == np.float32(24 * np.log(2))
+        assert np.all(top_lp[1] == np.float32(-24 * np.log(2)))
+
+
 def test_logprobs_padding_costs_little(env, dev):
     """Rows of zeros that pad a batch are no slower than rows of logits, but for the choice among equal ones (12 times
     as slow with every group gone through)."""
