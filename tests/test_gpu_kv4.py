@@ -117,6 +117,33 @@ def test_store(env, dev, page_tokens, kv_heads, width, heads, rotated, halves, s
     step([(0, p) for p in range(5, 29)])
 
 
+@pytest.mark.parametrize("width,rotated,halves,shift,pad", [(64, 64, False, 0, 0), (128, 64, True, 0, 4),
+                                                            (256, 38, True, 4, 1), (512, 512, False, 8, 0)])
+def test_store_in_place(env, dev, width, rotated, halves, shift, pad):
+    """q rotated where it is, beside the k and v of the same rows, which stay; rows that go nowhere are rotated too."""
+    rt, kern, stream = env
+    rng = np.random.default_rng(width)
+    heads, kv_heads, count = 5, 2, 90
+    cache = DeviceCache4(env, dev, 4, 32, kv_heads, width, rng)
+    n = (heads + 2 * kv_heads) * width
+    rows = rng.standard_normal((count, n + pad)).astype(np.float32)
+    x = rows[:, :n].reshape(count, -1, width)
+    slots = rng.permutation(4 * 32)[:count].astype(np.int32)
+    slots[[3, 50, count - 1]] = -1
+    angles = angles_of(np.arange(count), env[1].rope_frequencies(rotated, 10000.0)[0], 1.0).astype(np.float32)
+    src = dev.put(rows, shift)
+    kern.kv4_store(cache.arg, dev.put(slots), count, src + 4 * heads * width, n + pad, src + 4 * (heads + kv_heads) * width,
+                   n + pad, dev.put(angles), rotated, int(halves), src, n + pad, src, n + pad, heads, stream)
+    rt.sync(stream)
+    got = dev.get(src, rows)
+    assert np.array_equal(got[:, heads * width:], rows[:, heads * width:])
+    want = rotate(x[:, :heads], angles, halves).reshape(count, -1)
+    assert np.all(np.abs(got[:, :heads * width] - want) <= np.abs(want) * F32_HALF * (1 + 1e-6) + 2.0 ** -149)
+    store(cache.k, cache.v, slots, rotate(x[:, heads:heads + kv_heads], angles, halves).astype(np.float32),
+          x[:, heads + kv_heads:])
+    cache.check()
+
+
 def test_store_values(env, dev):
     """Extremes that tie, quotients next to and on borders, steps at both ends, blocks of zeros, what is not finite."""
     rng = np.random.default_rng(3)
@@ -533,6 +560,28 @@ def test_attention_ragged_split(env, dev, heads, kv_heads, width, tokens):
     for workspace in (size, size // 2 & ~15):
         got = run_attention(env, dev, cache, q, starts, lengths, table, longest=9000, workspace=workspace)
         check_attention(cache, q, got, starts, lengths, table)
+
+
+@pytest.mark.parametrize("heads,kv_heads,width", [(8, 2, 128), (4, 2, 64), (4, 2, 256), (2, 1, 512)])
+@pytest.mark.parametrize("counts", [[1, 1], [150, 3]])
+def test_attention_common_rows(env, dev, heads, kv_heads, width, counts):
+    """q and out as columns of the same rows, with others between them that stay."""
+    rt, kern, stream = env
+    lengths = [300, 171]
+    cache, q, starts, table = make_attention(env, dev, lengths, counts, heads, kv_heads, width, 32, 17)
+    n, gap, rows = heads * width, 8, len(q)
+    both = np.full((rows, 2 * n + gap), 0.25, np.float32)
+    both[:, n + gap:] = q.reshape(rows, n)
+    at = dev.put(both)
+    size = kern.kv4_attention_bytes(cache.arg, rows, 2, max(counts), 300, heads, 0)
+    scratch = dev.put(np.full(max(size, 16), 0xFF, np.uint8))
+    kern.kv4_attention(cache.arg, at + 4 * (n + gap), 2 * n + gap, at, 2 * n + gap, rows, dev.put(starts),
+                       dev.put(np.array(lengths, np.int32)), dev.put(table), table.shape[1], 2, max(counts), 300, heads, 0,
+                       width ** -0.5, scratch, size, stream)
+    rt.sync(stream)
+    got = dev.get(at, both)
+    assert np.array_equal(got[:, n:], both[:, n:])
+    check_attention(cache, q, got[:, :n].reshape(rows, heads, width), starts, lengths, table)
 
 
 def test_attention_scales(env, dev):
