@@ -98,6 +98,7 @@ struct List {
     int groups[kListed];
     uint32_t reach[2][kThreads / 64];
     unsigned n, listed;
+    unsigned equal[kMostGroups / 64];   // groups of each set whose maximum is the bound
 };
 
 // Leaves, of more keys than are worth comparing with each other (634 rows of 984, 33 of them: 34 us without
@@ -284,11 +285,10 @@ static_assert(4 * kThreads * Maxima::kChunks >= kMostGroups, "every group of a r
 // are below the next one's, so no other group has a token that comes as early.
 __device__ void list_first(List &list, int top, float from, bool wide, const Maxima &mine)
 {
-    static_assert(kMostGroups / 64 <= 64, "a lane each");
-    unsigned *equal = (unsigned *)list.next;   // groups of a set whose maximum is the bound
+    static_assert(kMostGroups / 64 == 64, "a lane each");
     const int tid = threadIdx.x, lane = tid & 63;
     __syncthreads();   // the count is read
-    if (tid < 64) equal[tid] = 0;
+    if (tid < 64) list.equal[tid] = 0;
     if (tid == 0) list.listed = 0;
     __syncthreads();
 #pragma unroll
@@ -296,10 +296,10 @@ __device__ void list_first(List &list, int top, float from, bool wide, const Max
         const float v[4] = {mine.v[i].x, mine.v[i].y, mine.v[i].z, mine.v[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (v[e] == from) atomicAdd(&equal[Maxima::number(wide, i, e) / 64], 1u);
+            if (v[e] == from) atomicAdd(&list.equal[Maxima::number(wide, i, e) / 64], 1u);
     }
     __syncthreads();
-    int sum = (int)equal[lane];
+    int sum = (int)list.equal[lane];
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
         const int v = __shfl_up(sum, o, 64);

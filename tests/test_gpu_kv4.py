@@ -804,7 +804,7 @@ def test_logprobs_longest_row(env, dev, shift, workspace):
 
 
 def test_logprobs_padding_costs_little(env, dev):
-    """Rows of zeros that pad a batch are no slower than rows of logits, but for the choice among equal ones (12 times
+    """Rows of zeros that pad a batch are no slower than rows of logits, but for the choice among equal ones (17 times
     as slow with every group gone through)."""
     rt, kern, stream = env
     rows, n, top = 64, 128256, 20
